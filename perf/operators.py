@@ -23,7 +23,7 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 SIZE = {"bf16": 2, "fp16": 2, "fp32": 4}
 BLK = 128
 E4M3_MAX = 448.0
-TINY = 2.0 ** -126            # the smallest scale: a block of zeros has it
+TINY = 2.0 ** -80             # the smallest scale: a block of zeros has it
 
 
 def _route(name, M, E, topk, scoring="softmax", groups=1, kept=1, bias=False, renorm=True, scale=1.0, masked=0,
