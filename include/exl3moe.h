@@ -360,6 +360,38 @@ int exl3_copy_batch(void* const* dst, const void* const* src, const int64_t* nby
 int exl3_table_update(int64_t* ptrs_all, int32_t* slot_of, int32_t* slot_key, int32_t* slot_last, const int64_t* rec,
                       int64_t n, void* stream);
 
+/* ---- routing, and the 8-bit float linear (none of these has a counterpart in the reference's op libraries) ---------- */
+
+/* The picks of every row of router logits and their weights, as exl3_moe_forward takes them. logits: [M, E], dtype
+ * EXL3_DT_*, `stride` elements between rows. scoring 0: softmax, 1: sigmoid. bias: fp32 [E] or NULL, added to the scores
+ * for the choice alone. E / n_group neighbouring experts form a group, and only the experts of the topk_group best groups
+ * compete (by their largest score; with a bias, by the sum of their two largest). Picks come in descending order of what
+ * they are chosen by, equal ones by index; a NaN counts as the largest. w: the picks' scores, over their sum with
+ * renormalize (0 where that sum is 0: a row of -inf), times scale. The ids of a row are always topk different experts.
+ * 1 <= E <= 1024, topk <= 64 and <= topk_group * E / n_group, n_group <= 64 and a divisor of E. ids int32, w fp32 [M, topk]. */
+int exl3_moe_route(const void* logits, int dtype, int64_t stride, int M, int E, const float* bias, int topk, int scoring,
+                   int n_group, int topk_group, int renormalize, float scale, int32_t* ids, float* w, void* stream);
+
+/* Rows of 8-bit floats (e4m3, OCP) with one fp32 scale per 128 columns: s = max(amax / 448, 2^-80), q = x / s rounded to
+ * the nearest, halves to even (scale and quotient are rounded to 32 bits first). kp = k rounded up to 128. x: [M, k] of
+ * x_dtype with x_stride elements between rows; q: [M, kp], zeros behind column k; s: fp32 [M, kp / 128]. An infinite or
+ * NaN element makes its block's scale infinite or NaN. */
+int exl3_fp8_quant(const void* x, int x_dtype, int64_t x_stride, int M, int k, void* q, float* s, void* stream);
+/* the same of silu(gate) * up (in fp32) of gate|up rows [M, 2 k] */
+int exl3_fp8_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int M, int k, void* q, float* s, void* stream);
+/* out[m][n] = sum over blocks b of s[m][b] sw[n / 128][b] (sum over k in b of q[m][k] w[n][k]) + bias[n], fp32 sums, rounded
+ * once to out_dtype. q, s as above; w: e4m3 [n, kp], zeros behind column k; sw: fp32 [ceil(n / 128), kp / 128]; bias: fp32
+ * [n] or NULL; q and w start on 16 bytes. workspace: exl3_fp8_matmul_workspace bytes, no state between calls; its size
+ * never falls as M grows. */
+size_t exl3_fp8_matmul_workspace(int M, int k, int n);
+int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
+                    void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+/* the same of x [M, k], quantised within the call */
+size_t exl3_fp8_linear_workspace(int M, int k, int n);
+int exl3_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const float* sw,
+                    const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -236,4 +236,36 @@ static inline size_t decode_exchange_words(int npairs, int H, int I) {
            (size_t)npairs * (H / 128);
 }
 
+// moe_route.hip: the picks of every row of router logits and their weights
+constexpr int kRouteMaxTopk = 64;   // one pick per lane
+constexpr int kRouteMaxGroups = 64;
+struct RouteArgs {
+    const void* logits; int64_t stride;            // [M, E] with `stride` elements between rows
+    const float* bias;                             // [E] or null
+    int M, E, topk, sigmoid, n_group, topk_group, renormalize;
+    float scale;
+    int32_t* ids; float* w;                        // [M, topk]
+};
+hipError_t launch_route(const RouteArgs& a, int dtype, hipStream_t s);
+
+// The 8-bit float linear: rows in e4m3 with one fp32 scale per 128 columns, weights in e4m3 with one per 128 x 128 block
+constexpr int kFp8Block = 128;
+static inline int fp8_blocks(int n) { return n / kFp8Block + (n % kFp8Block != 0); }
+// fp8_rows.hip. silu: x holds gate|up rows of 2 k values and the rows written are silu(gate) * up
+struct Fp8RowsArgs {
+    const void* x; int64_t x_stride;
+    int M, k;
+    uint8_t* q; float* s;                          // [M, 128 ceil(k / 128)] (zeros behind k), [M, ceil(k / 128)]
+};
+hipError_t launch_fp8_rows(const Fp8RowsArgs& a, int x_dt, bool silu, hipStream_t st);
+// fp8_linear.hip: out[m][n] = sum_b s[m][b] sw[n / 128][b] sum_(k in b) q[m][k] w[n][k] + bias[n]
+struct Fp8ProductArgs {
+    const uint8_t* q; const float* s;              // as above, kb = ceil(k / 128) blocks
+    const uint8_t* w; const float* sw;             // [n, 128 kb], [ceil(n / 128), kb]
+    const float* bias;                             // [n] or null
+    int M, n, kb;
+    void* out; int64_t out_stride;
+};
+hipError_t launch_fp8_product(const Fp8ProductArgs& a, int out_dt, hipStream_t st);
+
 }  // namespace exl3

@@ -1,0 +1,88 @@
+// Rows to e4m3 with one fp32 scale per 128 columns: s = max(amax / 448, 2^-80), q = e4m3(x / s), where s and the quotient
+// are rounded to 32 bits (as a division does) and the quotient to the nearest e4m3 value, halves to even.
+//
+// 448 is e4m3's largest value, so nothing saturates (the quotient of the largest element is 448 or its neighbour, which
+// rounds to 448). The floor keeps every step of the division exact in 32 bits; a block below 448 * 2^-80 loses precision
+// down to 0. An infinite or NaN element makes its block's scale infinite or NaN, and with it the row of a product.
+#pragma once
+#include "exl3_common.cuh"
+
+namespace exl3 {
+
+constexpr float kE4m3Max = 448.0f;
+constexpr float kFp8MinScale = 0x1p-80f;
+
+// |x| as an integer: ordered as the magnitudes are, NaN above infinity, so that the largest is the block's amax
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+
+__device__ __forceinline__ float fp8_scale(uint32_t amax_bits) {
+    const float s = __builtin_bit_cast(float, amax_bits) / kE4m3Max;
+    return s < kFp8MinScale ? kFp8MinScale : s;
+}
+
+// x / s for the elements of one block, correctly rounded: with inv the rounded 1 / s, q0 = x inv is within one unit of the
+// quotient, x - q0 s is exact in a multiply-add, and adding its share to q0 rounds once. (|x| >= 2^-10 s: below that both
+// give values that round to 0.) An infinite or NaN scale leaves q0: 0 for finite x, NaN else.
+struct Fp8Div {
+    float s, inv;
+    __device__ __forceinline__ explicit Fp8Div(float scale) {
+        inv = 1.0f / scale;
+        s = abs_bits(scale) < 0x7F800000u ? scale : 0.0f;
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        const float q = x * inv;
+        return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
+    }
+};
+
+// four values as e4m3, the first in the low byte
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+}
+
+// silu(g) * u = g u / (1 + exp(-g)). exp(-g) = 2^t (1 + e ln 2) with t = -g log2(e) rounded and e what the rounding lost, on
+// the hardware's exp2 and reciprocal: about 3 units in the last place. g = +-inf has no e.
+__device__ __forceinline__ float silu_times(float g, float u) {
+    constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+    const float t = -g * kLog2e;
+    const float e = abs_bits(t) < 0x7F800000u ? __builtin_fmaf(-g, kLog2e, -t) : 0.0f;
+    const float p = __builtin_amdgcn_exp2f(t);
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(p, e * kLn2, p)) * u;
+}
+
+// 8 consecutive elements of a row as fp32. WIDE: 16-byte aligned and all inside the row; else one by one, 0 from `n` on
+template <int DT, bool WIDE>
+__device__ __forceinline__ void load8(const void* x, size_t at, int n, float (&v)[8]) {
+    if constexpr (WIDE) {
+        if constexpr (DT == 2) {
+            const float4* p = (const float4*)((const float*)x + at);
+            const float4 a = p[0], b = p[1];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 r = *(const uint4*)((const uint16_t*)x + at);
+            const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (DT == 0) {
+                    const half2_t h = __builtin_bit_cast(half2_t, u[j]);
+                    v[2 * j] = (float)h[0];
+                    v[2 * j + 1] = (float)h[1];
+                } else {
+                    v[2 * j] = __builtin_bit_cast(float, u[j] << 16);
+                    v[2 * j + 1] = __builtin_bit_cast(float, u[j] & 0xFFFF0000u);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j >= n) v[j] = 0.0f;
+            else if constexpr (DT == 0) v[j] = (float)((const _Float16*)x)[at + j];
+            else if constexpr (DT == 1) v[j] = __builtin_bit_cast(float, (uint32_t)((const uint16_t*)x)[at + j] << 16);
+            else v[j] = ((const float*)x)[at + j];
+        }
+    }
+}
+
+}  // namespace exl3

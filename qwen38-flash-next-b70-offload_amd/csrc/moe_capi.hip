@@ -1254,4 +1254,155 @@ int exl3_memcpy_async(void* dst, const void* src, int64_t nbytes, void* stream) 
     return e == hipSuccess ? EXL3_OK : hip_fail(e, "hipMemcpyAsync");
 }
 
+// ---- routing, and the 8-bit float linear -----------------------------------------------------------------------------
+
+namespace {
+
+bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
+size_t dt_size(int dt) { return dt == EXL3_DT_F32 ? 4 : 2; }
+bool dt_ok(int dt) { return dt >= EXL3_DT_F16 && dt <= EXL3_DT_F32; }
+// a launch holds fewer than 2^32 threads
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;
+
+// the sizes every entry point of the 8-bit float linear takes
+int fp8_dims(const char* what, int M, int k, int n) {
+    if (M < 0 || k <= 0 || n <= 0) return fail(EXL3_EINVAL, "%s: M=%d k=%d n=%d", what, M, k, n);
+    if (k > 1 << 28 || n > 1 << 28) return fail(EXL3_EUNSUPPORTED, "%s: k=%d n=%d above 2^28", what, k, n);
+    return EXL3_OK;
+}
+
+int fp8_rows(const char* what, const void* x, int x_dtype, int64_t x_stride, int M, int k, bool silu, void* q, float* s,
+             void* stream) {
+    if (int r = fp8_dims(what, M, k, 1)) return r;
+    if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "%s: dtype %d", what, x_dtype);
+    if (M == 0) return EXL3_OK;
+    if (!x || !q || !s) return fail(EXL3_EINVAL, "%s: null pointer", what);
+    if (x_stride < (silu ? 2 : 1) * (int64_t)k) return fail(EXL3_EINVAL, "%s: row stride %lld", what, (long long)x_stride);
+    if (!aligned(x, dt_size(x_dtype)) || !aligned(q, 16) || !aligned(s, 4)) return fail(EXL3_EINVAL, "%s: alignment", what);
+    if ((M + (int64_t)16) * (fp8_blocks(k) + (int64_t)16) * 16 >= kMaxThreads)
+        return fail(EXL3_EUNSUPPORTED, "%s: M=%d rows of k=%d exceed one launch", what, M, k);
+    Fp8RowsArgs a{};
+    a.x = x;
+    a.x_stride = x_stride;
+    a.M = M;
+    a.k = k;
+    a.q = (uint8_t*)q;
+    a.s = s;
+    const hipError_t e = launch_fp8_rows(a, x_dtype, silu, (hipStream_t)stream);
+    return e == hipSuccess ? EXL3_OK : hip_fail(e, what);
+}
+
+int fp8_product_checks(const char* what, int M, int k, int n, const void* w, const float* sw, const float* bias,
+                       const void* out, int out_dtype, int64_t out_stride) {
+    if (int r = fp8_dims(what, M, k, n)) return r;
+    if (!dt_ok(out_dtype)) return fail(EXL3_EINVAL, "%s: out dtype %d", what, out_dtype);
+    if (M == 0) return EXL3_OK;
+    if (!w || !sw || !out) return fail(EXL3_EINVAL, "%s: null pointer", what);
+    if (out_stride < n) return fail(EXL3_EINVAL, "%s: row stride %lld of out", what, (long long)out_stride);
+    if (!aligned(w, 16) || !aligned(sw, 4) || !aligned(bias, 4) || !aligned(out, dt_size(out_dtype)))
+        return fail(EXL3_EINVAL, "%s: alignment", what);
+    if ((M + (int64_t)64) * (n + (int64_t)64) / 16 >= kMaxThreads)
+        return fail(EXL3_EUNSUPPORTED, "%s: M=%d n=%d exceed one launch", what, M, n);
+    return EXL3_OK;
+}
+
+size_t fp8_q_bytes(int M, int k) { return align256((size_t)M * fp8_blocks(k) * kFp8Block); }
+size_t fp8_s_bytes(int M, int k) { return align256((size_t)M * fp8_blocks(k) * 4); }
+
+}  // namespace
+
+int exl3_moe_route(const void* logits, int dtype, int64_t stride, int M, int E, const float* bias, int topk, int scoring,
+                   int n_group, int topk_group, int renormalize, float scale, int32_t* ids, float* w, void* stream) {
+    if (M < 0 || E <= 0 || E > kMaxExperts) return fail(EXL3_EINVAL, "moe_route: M=%d E=%d (E in 1..%d)", M, E, kMaxExperts);
+    if (!dt_ok(dtype)) return fail(EXL3_EINVAL, "moe_route: dtype %d", dtype);
+    if (scoring != 0 && scoring != 1) return fail(EXL3_EINVAL, "moe_route: scoring %d (0 softmax, 1 sigmoid)", scoring);
+    if (n_group <= 0 || n_group > kRouteMaxGroups || E % n_group || topk_group <= 0 || topk_group > n_group)
+        return fail(EXL3_EINVAL, "moe_route: %d of %d groups of %d experts", topk_group, n_group, E);
+    if (topk <= 0 || topk > kRouteMaxTopk || topk > topk_group * (E / n_group))
+        return fail(EXL3_EINVAL, "moe_route: topk=%d (up to %d, and to the %d experts that compete)", topk, kRouteMaxTopk,
+                    topk_group * (E / n_group));
+    if (M == 0) return EXL3_OK;
+    if (!logits || !ids || !w || stride < E) return fail(EXL3_EINVAL, "moe_route: null pointer or row stride");
+    if (!aligned(logits, dt_size(dtype)) || !aligned(bias, 4) || !aligned(ids, 4) || !aligned(w, 4))
+        return fail(EXL3_EINVAL, "moe_route: alignment");
+    if ((M + (int64_t)64) * 64 >= kMaxThreads) return fail(EXL3_EUNSUPPORTED, "moe_route: M=%d exceeds one launch", M);
+    RouteArgs a{};
+    a.logits = logits;
+    a.stride = stride;
+    a.bias = bias;
+    a.M = M;
+    a.E = E;
+    a.topk = topk;
+    a.sigmoid = scoring;
+    a.n_group = n_group;
+    a.topk_group = topk_group;
+    a.renormalize = renormalize;
+    a.scale = scale;
+    a.ids = ids;
+    a.w = w;
+    const hipError_t e = launch_route(a, dtype, (hipStream_t)stream);
+    return e == hipSuccess ? EXL3_OK : hip_fail(e, "moe_route launch");
+}
+
+int exl3_fp8_quant(const void* x, int x_dtype, int64_t x_stride, int M, int k, void* q, float* s, void* stream) {
+    return fp8_rows("fp8_quant", x, x_dtype, x_stride, M, k, false, q, s, stream);
+}
+
+int exl3_fp8_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int M, int k, void* q, float* s, void* stream) {
+    return fp8_rows("fp8_silu_mul_quant", gate_up, dtype, stride, M, k, true, q, s, stream);
+}
+
+size_t exl3_fp8_matmul_workspace(int M, int k, int n) {
+    (void)M;
+    (void)k;
+    (void)n;
+    return 0;
+}
+
+int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
+                    void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int r = fp8_product_checks("fp8_matmul", M, k, n, w, sw, bias, out, out_dtype, out_stride)) return r;
+    if (M == 0) return EXL3_OK;
+    if (!q || !s || !aligned(q, 16) || !aligned(s, 4)) return fail(EXL3_EINVAL, "fp8_matmul: q or s null or not aligned");
+    const size_t need = exl3_fp8_matmul_workspace(M, k, n);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(EXL3_EWORKSPACE, "fp8_matmul: workspace %zu < %zu bytes", workspace_bytes, need);
+    Fp8ProductArgs a{};
+    a.q = (const uint8_t*)q;
+    a.s = s;
+    a.w = (const uint8_t*)w;
+    a.sw = sw;
+    a.bias = bias;
+    a.M = M;
+    a.n = n;
+    a.kb = fp8_blocks(k);
+    a.out = out;
+    a.out_stride = out_stride;
+    const hipError_t e = launch_fp8_product(a, out_dtype, (hipStream_t)stream);
+    return e == hipSuccess ? EXL3_OK : hip_fail(e, "fp8_matmul launch");
+}
+
+size_t exl3_fp8_linear_workspace(int M, int k, int n) {
+    if (M <= 0 || k <= 0 || n <= 0) return 0;
+    return fp8_q_bytes(M, k) + fp8_s_bytes(M, k) + exl3_fp8_matmul_workspace(M, k, n);
+}
+
+int exl3_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const float* sw,
+                    const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+    if (int r = fp8_product_checks("fp8_linear", M, k, n, w, sw, bias, out, out_dtype, out_stride)) return r;
+    if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "fp8_linear: x dtype %d", x_dtype);
+    if (M == 0) return EXL3_OK;
+    if (!x || x_stride < k) return fail(EXL3_EINVAL, "fp8_linear: x null or row stride %lld", (long long)x_stride);
+    const size_t need = exl3_fp8_linear_workspace(M, k, n);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(EXL3_EWORKSPACE, "fp8_linear: workspace of %zu bytes on 16, got %zu", need, workspace_bytes);
+    uint8_t* q = (uint8_t*)workspace;
+    float* s = (float*)(q + fp8_q_bytes(M, k));
+    if (int r = fp8_rows("fp8_linear", x, x_dtype, x_stride, M, k, false, q, s, stream)) return r;
+    uint8_t* rest = (uint8_t*)s + fp8_s_bytes(M, k);
+    return exl3_fp8_matmul(q, s, M, k, n, w, sw, bias, out, out_dtype, out_stride, rest,
+                           workspace_bytes - (size_t)(rest - q), stream);
+}
+
 }  // extern "C"

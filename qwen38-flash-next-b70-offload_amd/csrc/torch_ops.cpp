@@ -455,6 +455,169 @@ at::Tensor linear_meta(at::Tensor x, at::Tensor trellis, at::Tensor suh, at::Ten
 
 bool linear_supported(int64_t K, int64_t cb) { return exl3_linear_supported((int)K, (int)cb) != 0; }
 
+// ---- exl3xpu_moe.moe_route and the 8-bit float linear of exl3xpu_C ----------------------------------------------------
+// (no counterpart in the reference). Every tensor of a call lives on the first one's device, which the call's launches,
+// allocations and stream are those of, whatever device is current.
+
+void on_device_of(const at::Tensor& x, const at::Tensor& t, const char* what) {
+    TORCH_CHECK(t.device() == x.device(), what, ": tensors on ", x.device(), " and ", t.device());
+}
+
+// fp32, contiguous and of `n` values on x's device; null where there is none
+const float* f32_or_null(const std::optional<at::Tensor>& t, const at::Tensor& x, int64_t n, const char* what) {
+    if (!t) return nullptr;
+    on_device_of(x, *t, what);
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 1 && t->numel() == n, what,
+                ": bias fp32 [", n, "] contiguous");
+    return t->data_ptr<float>();
+}
+
+// [..., n] as [rows, n] with unit column stride (a copy only where the strides are not those of such rows)
+at::Tensor rows_of(const at::Tensor& x, const char* what) {
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, what, ": [..., n] with n > 0, got ", x.sizes());
+    TORCH_CHECK(x.numel() / x.size(-1) <= INT32_MAX && x.size(-1) <= INT32_MAX, what, ": sizes ", x.sizes());
+    auto x2 = x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)});
+    return x2.size(0) == 0 || (x2.stride(1) == 1 && (x2.size(0) == 1 || x2.stride(0) >= x2.size(1))) ? x2 : x2.contiguous();
+}
+int64_t row_stride(const at::Tensor& x2) { return x2.size(0) > 1 ? x2.stride(0) : x2.size(1); }
+
+std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t n) {
+    auto v = sizes.vec();
+    v.back() = n;
+    return v;
+}
+int64_t fp8_up(int64_t k) { return (k + 127) / 128 * 128; }
+
+int scoring_code(c10::string_view scoring) {
+    TORCH_CHECK(scoring == "softmax" || scoring == "sigmoid", "moe_route: scoring 'softmax' or 'sigmoid', got '", scoring, "'");
+    return scoring == "sigmoid";
+}
+
+std::tuple<at::Tensor, at::Tensor> moe_route(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t topk,
+                                             c10::string_view scoring, int64_t n_group, int64_t topk_group,
+                                             bool renormalize, double scale) {
+    const c10::DeviceGuard guard(logits.device());
+    const int sc = scoring_code(scoring);
+    TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) > 0 && logits.size(-1) <= 1024, "moe_route: 1 to 1024 experts, got ",
+                logits.sizes());
+    const int64_t E = logits.size(-1);
+    for (int64_t v : {topk, n_group, topk_group})
+        TORCH_CHECK(v >= 1 && v <= E, "moe_route: topk, n_group and topk_group in 1..", E, ", got ", v);
+    const int dt = dtype_code(logits);
+    auto x2 = rows_of(logits, "moe_route");
+    const float* b = f32_or_null(bias, logits, E, "moe_route");
+    auto ids = at::empty(with_last(logits.sizes(), topk), logits.options().dtype(at::kInt));
+    auto w = at::empty(with_last(logits.sizes(), topk), logits.options().dtype(at::kFloat));
+    check(exl3_moe_route(x2.data_ptr(), dt, row_stride(x2), (int)x2.size(0), (int)E, b, (int)topk, sc, (int)n_group,
+                         (int)topk_group, renormalize, (float)scale, ids.data_ptr<int>(), w.data_ptr<float>(),
+                         cur_stream(logits)),
+          "moe_route");
+    return {ids, w};
+}
+
+std::tuple<at::Tensor, at::Tensor> moe_route_meta(const at::Tensor& logits, const std::optional<at::Tensor>&, int64_t topk,
+                                                  c10::string_view, int64_t, int64_t, bool, double) {
+    return {at::empty(with_last(logits.sizes(), topk), logits.options().dtype(at::kInt)),
+            at::empty(with_last(logits.sizes(), topk), logits.options().dtype(at::kFloat))};
+}
+
+std::tuple<at::Tensor, at::Tensor> fp8_rows_empty(const at::Tensor& x, int64_t k) {
+    return {at::empty(with_last(x.sizes(), fp8_up(k)), x.options().dtype(at::kFloat8_e4m3fn)),
+            at::empty(with_last(x.sizes(), fp8_up(k) / 128), x.options().dtype(at::kFloat))};
+}
+std::tuple<at::Tensor, at::Tensor> fp8_quant_meta(const at::Tensor& x) { return fp8_rows_empty(x, x.size(-1)); }
+std::tuple<at::Tensor, at::Tensor> fp8_silu_mul_quant_meta(const at::Tensor& x) {
+    return fp8_rows_empty(x, x.size(-1) / 2);
+}
+
+std::tuple<at::Tensor, at::Tensor> fp8_quant(const at::Tensor& x) {
+    const c10::DeviceGuard guard(x.device());
+    const int dt = dtype_code(x);
+    auto x2 = rows_of(x, "fp8_quant");
+    auto out = fp8_rows_empty(x, x.size(-1));
+    check(exl3_fp8_quant(x2.data_ptr(), dt, row_stride(x2), (int)x2.size(0), (int)x2.size(1), std::get<0>(out).data_ptr(),
+                         std::get<1>(out).data_ptr<float>(), cur_stream(x)),
+          "fp8_quant");
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> fp8_silu_mul_quant(const at::Tensor& x) {
+    const c10::DeviceGuard guard(x.device());
+    const int dt = dtype_code(x);
+    auto x2 = rows_of(x, "fp8_silu_mul_quant");
+    TORCH_CHECK(x2.size(1) % 2 == 0, "fp8_silu_mul_quant: gate|up rows of an even size, got ", x.sizes());
+    const int64_t k = x2.size(1) / 2;
+    auto out = fp8_rows_empty(x, k);
+    check(exl3_fp8_silu_mul_quant(x2.data_ptr(), dt, row_stride(x2), (int)x2.size(0), (int)k, std::get<0>(out).data_ptr(),
+                                  std::get<1>(out).data_ptr<float>(), cur_stream(x)),
+          "fp8_silu_mul_quant");
+    return out;
+}
+
+void fp8_weight_checks(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sw, int64_t k, const char* what) {
+    on_device_of(x, w, what);
+    on_device_of(x, sw, what);
+    TORCH_CHECK(w.scalar_type() == at::kFloat8_e4m3fn && w.is_contiguous() && w.dim() == 2 && w.size(1) == fp8_up(k) &&
+                    w.size(0) > 0 && w.size(0) <= INT32_MAX,
+                what, ": weight float8_e4m3fn [n, ", fp8_up(k), "] contiguous, got ", w.scalar_type(), " ", w.sizes());
+    TORCH_CHECK(sw.scalar_type() == at::kFloat && sw.is_contiguous() && sw.dim() == 2 &&
+                    sw.size(0) == fp8_up(w.size(0)) / 128 && sw.size(1) == w.size(1) / 128,
+                what, ": weight_scale fp32 [", fp8_up(w.size(0)) / 128, ", ", w.size(1) / 128, "] contiguous, got ",
+                sw.scalar_type(), " ", sw.sizes());
+}
+
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sw, const std::optional<at::Tensor>& bias) {
+    const c10::DeviceGuard guard(x.device());
+    const int dt = dtype_code(x);
+    auto x2 = rows_of(x, "fp8_linear");
+    const int M = (int)x2.size(0), k = (int)x2.size(1);
+    fp8_weight_checks(x, w, sw, k, "fp8_linear");
+    const int64_t n = w.size(0);
+    const float* b = f32_or_null(bias, x, n, "fp8_linear");
+    auto out = at::empty(with_last(x.sizes(), n), x.options());
+    if (M == 0) return out;
+    const size_t ws = exl3_fp8_linear_workspace(M, k, (int)n);
+    auto buf = at::empty({(int64_t)ws}, x.options().dtype(at::kByte));
+    check(exl3_fp8_linear(x2.data_ptr(), dt, row_stride(x2), M, k, (int)n, w.data_ptr(), sw.data_ptr<float>(), b,
+                          out.data_ptr(), dt, n, buf.data_ptr(), ws, cur_stream(x)),
+          "fp8_linear");
+    return out;
+}
+
+at::Tensor fp8_linear_meta(const at::Tensor& x, const at::Tensor& w, const at::Tensor&, const std::optional<at::Tensor>&) {
+    return at::empty(with_last(x.sizes(), w.size(0)), x.options());
+}
+
+at::Tensor fp8_matmul(const at::Tensor& q, const at::Tensor& s, const at::Tensor& w, const at::Tensor& sw,
+                      const std::optional<at::Tensor>& bias, at::ScalarType dtype) {
+    const c10::DeviceGuard guard(q.device());
+    TORCH_CHECK(q.scalar_type() == at::kFloat8_e4m3fn && q.is_contiguous() && q.dim() >= 1 && q.size(-1) > 0 &&
+                    q.size(-1) % 128 == 0 && q.size(-1) <= INT32_MAX && q.numel() / q.size(-1) <= INT32_MAX,
+                "fp8_matmul: q float8_e4m3fn [..., a multiple of 128] contiguous, got ", q.scalar_type(), " ", q.sizes());
+    const int k = (int)q.size(-1), M = (int)(q.numel() / k);
+    on_device_of(q, s, "fp8_matmul");
+    TORCH_CHECK(s.scalar_type() == at::kFloat && s.is_contiguous() && s.dim() == q.dim() &&
+                    s.sizes().vec() == with_last(q.sizes(), k / 128),
+                "fp8_matmul: s fp32 ", with_last(q.sizes(), k / 128), " contiguous, got ", s.scalar_type(), " ", s.sizes());
+    fp8_weight_checks(q, w, sw, k, "fp8_matmul");
+    const int64_t n = w.size(0);
+    const float* b = f32_or_null(bias, q, n, "fp8_matmul");
+    auto out = at::empty(with_last(q.sizes(), n), q.options().dtype(dtype));
+    const int dt = dtype_code(out);
+    if (M == 0) return out;
+    const size_t ws = exl3_fp8_matmul_workspace(M, k, (int)n);
+    auto buf = at::empty({(int64_t)ws}, q.options().dtype(at::kByte));
+    check(exl3_fp8_matmul(q.data_ptr(), s.data_ptr<float>(), M, k, (int)n, w.data_ptr(), sw.data_ptr<float>(), b,
+                          out.data_ptr(), dt, n, ws ? buf.data_ptr() : nullptr, ws, cur_stream(q)),
+          "fp8_matmul");
+    return out;
+}
+
+at::Tensor fp8_matmul_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor& w, const at::Tensor&,
+                           const std::optional<at::Tensor>&, at::ScalarType dtype) {
+    return at::empty(with_last(q.sizes(), w.size(0)), q.options().dtype(dtype));
+}
+
 }  // namespace
 
 TORCH_LIBRARY(exl3xpu_C, m) {
@@ -473,6 +636,18 @@ TORCH_LIBRARY(exl3xpu_C, m) {
     m.impl("exl3_had_out_h", c10::DispatchKey::CUDA, &had_out_h);
     m.def("exl3_reconstruct(Tensor trellis, Tensor(a!) w, int n0, int K, int cb) -> ()");
     m.impl("exl3_reconstruct", c10::DispatchKey::CUDA, &reconstruct);
+    m.def("fp8_quant(Tensor x) -> (Tensor q, Tensor s)");
+    m.impl("fp8_quant", c10::DispatchKey::CUDA, &fp8_quant);
+    m.impl("fp8_quant", c10::DispatchKey::Meta, &fp8_quant_meta);
+    m.def("fp8_silu_mul_quant(Tensor gate_up) -> (Tensor q, Tensor s)");
+    m.impl("fp8_silu_mul_quant", c10::DispatchKey::CUDA, &fp8_silu_mul_quant);
+    m.impl("fp8_silu_mul_quant", c10::DispatchKey::Meta, &fp8_silu_mul_quant_meta);
+    m.def("fp8_linear(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias=None) -> Tensor");
+    m.impl("fp8_linear", c10::DispatchKey::CUDA, &fp8_linear);
+    m.impl("fp8_linear", c10::DispatchKey::Meta, &fp8_linear_meta);
+    m.def("fp8_matmul(Tensor q, Tensor s, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType dtype) -> Tensor");
+    m.impl("fp8_matmul", c10::DispatchKey::CUDA, &fp8_matmul);
+    m.impl("fp8_matmul", c10::DispatchKey::Meta, &fp8_matmul_meta);
 }
 
 TORCH_LIBRARY(exl3xpu_moe, m) {
@@ -501,6 +676,10 @@ TORCH_LIBRARY(exl3xpu_moe, m) {
     m.def("moe_prefetch_worker_stop() -> int[]", &moe_prefetch_worker_stop);
     m.def("moe_align(Tensor topk_ids, Tensor topk_w, int n_experts, int pad) -> Tensor[]");
     m.impl("moe_align", c10::DispatchKey::CUDA, &moe_align);
+    m.def("moe_route(Tensor logits, Tensor? bias, int topk, str scoring, int n_group, int topk_group, bool renormalize, "
+          "float scale) -> (Tensor ids, Tensor w)");
+    m.impl("moe_route", c10::DispatchKey::CUDA, &moe_route);
+    m.impl("moe_route", c10::DispatchKey::Meta, &moe_route_meta);
     m.def("host_alloc(int nbytes) -> Tensor", &host_alloc);
     m.def("usm_kind(int ptr) -> int", &usm_kind);
     m.def("memcpy_async(int dst, int src, int nbytes) -> ()", &memcpy_async);

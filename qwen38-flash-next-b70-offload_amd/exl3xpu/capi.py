@@ -81,6 +81,15 @@ SIGNATURES = {
     "exl3_reconstruct": (c_i32, [c_p, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_p, c_p]),
     "exl3_had_in_q8": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_p, c_i32, c_p, c_p, c_i64, c_p]),
     "exl3_reconstruct_q8": (c_i32, [c_p, c_i32, c_i32, c_i32, c_i32, c_i32, c_p, c_p]),
+    "exl3_moe_route": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_p, c_i32, c_i32, c_i32, c_i32, c_i32, ctypes.c_float,
+                               c_p, c_p, c_p]),
+    "exl3_fp8_quant": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_p, c_p, c_p]),
+    "exl3_fp8_silu_mul_quant": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_p, c_p, c_p]),
+    "exl3_fp8_matmul_workspace": (c_sz, [c_i32, c_i32, c_i32]),
+    "exl3_fp8_matmul": (c_i32, [c_p, c_p, c_i32, c_i32, c_i32, c_p, c_p, c_p, c_p, c_i32, c_i64, c_p, c_sz, c_p]),
+    "exl3_fp8_linear_workspace": (c_sz, [c_i32, c_i32, c_i32]),
+    "exl3_fp8_linear": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_i32, c_p, c_p, c_p, c_p, c_i32, c_i64, c_p, c_sz,
+                                c_p]),
     "exl3_had_out_q8": (c_i32, [c_p, c_i32, c_i32, c_p, ctypes.c_float, c_p, c_p, c_i32, c_i64, c_p]),
 }
 

@@ -13,6 +13,7 @@ current stream unless a stream is given, and nothing synchronises the host unles
   store.evict(key, experts)                               repoint to host; the slot is reused in stream order
   store.forward(key, x, topk_ids, topk_w)                 routed-MoE output (routing weights applied)
   store.forward_cached(key, x, topk_ids, topk_w)          decode through the device-managed LRU cache
+  store.forward_routed(key, x, logits, router)            forward_cached of a routing.Router's picks
   store.prefetch / start_copy_prefetch / plan_prefetch / stop_copy_prefetch    predicted experts into slots early
   store.stage_layer(key, buf, stream)                     prefill: stage the layer's non-HBM experts into HBM
   store.forward_prefill_staged(key, x, topk_ids, topk_w)  prefill with the next layer staged on a copy stream
@@ -663,6 +664,14 @@ class ExpertStore:
                                          self.slot_key, self.slot_last, self.tick, self.host_base, self.slot_base,
                                          self.fill_all, self.fill_list, self.E if max_fill is None else int(max_fill),
                                          self.I, self.k_of(key), self.E, self.pend, self.done_seq)
+
+    def forward_routed(self, key, x: torch.Tensor, logits: torch.Tensor, router, cached: bool = True) -> torch.Tensor:
+        """Routed-MoE output of x [M, H] from its router logits [M, E]: the picks and weights of `router`
+        (exl3xpu.routing.Router), then forward_cached, or forward where cached is false."""
+        if logits.dim() != 2 or logits.size(-1) != self.E:
+            raise ValueError(f"exl3xpu: logits [{x.size(0)}, {self.E}], got {tuple(logits.shape)}")
+        ids, w = router(logits)
+        return self.forward_cached(key, x, ids, w) if cached else self.forward(key, x, ids, w)
 
     def prefetch(self, key, ids: torch.Tensor, max_fill: int = 16) -> None:
         """Claim exact-LRU slots for up to max_fill predicted experts `ids` of `key` that are not resident (the tick is

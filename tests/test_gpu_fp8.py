@@ -1,0 +1,384 @@
+"""The 8-bit float linear (torch.ops.exl3xpu_C.fp8_*, exl3xpu.fp8) against its definition in 64 bits, where it can go wrong:
+sizes around the 128-blocks and the tiles, strides, odd addresses, zero, tiny, huge, infinite and NaN blocks, one row and
+none, streams and graphs.
+
+Quantised rows have to be equal, bit for bit: scale and quotient are single roundings. Behind silu the value may be 8 units
+of 2^-24 off (exp2 and reciprocal 1 unit each, five roundings), the scale as many and one, so a quotient is at most 18 off
+and q the rounding of something within that. A product's error is at most that of its fp32 sums: 128 terms within an MFMA
+and three roundings per block, (128 + 3 blocks + 4) 2^-23 of the sum of magnitudes (2^-23: sums that truncate), then half a
+step of the output type. With bf16 and fp16 outputs the block sums come from e4m3 MFMAs, which align the products of 8
+neighbouring k to the exponent E of their largest and drop what is below 2^(E - 13): at most 7 products of a group lose less
+than 2^-13 of the largest each, so less than 7 2^-13 of the group's magnitudes; and as losses of random sign, 2^-13 sqrt(7 /
+3) times the root of the group's mean largest square, which for normal values (largest of 8 products: 4 times their own
+root mean square at the most) is sqrt(16 groups / 128 terms) 4 sqrt(7 / 3) 2^-13 = 2.6e-4 of the whole product's norm."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _fp8():
+    from exl3xpu import fp8
+    return fp8
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _e4m3(v):
+    """64-bit values to the nearest e4m3 value, halves to even."""
+    a = v.abs().clamp_min(2.0 ** -6)
+    step = torch.exp2(torch.floor(torch.log2(a)).clamp(-6, 8) - 3)
+    return torch.where(v.isfinite(), torch.round(v / step) * step, torch.full_like(v, math.nan))
+
+
+def _blocks(x):
+    M, k = x.shape
+    kb = -(-k // 128)
+    return torch.nn.functional.pad(x, (0, kb * 128 - k)).reshape(M, kb, 128)
+
+
+def _quant_ref(x):
+    """x in 64 bits -> (q, s), each rounded as the definition says."""
+    p = _blocks(x)
+    s = (p.abs().amax(-1) / 448).float().double().clamp_min(2.0 ** -80)
+    return _e4m3((p / s[..., None]).float().double()).reshape(x.size(0), -1), s
+
+
+def _weight(g, n, k):
+    w = torch.randn(n, k, generator=g, device="cuda") * 0.05
+    nb, kb = -(-n // 128), -(-k // 128)
+    p = torch.zeros(nb * 128, kb * 128, device="cuda")
+    p[:n, :k] = w
+    s = (p.view(nb, 128, kb, 128).abs().amax((1, 3)) / 448).clamp_min(1e-12)
+    q = (p.view(nb, 128, kb, 128) / s[:, None, :, None]).view(nb * 128, kb * 128)[:n, :k]
+    return q.to(torch.float8_e4m3fn), s
+
+
+def _product_ref(q, s, w, sw, bias):
+    """(the product, the sum of its terms' magnitudes) in 64 bits."""
+    n, k = w.shape
+    a = (q.double().reshape(q.size(0), -1, 128) * s.double()[..., None]).reshape(q.size(0), -1)[:, :k]
+    b = w.double() * sw.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    y, mag = a @ b.t(), a.abs() @ b.abs().t()
+    return (y, mag) if bias is None else (y + bias.double(), mag + bias.double().abs())
+
+
+def _check_product(y, q, s, w, sw, bias):
+    ref, mag = _product_ref(q, s, w, sw, bias)
+    half, loss = torch.finfo(y.dtype).eps / 2, 0.0 if y.dtype == torch.float32 else 7 * 2.0 ** -13
+    tol = ((128 + 3 * s.size(-1) + 4) * 2.0 ** -23 + loss) * mag
+    tol = tol + half * (ref.abs() + tol) + torch.finfo(y.dtype).smallest_normal
+    bad = ~((y.double() - ref).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), float(((y.double() - ref).abs() / tol).max()))
+    if y.numel() > 1000:
+        rel = float((y.double() - ref).norm() / ref.norm())
+        assert rel <= half + (2.6e-4 if loss else (128 + 3 * s.size(-1) + 4) * 2.0 ** -23), rel
+
+
+def _odd(t):
+    """The same values at an odd element of their storage."""
+    store = torch.zeros(t.numel() + 3, dtype=t.dtype, device=t.device)
+    v = store[1:1 + t.numel()].view(t.shape)
+    v.copy_(t)
+    return v
+
+
+@pytest.mark.parametrize("k", [1, 7, 8, 127, 128, 129, 500, 640, 1000, 2048, 2050])
+def test_quant(k):
+    g = _gen(k)
+    for dtype in DTYPES:
+        for M in (1, 2, 15, 16, 17, 130):
+            print(f"case fp8 quant k={k} M={M} {dtype}", flush=True)
+            x = (torch.randn(M, k, generator=g, device="cuda") * torch.exp(torch.randn(M, 1, generator=g, device="cuda"))).to(dtype)
+            if M > 2:
+                x[1] = 0
+                x[2, k // 2:] = 0
+            q, s = _fp8().quant(x)
+            torch.cuda.synchronize()
+            rq, rs = _quant_ref(x.double())
+            assert q.dtype == torch.float8_e4m3fn and q.shape == rq.shape and s.shape == rs.shape
+            assert torch.equal(s.double(), rs) and torch.equal(q.double(), rq)
+            for other in (_odd(x), torch.nn.functional.pad(x, (0, 9))[:, :k], x.t().contiguous().t()):
+                q2, s2 = _fp8().quant(other)
+                assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, s)
+
+
+def test_quant_every_half_step():
+    """Quotients that lie between two e4m3 values go to the even one, and every e4m3 value comes back as it is."""
+    vals = torch.arange(127, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn).float()      # 0 .. 448
+    mid = (vals[1:] + vals[:-1]) / 2
+    x = torch.zeros(4, 128, device="cuda")
+    x[0, :127] = vals
+    x[1, :126], x[1, 126] = mid, 448
+    x[2, :126], x[2, 126] = -torch.nextafter(mid, mid * 2), 448
+    x[3, :126], x[3, 126] = torch.nextafter(mid, mid * 0), -448
+    for scale in (1.0, 2.0 ** -60, 2.0 ** 90, 3.0, 1 / 3.0):
+        q, s = _fp8().quant(x * scale)
+        rq, rs = _quant_ref((x * scale).double())
+        assert torch.equal(s.double(), rs) and torch.equal(q.double(), rq), scale
+    q, s = _fp8().quant(x)
+    assert (s == 1).all() and torch.equal(q[0, :127].float(), vals)
+
+
+def test_quant_infinities_nan_and_extremes():
+    x = torch.randn(9, 400, generator=_gen(3), device="cuda")
+    x[0, 5] = math.inf
+    x[1, 200] = -math.inf
+    x[2, 300] = math.nan
+    x[3, :128] = 3.4e38
+    x[4] *= 1e-30
+    x[5] *= 1e-42
+    x[6, 130:250] = 0
+    x[7, 399] = math.nan
+    x[8] *= 1e36
+    q, s = _fp8().quant(x)
+    torch.cuda.synchronize()
+    q, s = q.float(), s.cpu()
+    assert s[0, 0] == math.inf and q[0, 5].isnan() and (q[0, [i for i in range(128) if i != 5]] == 0).all()
+    assert s[1, 1] == math.inf and s[2, 2].isnan() and q[2, 256:384].isnan().all() and s[7, 3].isnan()
+    assert s[[0, 1, 2], [1, 0, 0]].isfinite().all()
+    fine = [3, 4, 5, 6, 8]
+    rq, rs = _quant_ref(x[fine].double())
+    assert torch.equal(q[fine].double(), rq) and torch.equal(s[fine].double(), rs.cpu())
+    assert (q[5] == 0).all() and (s[5] == 2.0 ** -80).all()
+
+
+@pytest.mark.parametrize("k", [1, 60, 127, 128, 129, 512, 640, 1001])
+def test_silu_mul_quant(k):
+    g = _gen(100 + k)
+    for dtype in DTYPES:
+        for M in (1, 3, 16, 131):
+            print(f"case fp8 silu k={k} M={M} {dtype}", flush=True)
+            gu = (torch.randn(M, 2 * k, generator=g, device="cuda") * 4).to(dtype)
+            if M > 2:
+                gu[1, :k] = -90.0                            # silu far below what fp32 holds comfortably
+                gu[2] = 0
+            for t in (gu, _odd(gu), torch.nn.functional.pad(gu, (0, 5))[:, :2 * k]):
+                q, s = _fp8().silu_mul_quant(t)
+                torch.cuda.synchronize()
+                a, u = gu[:, :k].double(), gu[:, k:].double()
+                v = _blocks(a / (1 + torch.exp(-a)) * u)
+                rs = (v.abs().amax(-1) / 448).clamp_min(2.0 ** -80)
+                eps = 2.0 ** -24
+                assert ((s.double() - rs).abs() <= 9 * eps * rs).all()
+                quo = (v / rs[..., None]).reshape(M, -1)
+                lo, hi = _e4m3(quo.abs() * (1 - 19 * eps)), _e4m3(quo.abs() * (1 + 19 * eps))
+                got = q.double()
+                assert ((got.abs() >= lo) & (got.abs() <= hi) & ((got == 0) | (got.sign() == quo.sign()))).all()
+
+
+def test_silu_infinities_and_nan():
+    gu = torch.ones(5, 256, device="cuda")
+    gu[0, 3] = math.inf
+    gu[1, 3] = -math.inf
+    gu[2, 3] = math.nan
+    gu[3, 130] = math.inf
+    gu[4, 3] = -200.0
+    q, s = _fp8().silu_mul_quant(gu)
+    torch.cuda.synchronize()
+    assert s[0, 0] == math.inf and s[1, 0].isnan() and s[2, 0].isnan() and s[3, 0] == math.inf and s[4, 0].isfinite()
+    assert q[4, 3].float() == 0 and (q[0].float().nan_to_num() == 0).all()
+
+
+SIZES = [(1, 128), (5, 1), (16, 129), (17, 640), (127, 1000), (128, 512), (129, 2048), (200, 127), (384, 1152), (1000, 2000)]
+
+
+@pytest.mark.parametrize("n,k", SIZES)
+def test_linear(n, k):
+    g = _gen(7 * n + k)
+    w, sw = _weight(g, n, k)
+    bias = torch.randn(n, generator=g, device="cuda")
+    lin, linb = _fp8().Fp8Linear(w, sw), _fp8().Fp8Linear(w, sw, bias)
+    for M in (1, 2, 3, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 127, 128, 129, 255, 257, 300):
+        for dtype in DTYPES:
+            print(f"case fp8 linear n={n} k={k} M={M} {dtype}", flush=True)
+            x = torch.randn(M, k, generator=g, device="cuda").to(dtype)
+            y, yb = lin(x), linb(x)
+            torch.cuda.synchronize()
+            assert y.dtype == dtype and y.shape == (M, n)
+            q, s = _quant_ref(x.double())
+            _check_product(y, q, s, w, sw, None)
+            _check_product(yb, q, s, w, sw, bias)
+            q, s = _fp8().quant(x)
+            assert torch.equal(lin.quantised(q, s, dtype), y)
+            assert torch.equal(lin(_odd(x)), y)
+
+
+@pytest.mark.parametrize("M,n,k", [(700, 512, 2048), (1025, 640, 384), (2048, 2048, 512), (513, 4096, 130), (64, 8192, 256),
+                                   (40, 2048, 4096), (1, 12288, 2048), (4, 1024, 2048), (300, 12288, 512)])
+def test_linear_larger(M, n, k):
+    g = _gen(M + n)
+    w, sw = _weight(g, n, k)
+    lin = _fp8().Fp8Linear(w, sw)
+    for dtype in DTYPES:
+        print(f"case fp8 linear M={M} n={n} k={k} {dtype}", flush=True)
+        x = (torch.randn(M, k, generator=g, device="cuda") * torch.exp(torch.randn(M, 1, generator=g, device="cuda"))).to(dtype)
+        y = lin(x)
+        torch.cuda.synchronize()
+        _check_product(y, *_quant_ref(x.double()), w, sw, None)
+        assert torch.equal(lin(x), y)                        # the same sums in the same order
+
+
+def test_linear_rows_do_not_see_each_other():
+    """A NaN or an infinity stays in its row, and a NaN weight in its column."""
+    g = _gen(21)
+    for M in (5, 40, 300):
+        w, sw = _weight(g, 300, 384)
+        x = torch.randn(M, 384, generator=g, device="cuda").bfloat16()
+        want = _fp8().Fp8Linear(w, sw)(x)
+        x[1, 200] = math.nan
+        x[3, 0] = math.inf
+        raw = w.clone().view(torch.uint8)
+        raw[130, 5] = 0x7F                                   # e4m3's NaN
+        y = _fp8().Fp8Linear(raw.view(torch.float8_e4m3fn), sw)(x)
+        torch.cuda.synchronize()
+        assert y[1].isnan().all() and y[3].isnan().all() and y[:, 130].isnan().all()
+        rows = [m for m in range(M) if m not in (1, 3)]
+        cols = [i for i in range(300) if i != 130]
+        assert torch.equal(y[rows][:, cols], want[rows][:, cols])
+
+
+def test_linear_shapes_strides_and_empty():
+    g = _gen(23)
+    w, sw = _weight(g, 260, 300)
+    lin = _fp8().Fp8Linear(w, sw)
+    x = torch.randn(24, 300, generator=g, device="cuda").bfloat16()
+    y = lin(x)
+    assert torch.equal(lin(x.view(2, 3, 4, 300)), y.view(2, 3, 4, 260))
+    assert torch.equal(lin(x[0]), lin(x[:1])[0])
+    assert torch.equal(lin(torch.nn.functional.pad(x, (0, 7))[:, :300]), y)
+    assert torch.equal(lin(x.t().contiguous().t()), y)
+    assert torch.equal(lin(x[:1].expand(24, 300)), lin(x[:1]).expand(24, 260))
+    assert lin(x[:0]).shape == (0, 260) and lin(x.view(4, 6, 300)[:, :0]).shape == (4, 0, 260)
+    q, s = _fp8().quant(x.view(4, 6, 300))
+    assert torch.equal(lin.quantised(q, s, torch.bfloat16), y.view(4, 6, 260))
+    assert lin.quantised(q[:, :0], s[:, :0], torch.float16).shape == (4, 0, 260)
+
+
+def test_c_abi_leaves_what_is_behind_a_row():
+    """Columns behind n and rows behind M of a wider output are left as they were, and a workspace of a larger call does
+    for a smaller one."""
+    from exl3xpu import capi
+    L, st = capi.lib(), torch.cuda.current_stream().cuda_stream
+    g = _gen(25)
+    for M, n, k in ((1, 130, 256), (20, 200, 384), (200, 257, 512)):
+        w, sw = _weight(g, n, k)
+        x = torch.randn(M, k, generator=g, device="cuda").bfloat16()
+        out = torch.full((M + 3, n + 5), 7.0, dtype=torch.bfloat16, device="cuda")
+        ws = torch.empty(L.exl3_fp8_linear_workspace(M + 500, k, n), dtype=torch.uint8, device="cuda")
+        print(f"case fp8 c-abi M={M} n={n} k={k}", flush=True)
+        capi.check(L.exl3_fp8_linear(x.data_ptr(), 1, k, M, k, n, w.data_ptr(), sw.data_ptr(), None, out.data_ptr(), 1,
+                                     n + 5, ws.data_ptr(), ws.numel(), st))
+        torch.cuda.synchronize()
+        assert torch.equal(out[:M, :n], _fp8().Fp8Linear(w, sw)(x))
+        assert (out[M:] == 7).all() and (out[:, n:] == 7).all()
+
+
+def test_refusals():
+    g = _gen(27)
+    w, sw = _weight(g, 256, 256)
+    lin = _fp8().Fp8Linear(w, sw)
+    C = lin._op
+    x = torch.randn(4, 256, generator=g, device="cuda").bfloat16()
+    q, s = _fp8().quant(x)
+    bad = [lambda: lin(x[:, :255]), lambda: lin(x.double()), lambda: lin(x.to(torch.float8_e4m3fn)),
+           lambda: C.fp8_linear(x, w.float(), sw, None), lambda: C.fp8_linear(x, w.t(), sw, None),
+           lambda: C.fp8_linear(x, w, sw[:1], None), lambda: C.fp8_linear(x, w, sw.double(), None),
+           lambda: C.fp8_linear(x, w, sw, torch.zeros(255, device="cuda")),
+           lambda: C.fp8_linear(x, w, sw, torch.zeros(256, device="cuda").bfloat16()),
+           lambda: C.fp8_linear(x, w.cpu(), sw, None), lambda: C.fp8_matmul(q, s[:3], w, sw, None, torch.bfloat16),
+           lambda: C.fp8_matmul(q[:, :200], s, w, sw, None, torch.bfloat16),
+           lambda: C.fp8_matmul(q, s, w, sw, None, torch.int32),
+           lambda: C.fp8_matmul(q.view(torch.float8_e5m2), s, w, sw, None, torch.bfloat16),
+           lambda: _fp8().quant(x.int()), lambda: _fp8().quant(x[:, :0]), lambda: _fp8().silu_mul_quant(x[:, :255])]
+    for i, f in enumerate(bad):
+        with pytest.raises((RuntimeError, ValueError)):
+            f()
+            pytest.fail(f"call {i} was taken")
+    with pytest.raises(NotImplementedError):
+        _fp8().quant(x.cpu())
+
+
+def _mlp(g, k, I):  # noqa: E741
+    fp8 = _fp8()
+    return fp8.Fp8Mlp(fp8.Fp8Linear(*_weight(g, 2 * I, k)), fp8.Fp8Linear(*_weight(g, k, I)))
+
+
+@pytest.mark.parametrize("M", [1, 4, 37, 300])
+def test_mlp_is_its_parts(M):
+    g = _gen(31)
+    for k, I in ((2048, 512), (512, 640), (300, 200)):  # noqa: E741
+        mlp = _mlp(g, k, I)
+        x = torch.randn(M, k, generator=g, device="cuda").bfloat16()
+        gu = mlp.gate_up(x)
+        q, s = _fp8().silu_mul_quant(gu)
+        assert torch.equal(mlp(x), mlp.down.quantised(q, s, x.dtype))
+
+
+def _layer(g, M):
+    """An MoE layer as a model runs it: router, routed experts through the cache, shared expert."""
+    from exl3xpu.moe_offload import ExpertStore
+    from exl3xpu.routing import Router
+    from exl3xpu.synth import expert_blob
+    H, I, E = 256, 128, 16  # noqa: E741
+    store = ExpertStore(H, I, 3, E, E, max_layers=1)
+    store.add_layer("layer0", torch.stack([expert_blob(5, e, H, I, 3) for e in range(E)]))
+    mlp, wr = _mlp(g, H, I), torch.randn(E, H, generator=g, device="cuda") / 16
+    router = Router(4, scoring="sigmoid", bias=0.05 * torch.randn(E, generator=g, device="cuda"), n_group=4, topk_group=2)
+
+    def forward(x):
+        return store.forward_routed("layer0", x, x.float() @ wr.t(), router) + mlp(x)
+    return store, router, mlp, wr, forward
+
+
+def test_layer_together():
+    g = _gen(33)
+    for M in (1, 3, 40):
+        store, router, mlp, wr, forward = _layer(g, M)
+        x = torch.randn(M, 256, generator=g, device="cuda").bfloat16()
+        ids, w = router(x.float() @ wr.t())
+        want = store.forward("layer0", x, ids, w) + mlp(x)
+        got = forward(x)
+        assert torch.equal(got, want)
+        assert torch.equal(store.forward_routed("layer0", x, x.float() @ wr.t(), router, cached=False) + mlp(x), want)
+        with pytest.raises(ValueError):
+            store.forward_routed("layer0", x, (x.float() @ wr.t())[:, :8], router)
+
+
+def test_layer_in_two_graphs_and_on_streams():
+    """Two captured layers replayed in turn, eager work between; then the parts on two streams at once."""
+    g = _gen(35)
+    M = 3
+    store, router, mlp, wr, forward = _layer(g, M)
+    xs = [torch.randn(M, 256, generator=g, device="cuda").bfloat16() for _ in range(3)]
+    want = [forward(x).clone() for x in xs]
+    torch.cuda.synchronize()
+    bufs, outs, graphs = [xs[0].clone(), xs[1].clone()], [], []
+    for b in bufs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(forward(b))
+        graphs.append(gr)
+    for i, j in ((0, 1), (2, 0), (1, 2), (2, 1)):
+        bufs[0].copy_(xs[i])
+        bufs[1].copy_(xs[j])
+        graphs[0].replay()
+        graphs[1].replay()
+        assert torch.equal(forward(xs[j]), want[j])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[i]) and torch.equal(outs[1], want[j])
+    big = [torch.randn(m, 256, generator=g, device="cuda").bfloat16() for m in (500, 30)]
+    alone = [mlp(x).clone() for x in big]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in big], [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(mlp(big[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, alone[i]) for i in range(2) for t in got[i])
