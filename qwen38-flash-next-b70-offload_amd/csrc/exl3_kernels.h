@@ -250,7 +250,7 @@ hipError_t launch_route(const RouteArgs& a, int dtype, hipStream_t s);
 
 // The 8-bit float linear: rows in e4m3 with one fp32 scale per 128 columns, weights in e4m3 with one per 128 x 128 block
 constexpr int kFp8Block = 128;
-static inline int fp8_blocks(int n) { return n / kFp8Block + (n % kFp8Block != 0); }
+__host__ __device__ static inline int fp8_blocks(int n) { return n / kFp8Block + (n % kFp8Block != 0); }
 // fp8_rows.hip. silu: x holds gate|up rows of 2 k values and the rows written are silu(gate) * up
 struct Fp8RowsArgs {
     const void* x; int64_t x_stride;
@@ -258,14 +258,22 @@ struct Fp8RowsArgs {
     uint8_t* q; float* s;                          // [M, 128 ceil(k / 128)] (zeros behind k), [M, ceil(k / 128)]
 };
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, int x_dt, bool silu, hipStream_t st);
+// 16-byte loads of such rows: every row starts on 16 bytes and no group of 8 elements crosses its end
+static inline bool fp8_rows_wide(const void* x, int64_t x_stride, int k, int x_dt) {
+    return (uintptr_t)x % 16 == 0 && x_stride * (x_dt == 2 ? 4 : 2) % 16 == 0 && k % 8 == 0;
+}
 // fp8_linear.hip: out[m][n] = sum_b s[m][b] sw[n / 128][b] sum_(k in b) q[m][k] w[n][k] + bias[n]
 struct Fp8ProductArgs {
-    const uint8_t* q; const float* s;              // as above, kb = ceil(k / 128) blocks
+    const uint8_t* q; const float* s;              // as above, kb = ceil(k / 128) blocks; null: quantised from rows below
     const uint8_t* w; const float* sw;             // [n, 128 kb], [ceil(n / 128), kb]
     const float* bias;                             // [n] or null
     int M, n, kb;
     void* out; int64_t out_stride;
+    const void* x; int64_t x_stride; int k, x_dt;  // rows as Fp8RowsArgs has them
+    bool silu, x_wide;
 };
+// whether the product quantises its rows itself (no launch_fp8_rows before it)
+bool fp8_product_quantises(int M, int k, int n);
 hipError_t launch_fp8_product(const Fp8ProductArgs& a, int out_dt, hipStream_t st);
 
 }  // namespace exl3

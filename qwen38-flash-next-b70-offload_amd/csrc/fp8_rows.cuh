@@ -85,4 +85,41 @@ __device__ __forceinline__ void load8(const void* x, size_t at, int n, float (&v
     }
 }
 
+// the largest over the 16 lanes of a DPP row, in every one of them (row_ror 8, 4, 2, 1)
+template <int CTRL>
+__device__ __forceinline__ uint32_t ror_max(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+    return ror_max<0x121>(ror_max<0x122>(ror_max<0x124>(ror_max<0x128>(v))));
+}
+
+// 8 of a block's 128 values before they are quantised: those of x at `at`, or silu(x[at]) x[at + k]; `n` of them (any
+// number, also negative) lie inside the row, the others are 0
+template <int DT, bool SILU, bool WIDE>
+__device__ __forceinline__ void block_values(const void* x, size_t at, int k, int n, float (&v)[8]) {
+    if (n <= 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        return;
+    }
+    load8<DT, WIDE>(x, at, n, v);
+    if constexpr (SILU) {
+        float u[8];
+        load8<DT, WIDE>(x, at + k, n, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = silu_times(v[j], u[j]);
+    }
+}
+
+// the 8 values' e4m3 and the scale of the block that the 16 lanes of a DPP row hold
+__device__ __forceinline__ uint2 quant_block(const float (&v)[8], float& s) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max(amax, abs_bits(v[j]));
+    s = fp8_scale(row16_max(amax));
+    const Fp8Div d(s);
+    return {pack_e4m3(d(v[0]), d(v[1]), d(v[2]), d(v[3])), pack_e4m3(d(v[4]), d(v[5]), d(v[6]), d(v[7]))};
+}
+
 }  // namespace exl3

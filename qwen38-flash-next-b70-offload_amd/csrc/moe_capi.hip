@@ -1267,7 +1267,8 @@ constexpr int64_t kMaxThreads = (int64_t)1 << 32;
 // the sizes every entry point of the 8-bit float linear takes
 int fp8_dims(const char* what, int M, int k, int n) {
     if (M < 0 || k <= 0 || n <= 0) return fail(EXL3_EINVAL, "%s: M=%d k=%d n=%d", what, M, k, n);
-    if (k > 1 << 28 || n > 1 << 28) return fail(EXL3_EUNSUPPORTED, "%s: k=%d n=%d above 2^28", what, k, n);
+    // (a tile's 256 rows of k are one buffer of less than 2^32 bytes)
+    if (k > 1 << 22 || n > 1 << 28) return fail(EXL3_EUNSUPPORTED, "%s: k=%d above 2^22 or n=%d above 2^28", what, k, n);
     return EXL3_OK;
 }
 
@@ -1397,6 +1398,25 @@ int exl3_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, 
     const size_t need = exl3_fp8_linear_workspace(M, k, n);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return fail(EXL3_EWORKSPACE, "fp8_linear: workspace of %zu bytes on 16, got %zu", need, workspace_bytes);
+    if (fp8_product_quantises(M, k, n)) {
+        if (!aligned(x, dt_size(x_dtype))) return fail(EXL3_EINVAL, "fp8_linear: alignment of x");
+        Fp8ProductArgs a{};
+        a.x = x;
+        a.x_stride = x_stride;
+        a.x_dt = x_dtype;
+        a.k = k;
+        a.x_wide = fp8_rows_wide(x, x_stride, k, x_dtype);
+        a.w = (const uint8_t*)w;
+        a.sw = sw;
+        a.bias = bias;
+        a.M = M;
+        a.n = n;
+        a.kb = fp8_blocks(k);
+        a.out = out;
+        a.out_stride = out_stride;
+        const hipError_t e = launch_fp8_product(a, out_dtype, (hipStream_t)stream);
+        return e == hipSuccess ? EXL3_OK : hip_fail(e, "fp8_linear launch");
+    }
     uint8_t* q = (uint8_t*)workspace;
     float* s = (float*)(q + fp8_q_bytes(M, k));
     if (int r = fp8_rows("fp8_linear", x, x_dtype, x_stride, M, k, false, q, s, stream)) return r;
