@@ -98,11 +98,8 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
 // number, also negative) lie inside the row, the others are 0
 template <int DT, bool SILU, bool WIDE>
 __device__ __forceinline__ void block_values(const void* x, size_t at, int k, int n, float (&v)[8]) {
-    if (n <= 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        return;
-    }
+    // (no branch where a whole group of 8 is loaded or none: the row before any other takes the place of none)
+    if (WIDE) at = n > 0 ? at : 0;
     load8<DT, WIDE>(x, at, n, v);
     if constexpr (SILU) {
         float u[8];
@@ -110,6 +107,9 @@ __device__ __forceinline__ void block_values(const void* x, size_t at, int k, in
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = silu_times(v[j], u[j]);
     }
+    if (WIDE)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = n > 0 ? v[j] : 0.0f;
 }
 
 // the 8 values' e4m3 and the scale of the block that the 16 lanes of a DPP row hold

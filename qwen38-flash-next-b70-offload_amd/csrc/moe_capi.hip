@@ -1268,7 +1268,7 @@ constexpr int64_t kMaxThreads = (int64_t)1 << 32;
 int fp8_dims(const char* what, int M, int k, int n) {
     if (M < 0 || k <= 0 || n <= 0) return fail(EXL3_EINVAL, "%s: M=%d k=%d n=%d", what, M, k, n);
     // (a tile's 256 rows of k are one buffer of less than 2^32 bytes)
-    if (k > 1 << 22 || n > 1 << 28) return fail(EXL3_EUNSUPPORTED, "%s: k=%d above 2^22 or n=%d above 2^28", what, k, n);
+    if (k > 1 << 22 || n > 1 << 27) return fail(EXL3_EUNSUPPORTED, "%s: k=%d above 2^22 or n=%d above 2^27", what, k, n);
     return EXL3_OK;
 }
 
@@ -1302,7 +1302,7 @@ int fp8_product_checks(const char* what, int M, int k, int n, const void* w, con
     if (out_stride < n) return fail(EXL3_EINVAL, "%s: row stride %lld of out", what, (long long)out_stride);
     if (!aligned(w, 16) || !aligned(sw, 4) || !aligned(bias, 4) || !aligned(out, dt_size(out_dtype)))
         return fail(EXL3_EINVAL, "%s: alignment", what);
-    if ((M + (int64_t)64) * (n + (int64_t)64) / 16 >= kMaxThreads)
+    if ((M + (int64_t)255) * (n + (int64_t)255) / 64 >= kMaxThreads)
         return fail(EXL3_EUNSUPPORTED, "%s: M=%d n=%d exceed one launch", what, M, n);
     return EXL3_OK;
 }
