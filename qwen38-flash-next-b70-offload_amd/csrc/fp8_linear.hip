@@ -19,14 +19,14 @@ void launch_fp8_tile_32(int tile, bool few, const Fp8ProductArgs& a, int out_dt,
 
 namespace {
 constexpr int kCus = 256;
-// rows up to which the product quantises them itself, and the bytes of LDS that they may take
-constexpr int kOwnRows = 16, kOwnBytes = 48 * 1024;
+// rows up to which the product quantises them itself, and their blocks of 128: as many as a workgroup quantises at once
+constexpr int kOwnRows = 16, kOwnBlocks = 128;
 }  // namespace
 
 bool fp8_product_quantises(int M, int k, int n) {
     (void)n;
     const int kb = fp8_blocks(k);
-    return M <= kOwnRows && (int64_t)M * ((kb | 1) * (int64_t)kFp8Block + kb * 4) <= kOwnBytes;
+    return M <= kOwnRows && (int64_t)M * kb <= kOwnBlocks;
 }
 
 hipError_t launch_fp8_product(const Fp8ProductArgs& a, int out_dt, hipStream_t st) {

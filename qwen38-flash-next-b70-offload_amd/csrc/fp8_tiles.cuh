@@ -53,14 +53,14 @@ __device__ __forceinline__ v4f block_sum(const Frag<true>& a, const Frag<true>& 
 }
 
 // four outputs as fp16 (DT 0) or bf16 (DT 1)
-__device__ __forceinline__ v4u narrow4(v4f v, int dt) {
+template <int DT>
+__device__ __forceinline__ v4u narrow4(v4f v) {
     v4u u;
-    if (dt == 0)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = __builtin_bit_cast(uint16_t, (_Float16)v[j]);
-    else
-#pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (DT == 0) u[j] = __builtin_bit_cast(uint16_t, (_Float16)v[j]);
+        else u[j] = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
+    }
     return u;
 }
 
@@ -84,7 +84,7 @@ __device__ __forceinline__ int piece_at(int row, int c) { return c ^ ((row >> 1)
 template <int QB, int BN>
 struct Stage {
     uint8_t w[BN * 128];
-    uint8_t q[QB * 128 + 16];
+    uint8_t q[QB ? QB * 128 : 16];
     float s[QB < 64 ? 64 : QB];
     float sw[64];                                    // [0], and [1] for 256 columns
 };
@@ -97,12 +97,14 @@ template <int THREADS, int DT, bool SILU, bool WIDE, class F>
 __device__ __forceinline__ void quant_rows(const Fp8ProductArgs& A, uint8_t* q, float* s, F between) {
     constexpr int kTogether = 4, kGroups = THREADS / 16;
     const int i = threadIdx.x & 15, tasks = A.M * A.kb, rb = own_row_bytes(A.kb);
+    const uint32_t magic = (65536 + A.kb - 1) / A.kb;        // t / kb for t < 65536 / kb (there are few: kOwnBlocks)
+    auto row_of = [&](int t) { return (int)((uint32_t)t * magic >> 16); };
     int t0 = threadIdx.x >> 4;
     float v[kTogether][8];
     auto values = [&] {                              // (the loads of four blocks before the first is needed)
 #pragma unroll
         for (int u = 0; u < kTogether; ++u) {
-            const int t = t0 + u * kGroups, m = t / A.kb, c = (t - m * A.kb) * kFp8Block + i * 8;
+            const int t = t0 + u * kGroups, m = row_of(t), c = (t - m * A.kb) * kFp8Block + i * 8;
             block_values<DT, SILU, WIDE>(A.x, (size_t)m * A.x_stride + c, A.k, t < tasks ? A.k - c : 0, v[u]);
         }
     };
@@ -111,7 +113,7 @@ __device__ __forceinline__ void quant_rows(const Fp8ProductArgs& A, uint8_t* q, 
     while (true) {
 #pragma unroll
         for (int u = 0; u < kTogether; ++u) {
-            const int t = t0 + u * kGroups, m = t / A.kb, b = t - m * A.kb;
+            const int t = t0 + u * kGroups, m = row_of(t), b = t - m * A.kb;
             float sc;
             const uint2 o = quant_block(v[u], sc);
             if (t >= tasks) continue;
@@ -314,13 +316,17 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp8_tile_kernel(Fp8ProductA
         // are next to each other; the pieces of a row in an order that differs from row to row (banks)
         constexpr int kPieces = TN * 2;              // 16-byte pieces of a row
         uint16_t* o = lds.last.out[wv];
+        auto to_out = [&](auto dt) {
 #pragma unroll
-        for (int j = 0; j < TM; ++j)
+            for (int j = 0; j < TM; ++j)
 #pragma unroll
-            for (int i = 0; i < TN; ++i) {
-                const int m = j * 16 + r, piece = (i * 2 + (g >> 1)) ^ (m & (kPieces - 1));
-                *(v4u*)(o + (m * kPieces + piece) * 8 + (g & 1) * 4) = narrow4(acc[j][i] + bias[i], out_dt);
-            }
+                for (int i = 0; i < TN; ++i) {
+                    const int m = j * 16 + r, piece = (i * 2 + (g >> 1)) ^ (m & (kPieces - 1));
+                    *(v4u*)(o + (m * kPieces + piece) * 8 + (g & 1) * 4) = narrow4<decltype(dt)::value>(acc[j][i] + bias[i]);
+                }
+        };
+        if (out_dt == 0) to_out(std::integral_constant<int, 0>());
+        else to_out(std::integral_constant<int, 1>());
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         const bool wide = A.out_stride % 8 == 0 && (uintptr_t)A.out % 16 == 0;
@@ -356,7 +362,7 @@ template <bool EXACT>
 void launch_fp8_tile(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
     if (!a.q) {
         if (tile == kTile16) launch_fp8_tiles<EXACT, true, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
-        else launch_fp8_tiles<EXACT, true, 16, 32, 1, 2, 4, 2>(a, out_dt, st);
+        else launch_fp8_tiles<EXACT, true, 16, 32, 1, 2, 2, 4>(a, out_dt, st);
     } else if (tile == kTile16) launch_fp8_tiles<EXACT, false, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
     else if (tile == kTile16x32) launch_fp8_tiles<EXACT, false, 16, 32, 1, 2, 4, 2>(a, out_dt, st);
     else if (tile == kTile32) launch_fp8_tiles<EXACT, false, 32, 32, 1, 2, 4, 2>(a, out_dt, st);

@@ -11,8 +11,10 @@
 //           nothing underflows), times scale; a sum of 0 (every pick at -inf) gives weights of 0
 //
 // One wave per row. Lane i holds the E / 64 neighbouring experts from i * NPL, so the lowest lane of a tie holds the
-// lowest index. A pick is one maximum over the lanes (six DPP steps), the first lane that has it, and that lane's next
-// maximum. Nothing is kept between calls and no row depends on another.
+// lowest index; it sorts their keys (a network of max and min, without the indices). A pick is then one maximum over the
+// lanes' first keys (six DPP steps), the first lane that has it, and that lane's keys move up. What the picks were is found
+// at the end, all at once: lane r looks up the place of pick r's key among the keys of the lane that it came from. Nothing is
+// kept between calls and no row depends on another.
 #include "exl3_common.cuh"
 #include "exl3_kernels.h"
 
@@ -23,45 +25,89 @@ namespace {
 
 constexpr int kRouteWaves = 4;
 
-// order-preserving keys: larger value, larger key; -0 as +0, NaN above everything, 0 below everything (no expert)
+// Keys in the order of their values: the larger value has the larger key, -0 that of +0, NaN one above all others, and
+// kNone (no expert, or one that was picked) is below all. 32 bits: the logit's bits, turned; 64 bits: the value itself, with
+// places of their own for what has none among the finite ones (score + bias is below 1e39).
 __device__ __forceinline__ uint32_t key_of(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.0f);
-    return v != v ? 0xFFFFFFFFu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ uint64_t key_of(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
-    return v != v ? ~0ull : (u >> 63) ? ~u : u | 0x8000000000000000ull;
+    const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.0f), k = u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+    return v != v ? 0xFFFFFFFFu : k;
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
     return __builtin_bit_cast(float, (k & 0x80000000u) ? (k == 0xFFFFFFFFu ? 0x7FC00000u : k & 0x7FFFFFFFu) : ~k);
 }
-__device__ __forceinline__ double value_of(uint64_t k) {
-    return __builtin_bit_cast(double, (k >> 63) ? (k == ~0ull ? 0x7FF8000000000000ull : k & 0x7FFFFFFFFFFFFFFFull) : ~k);
+constexpr double kInf = 1e300, kNan = 2e300;
+__device__ __forceinline__ double key_of(double v) {
+    return v != v ? kNan : v == INFINITY ? kInf : v == -INFINITY ? -kInf : v + 0.0;
 }
+__device__ __forceinline__ double value_of(double k) {
+    return k == kNan ? __builtin_nan("") : k == kInf ? INFINITY : k == -kInf ? -INFINITY : k;
+}
+template <class Key> constexpr Key kNone = std::is_same_v<Key, double> ? (Key)-INFINITY : (Key)0;
 
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+__device__ __forceinline__ uint32_t smaller(uint32_t a, uint32_t b) { return min(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return __builtin_fmin(a, b); }
+
+// v of the lane that CTRL names, `none` where there is no such lane
 template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
-    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+__device__ __forceinline__ uint32_t dpp(uint32_t v, uint32_t none) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, 0xF, 0xF, false);
 }
-// the largest value over the wave, in every lane
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    v = dpp_max<0x111>(v);      // row_shr 1, 2, 4, 8: lane 15 of each row of 16 has the row's
-    v = dpp_max<0x112>(v);
-    v = dpp_max<0x114>(v);
-    v = dpp_max<0x118>(v);
-    v = dpp_max<0x142>(v);      // row_bcast 15 and 31: lane 63 has the wave's
-    v = dpp_max<0x143>(v);
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v, float none) {
+    return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, none)));
 }
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-    const uint32_t hi = (uint32_t)(v >> 32), m = wave_max(hi);
-    return (uint64_t)m << 32 | wave_max(hi == m ? (uint32_t)v : 0u);
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v, double none) {
+    const uint64_t a = __builtin_bit_cast(uint64_t, v), b = __builtin_bit_cast(uint64_t, none);
+    return __builtin_bit_cast(double, (uint64_t)dpp<CTRL>((uint32_t)(a >> 32), (uint32_t)(b >> 32)) << 32 |
+                                          dpp<CTRL>((uint32_t)a, (uint32_t)b));
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+__device__ __forceinline__ float lane_value(float v, int l) {
+    return __builtin_bit_cast(float, lane_value(__builtin_bit_cast(uint32_t, v), l));
+}
+__device__ __forceinline__ double lane_value(double v, int l) {
+    const uint64_t a = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)lane_value((uint32_t)(a >> 32), l) << 32 | lane_value((uint32_t)a, l));
+}
+// f over the wave's values: row_shr 1, 2, 4, 8 (lane 15 of each row of 16 has the row's), row_bcast 15 and 31 (lane 63)
+template <class T, class F>
+__device__ __forceinline__ T over_wave(T v, T none, F f) {
+    v = f(v, dpp<0x111>(v, none));
+    v = f(v, dpp<0x112>(v, none));
+    v = f(v, dpp<0x114>(v, none));
+    v = f(v, dpp<0x118>(v, none));
+    v = f(v, dpp<0x142>(v, none));
+    v = f(v, dpp<0x143>(v, none));
+    return lane_value(v, 63);
+}
+template <class Key>
+__device__ __forceinline__ Key wave_max(Key v) {
+    return over_wave(v, kNone<Key>, [](Key a, Key b) { return larger(a, b); });
 }
 template <class T>
 __device__ __forceinline__ T wave_sum(T v) {
+    return over_wave(v, (T)0, [](T a, T b) { return a + b; });
+}
+
+template <class Key, int N>
+__device__ __forceinline__ void sort_descending(Key (&k)[N]) {
+    // odd-even merge sort of N = 2^i keys
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int q = p; q > 0; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const Key a = k[i + j], b = k[i + j + q];
+                        k[i + j] = larger(a, b);
+                        k[i + j + q] = smaller(a, b);
+                    }
 }
 
 template <int DT>
@@ -71,13 +117,30 @@ __device__ __forceinline__ float logit_at(const void* p, size_t i) {
     else return ((const float*)p)[i];
 }
 
-// softmax terms relative to the row's largest logit (0 where that is -inf, so that exp gives 0)
+// a lane's logits in loads of up to 16 bytes (its share starts on its own size, up to 16 bytes, and is all there)
+template <int DT, int NPL>
+__device__ __forceinline__ void logits_wide(const void* p, size_t at, float (&v)[NPL]) {
+    constexpr int kSize = DT == 2 ? 4 : 2, kBytes = NPL * kSize, kEach = kBytes < 16 ? kBytes : 16;
+    struct alignas(kEach) Piece {
+        uint8_t b[kEach];
+    };
+    union {
+        Piece piece[kBytes / kEach];
+        std::conditional_t<DT == 2, float, uint16_t> x[NPL];
+    } u;
+#pragma unroll
+    for (int i = 0; i < kBytes / kEach; ++i) u.piece[i] = ((const Piece*)((const uint8_t*)p + at * kSize))[i];
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) v[j] = logit_at<DT>(u.x, j);
+}
+
+// the softmax is taken relative to the row's largest logit (to 0 where that is -inf, so that exp gives 0)
 template <class T>
 __device__ __forceinline__ T top_or_0(T top) { return top == -(T)INFINITY ? (T)0 : top; }
 
 template <int NPL, bool BIAS, int DT>
-__global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A) {
-    using Key = std::conditional_t<BIAS, uint64_t, uint32_t>;
+__global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, int wide) {
+    using Key = std::conditional_t<BIAS, double, uint32_t>;
     using Val = std::conditional_t<BIAS, double, float>;
     __shared__ Key lkeys[kRouteWaves][64 * NPL];
     __shared__ Key gkeys[kRouteWaves][kRouteMaxGroups];
@@ -86,67 +149,75 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A) {
     if (row >= A.M) return;
     const size_t base = (size_t)row * A.stride;
     const int e0 = l * NPL;
+    Key* lk = lkeys[wv];
 
     float lg[NPL];
-    uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-        lg[j] = e0 + j < A.E ? logit_at<DT>(A.logits, base + e0 + j) : -INFINITY;
-        most = max(most, e0 + j < A.E ? key_of(lg[j]) : 0u);
+    for (int j = 0; j < NPL; ++j) lg[j] = -INFINITY;
+    if (wide) {
+        if (e0 < A.E) logits_wide<DT>(A.logits, base + e0, lg);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+            if (e0 + j < A.E) lg[j] = logit_at<DT>(A.logits, base + e0 + j);
     }
     // the row's softmax where the keys or the weights need it
     Val top = 0, total = 1;
     if (!A.sigmoid && (BIAS || !A.renormalize)) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) most = max(most, key_of(lg[j]));
         top = top_or_0((Val)value_of(wave_max(most)));
         total = 0;
 #pragma unroll
-        for (int j = 0; j < NPL; ++j)
-            if (e0 + j < A.E) total += BIAS ? exp((double)lg[j] - top) : (Val)expf(lg[j] - (float)top);
+        for (int j = 0; j < NPL; ++j) total += BIAS ? exp((double)lg[j] - top) : (Val)expf(lg[j] - (float)top);
         total = wave_sum(total);
         if (total == 0) total = 1;
     }
     Key key[NPL];
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
+        const bool there = e0 + j < A.E;
         if constexpr (BIAS) {
             const double v = lg[j];
             const double sc = A.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - top) / total;
-            key[j] = e0 + j < A.E ? key_of(sc + (double)A.bias[e0 + j]) : 0;
+            const Key k = key_of(sc + (double)A.bias[there ? e0 + j : 0]);
+            key[j] = there ? k : kNone<Key>;
         } else {
-            key[j] = e0 + j < A.E ? key_of(lg[j]) : 0;
+            const Key k = key_of(lg[j]);
+            key[j] = there ? k : kNone<Key>;
         }
+        lk[e0 + j] = key[j];
     }
+    auto lds_ready = [] {                            // (a wave's own part of LDS)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    lds_ready();
 
     if (A.n_group > 1) {
         const int G = A.n_group, gs = A.E / G;
-        Key* lk = lkeys[wv];
         Key* gk = gkeys[wv];
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) lk[e0 + j] = key[j];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
         // P = the power of two up to 64 / G lanes per group; each lane the two largest of its share, then of the group's
         const int P = 1 << (31 - __builtin_clz(64 / G)), g = l / P;
-        Key t1 = 0, t2 = 0;
+        Key t1 = kNone<Key>, t2 = kNone<Key>;
         if (g < G)
             for (int i = l & (P - 1); i < gs; i += P) {
                 const Key k = lk[g * gs + i];
-                t2 = k > t1 ? t1 : k > t2 ? k : t2;
-                t1 = k > t1 ? k : t1;
+                t2 = larger(t2, smaller(t1, k));
+                t1 = larger(t1, k);
             }
         for (int d = 1; d < P; d *= 2) {
             const Key o1 = __shfl_xor(t1, d), o2 = __shfl_xor(t2, d);
-            const Key lo = t1 > o1 ? o1 : t1, hi2 = t2 > o2 ? t2 : o2;
-            t1 = t1 > o1 ? t1 : o1;
-            t2 = lo > hi2 ? lo : hi2;
+            t2 = larger(smaller(t1, o1), larger(t2, o2));
+            t1 = larger(t1, o1);
         }
         if (g < G && (l & (P - 1)) == 0) {
             if constexpr (BIAS) gk[g] = gs > 1 ? key_of(value_of(t1) + value_of(t2)) : t1;
             else gk[g] = t1;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const Key mine = l < G ? gk[l] : 0;
+        lds_ready();
+        const Key mine = l < G ? gk[l] : kNone<Key>;
         int rank = 0;
         for (int h = 0; h < G; ++h) {
             const Key o = gk[h];
@@ -156,37 +227,46 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A) {
         const uint32_t magic = ((1u << 20) + gs - 1) / gs;      // e / gs for e < 1024 (e * gs < 2^20)
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
-            if (!(kept >> (((uint32_t)(e0 + j) * magic) >> 20) & 1)) key[j] = 0;
+            if (!(kept >> (((uint32_t)(e0 + j) * magic) >> 20) & 1)) lk[e0 + j] = key[j] = kNone<Key>;
+        lds_ready();
     }
 
-    // the picks: lane r keeps pick r
-    Key m = 0;
-    int jm = 0, id = 0;
-    Key picked = 0;
-#pragma unroll
-    for (int j = 0; j < NPL; ++j)
-        if (key[j] > m) m = key[j], jm = j;
+    // the picks: lane r keeps pick r's key, the lane it came from, and how many picks before it took that key from that lane
+    sort_descending(key);
+    Key picked = kNone<Key>, last = kNone<Key>;
+    int from = 0, nth = 0, last_from = -1, n = 0;
     for (int r = 0; r < A.topk; ++r) {
-        const Key wm = wave_max(m);
-        const int win = __builtin_ctzll(__ballot(m == wm));
-        const int e = win * NPL + __builtin_amdgcn_readlane(jm, win);
-        if (l == r) id = e, picked = wm;
-        const int gone = l == win ? jm : -1;
-        m = 0;
-        jm = 0;
+        const Key most = wave_max(key[0]);
+        const uint64_t have = __ballot(key[0] == most);
+        const int win = __builtin_ctzll(have);
+        n = win == last_from && most == last ? n + 1 : 0;
+        last = most;
+        last_from = win;
+        const bool here = l == r;
+        picked = here ? most : picked;
+        from = here ? win : from;
+        nth = here ? n : nth;
+        const bool mine = l == win;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-            if (j == gone) key[j] = 0;
-            if (key[j] > m) m = key[j], jm = j;
+            const Key here = key[j], next = j + 1 < NPL ? key[j + 1] : kNone<Key>;
+            key[j] = mine ? next : here;
         }
     }
-
     const bool live = l < A.topk;
+    int id = from * NPL;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) {                  // the place of the nth (from 0) key of this value
+        const bool same = lk[from * NPL + j] == picked;
+        if (same && nth == 0) id = from * NPL + j;
+        nth -= same;
+    }
+
     float x, w;
     if constexpr (BIAS) x = live ? logit_at<DT>(A.logits, base + id) : -INFINITY;
     else x = live ? value_of(picked) : -INFINITY;
     if (A.sigmoid) w = 1.0f / (1.0f + expf(-x));
-    else if (A.renormalize) w = expf(x - top_or_0(value_of(wave_max(live ? key_of(x) : 0u))));
+    else if (A.renormalize) w = expf(x - top_or_0(BIAS ? value_of(wave_max(live ? key_of(x) : 0u)) : lane_value(x, 0)));
     else w = (float)((BIAS ? exp((double)x - top) : (Val)expf(x - (float)top)) / total);
     if (!live) w = 0;
     if (A.renormalize) {
@@ -202,9 +282,11 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A) {
 template <int NPL, bool BIAS>
 void route_dt(const RouteArgs& a, int dtype, hipStream_t s) {
     const dim3 grid((unsigned)((a.M + (int64_t)kRouteWaves - 1) / kRouteWaves)), block(64 * kRouteWaves);
-    if (dtype == 0) hipLaunchKernelGGL((route_kernel<NPL, BIAS, 0>), grid, block, 0, s, a);
-    else if (dtype == 1) hipLaunchKernelGGL((route_kernel<NPL, BIAS, 1>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((route_kernel<NPL, BIAS, 2>), grid, block, 0, s, a);
+    const int esz = dtype == 2 ? 4 : 2, each = NPL * esz < 16 ? NPL * esz : 16;
+    const int wide = a.E % NPL == 0 && (uintptr_t)a.logits % each == 0 && a.stride * esz % each == 0;
+    if (dtype == 0) hipLaunchKernelGGL((route_kernel<NPL, BIAS, 0>), grid, block, 0, s, a, wide);
+    else if (dtype == 1) hipLaunchKernelGGL((route_kernel<NPL, BIAS, 1>), grid, block, 0, s, a, wide);
+    else hipLaunchKernelGGL((route_kernel<NPL, BIAS, 2>), grid, block, 0, s, a, wide);
 }
 
 template <int NPL>
