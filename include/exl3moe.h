@@ -381,7 +381,8 @@ int exl3_fp8_quant(const void* x, int x_dtype, int64_t x_stride, int M, int k, v
 int exl3_fp8_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int M, int k, void* q, float* s, void* stream);
 /* out[m][n] = sum over blocks b of s[m][b] sw[n / 128][b] (sum over k in b of q[m][k] w[n][k]) + bias[n], fp32 sums, rounded
  * once to out_dtype. q, s as above; w: e4m3 [n, kp], zeros behind column k; sw: fp32 [ceil(n / 128), kp / 128]; bias: fp32
- * [n] or NULL; q and w start on 16 bytes. workspace: exl3_fp8_matmul_workspace bytes, no state between calls; its size
+ * [n] or NULL; q and w start on 16 bytes. For fp16 and bf16 outputs the sums of 128 products may be off by 7 * 2^-13 of
+ * their products' magnitudes at most (1.5e-5 of the output's size for normal values), for fp32 by no more than fp32 sums. workspace: exl3_fp8_matmul_workspace bytes, no state between calls; its size
  * never falls as M grows. */
 size_t exl3_fp8_matmul_workspace(int M, int k, int n);
 int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
@@ -391,6 +392,13 @@ size_t exl3_fp8_linear_workspace(int M, int k, int n);
 int exl3_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const float* sw,
                     const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                     size_t workspace_bytes, void* stream);
+/* A gated MLP: exl3_fp8_linear of x [M, k] with gate|up weights of 2 I rows (gu: [2 I, k up to a multiple of 128], scales
+ * gu_scale, gu_bias fp32 [2 I] or NULL) whose sums are as exact as those of fp32 outputs, rounded to `dtype`, then silu(gate) * up quantised and multiplied with the down
+ * weights (dn: [n, I up to a multiple of 128], dn_scale, dn_bias fp32 [n] or NULL). x and out are of `dtype`. */
+size_t exl3_fp8_mlp_workspace(int M, int k, int I, int n, int dtype);
+int exl3_fp8_mlp(const void* x, int dtype, int64_t x_stride, int M, int k, int I, int n, const void* gu,
+                 const float* gu_scale, const float* gu_bias, const void* dn, const float* dn_scale, const float* dn_bias,
+                 void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,10 +20,10 @@ BUILD = os.path.join(HERE, "_build")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 ARCH = "gfx950"
 
-HIP_SOURCES = ["fp8_tiles_f32.hip", "fp8_tiles_f16.hip", "moe_route.hip", "moe_products_k3.hip", "moe_products_k2.hip", "moe_products_k4.hip", "linear_rows_k4.hip",
+HIP_SOURCES = ["moe_products_k3.hip", "moe_products_k2.hip", "moe_products_k4.hip", "linear_rows_k4.hip",
                "linear_rows_k23.hip", "linear_rows_k56.hip", "linear_rows_k6.hip", "moe_decode.hip", "linear.hip",
-               "moe_cache.hip", "moe_align.hip", "moe_grouped.hip", "linear_rows.hip", "moe_capi.hip",
-               "fp8_linear.hip", "fp8_rows.hip"]
+               "moe_cache.hip", "moe_align.hip", "moe_grouped.hip", "linear_rows.hip", "moe_capi.hip", "moe_route.hip",
+               "fp8_tiles_exact.hip", "fp8_tiles_e4m3.hip", "fp8_linear.hip", "fp8_rows.hip"]
 HOST_SOURCES = ["tier_host.cpp"]          # host-only C++ (g++)
 HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",
                "-packed-fp32-ops", "-Wno-unused-command-line-argument"]

@@ -271,6 +271,7 @@ struct Fp8ProductArgs {
     void* out; int64_t out_stride;
     const void* x; int64_t x_stride; int k, x_dt;  // rows as Fp8RowsArgs has them
     bool silu, x_wide;
+    bool exact;                                    // sums without the e4m3 MFMA's losses (fp32 outputs always have them)
 };
 // whether the product quantises its rows itself (no launch_fp8_rows before it)
 bool fp8_product_quantises(int M, int k, int n);

@@ -14,8 +14,8 @@
 
 namespace exl3 {
 
-void launch_fp8_tile_16(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st);
-void launch_fp8_tile_32(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st);
+void launch_fp8_tile_e4m3(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st);
+void launch_fp8_tile_exact(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st);
 
 namespace {
 constexpr int kCus = 256;
@@ -31,7 +31,7 @@ bool fp8_product_quantises(int M, int k, int n) {
 
 hipError_t launch_fp8_product(const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
     constexpr int kSizes[][2] = {{16, 16}, {16, 32}, {32, 32}, {64, 64}, {128, 128}, {256, 256}};
-    const bool exact = out_dt == 2;
+    const bool exact = a.exact || out_dt == 2;
     int tile = 0;
     bool few = true;
     for (int64_t i = 0, least = 0; i < (!a.q ? kTile16x32 : exact ? kTile128 : kTile256) + 1; ++i) {
@@ -40,8 +40,8 @@ hipError_t launch_fp8_product(const Fp8ProductArgs& a, int out_dt, hipStream_t s
         const int64_t bytes = (tiles > kCus ? tiles : kCus) * (bm + bn);
         if (i == 0 || bytes < least) least = bytes, tile = (int)i, few = tiles <= kCus;
     }
-    if (exact) launch_fp8_tile_32(tile, few, a, out_dt, st);
-    else launch_fp8_tile_16(tile, few, a, out_dt, st);
+    if (exact) launch_fp8_tile_exact(tile, few, a, out_dt, st);
+    else launch_fp8_tile_e4m3(tile, few, a, out_dt, st);
     return hipGetLastError();
 }
 

@@ -40,8 +40,9 @@ __device__ __forceinline__ Frag<EXACT> frag_of(v4i a, v4i b) {
 
 // The sum over one block. The e4m3 MFMA adds products in groups of 8 k, aligned to the group's largest and cut 13 bits
 // below its leading one (1.5e-5 of the sum's own size for normal values, up to 1.7e-4 of the magnitudes for wild ones):
-// far below the rounding of bf16 or fp16 outputs, and not what fp32 outputs promise. Those take the bf16 MFMA on the same
-// values (products exact, fp32 sums: 3e-8), at half the rate and with the conversions.
+// far below the rounding of bf16 or fp16 outputs. fp32 outputs promise more, and so do sums that are quantised again (there
+// 1.5e-5 takes 3e-4 of the values over a border between two of e4m3's, 1.5e-3 in what they are multiplied to): those take the
+// bf16 MFMA on the same values (products exact, fp32 sums: 3e-8), at half the rate and with the conversions.
 __device__ __forceinline__ v4f block_sum(const Frag<false>& a, const Frag<false>& b) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
 }
@@ -145,7 +146,7 @@ __device__ __forceinline__ void quant_rows(const Fp8ProductArgs& A, uint8_t* q, 
 // A workgroup computes BM rows x BN columns: KG groups of WM x WN waves, of which group i takes the blocks of k i, KG + i, ...
 // and brings them to LDS by direct loads, ST stages of its own. The groups' sums join at the end, in the groups' order. OWN:
 // the workgroup quantises its (up to 16) rows itself while its first weights are on their way, and `own` is their LDS.
-// EXACT: fp32 outputs from sums without the e4m3 MFMA's losses; else fp16 (out_dt 0) or bf16 outputs.
+// EXACT: sums without the e4m3 MFMA's losses, outputs in fp16, bf16 or fp32 (out_dt 0, 1, 2); else fp16 or bf16 outputs.
 template <bool EXACT, bool OWN, int BM, int BN, int WM, int WN, int KG, int ST>
 __global__ void __launch_bounds__(64 * WM * WN * KG) fp8_tile_kernel(Fp8ProductArgs A, int mt, int nt, int per, int out_dt) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, QB = OWN ? 0 : BM;
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp8_tile_kernel(Fp8ProductA
                 const int n = n0 + wn + i * 16 + g * 4 + c;
                 bias[i][c] = n < A.n ? A.bias[n] : 0.0f;
             }
-    if constexpr (EXACT) {
+    if (EXACT && out_dt == 2) {
         // a lane's four columns at once where they are there and every row's fours start on 16 bytes
         const bool wide = A.n % 4 == 0 && A.out_stride % 4 == 0 && (uintptr_t)A.out % 16 == 0;
 #pragma unroll

@@ -1360,6 +1360,25 @@ size_t exl3_fp8_matmul_workspace(int M, int k, int n) {
     return 0;
 }
 
+namespace {
+
+// the product of quantised rows, or (q null) of rows that it quantises itself, which `a` has then; arguments checked, M > 0
+int fp8_product(const char* what, Fp8ProductArgs a, int M, int k, int n, const void* w, const float* sw, const float* bias,
+                void* out, int out_dtype, int64_t out_stride, void* stream) {
+    a.w = (const uint8_t*)w;
+    a.sw = sw;
+    a.bias = bias;
+    a.M = M;
+    a.n = n;
+    a.kb = fp8_blocks(k);
+    a.out = out;
+    a.out_stride = out_stride;
+    const hipError_t e = launch_fp8_product(a, out_dtype, (hipStream_t)stream);
+    return e == hipSuccess ? EXL3_OK : hip_fail(e, what);
+}
+
+}  // namespace
+
 int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
                     void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
     if (int r = fp8_product_checks("fp8_matmul", M, k, n, w, sw, bias, out, out_dtype, out_stride)) return r;
@@ -1371,16 +1390,7 @@ int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const vo
     Fp8ProductArgs a{};
     a.q = (const uint8_t*)q;
     a.s = s;
-    a.w = (const uint8_t*)w;
-    a.sw = sw;
-    a.bias = bias;
-    a.M = M;
-    a.n = n;
-    a.kb = fp8_blocks(k);
-    a.out = out;
-    a.out_stride = out_stride;
-    const hipError_t e = launch_fp8_product(a, out_dtype, (hipStream_t)stream);
-    return e == hipSuccess ? EXL3_OK : hip_fail(e, "fp8_matmul launch");
+    return fp8_product("fp8_matmul launch", a, M, k, n, w, sw, bias, out, out_dtype, out_stride, stream);
 }
 
 size_t exl3_fp8_linear_workspace(int M, int k, int n) {
@@ -1388,41 +1398,74 @@ size_t exl3_fp8_linear_workspace(int M, int k, int n) {
     return fp8_q_bytes(M, k) + fp8_s_bytes(M, k) + exl3_fp8_matmul_workspace(M, k, n);
 }
 
+namespace {
+
+// the product of rows that are quantised within the call, of x or (silu) of gate|up rows x; arguments checked, M > 0
+int fp8_rows_product(const char* what, const void* x, int x_dtype, int64_t x_stride, bool silu, bool exact, int M, int k, int n,
+                     const void* w, const float* sw, const float* bias, void* out, int out_dtype, int64_t out_stride,
+                     void* workspace, void* stream) {
+    Fp8ProductArgs a{};
+    a.exact = exact;
+    if (fp8_product_quantises(M, k, n)) {
+        a.x = x;
+        a.x_stride = x_stride;
+        a.x_dt = x_dtype;
+        a.k = k;
+        a.silu = silu;
+        a.x_wide = fp8_rows_wide(x, x_stride, k, x_dtype);
+    } else {
+        uint8_t* q = (uint8_t*)workspace;
+        float* s = (float*)(q + fp8_q_bytes(M, k));
+        if (int r = fp8_rows(what, x, x_dtype, x_stride, M, k, silu, q, s, stream)) return r;
+        a.q = q;
+        a.s = s;
+    }
+    return fp8_product(what, a, M, k, n, w, sw, bias, out, out_dtype, out_stride, stream);
+}
+
+}  // namespace
+
 int exl3_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const float* sw,
                     const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                     size_t workspace_bytes, void* stream) {
     if (int r = fp8_product_checks("fp8_linear", M, k, n, w, sw, bias, out, out_dtype, out_stride)) return r;
     if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "fp8_linear: x dtype %d", x_dtype);
     if (M == 0) return EXL3_OK;
-    if (!x || x_stride < k) return fail(EXL3_EINVAL, "fp8_linear: x null or row stride %lld", (long long)x_stride);
+    if (!x || x_stride < k || !aligned(x, dt_size(x_dtype)))
+        return fail(EXL3_EINVAL, "fp8_linear: x null, its alignment or row stride %lld", (long long)x_stride);
     const size_t need = exl3_fp8_linear_workspace(M, k, n);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return fail(EXL3_EWORKSPACE, "fp8_linear: workspace of %zu bytes on 16, got %zu", need, workspace_bytes);
-    if (fp8_product_quantises(M, k, n)) {
-        if (!aligned(x, dt_size(x_dtype))) return fail(EXL3_EINVAL, "fp8_linear: alignment of x");
-        Fp8ProductArgs a{};
-        a.x = x;
-        a.x_stride = x_stride;
-        a.x_dt = x_dtype;
-        a.k = k;
-        a.x_wide = fp8_rows_wide(x, x_stride, k, x_dtype);
-        a.w = (const uint8_t*)w;
-        a.sw = sw;
-        a.bias = bias;
-        a.M = M;
-        a.n = n;
-        a.kb = fp8_blocks(k);
-        a.out = out;
-        a.out_stride = out_stride;
-        const hipError_t e = launch_fp8_product(a, out_dtype, (hipStream_t)stream);
-        return e == hipSuccess ? EXL3_OK : hip_fail(e, "fp8_linear launch");
-    }
-    uint8_t* q = (uint8_t*)workspace;
-    float* s = (float*)(q + fp8_q_bytes(M, k));
-    if (int r = fp8_rows("fp8_linear", x, x_dtype, x_stride, M, k, false, q, s, stream)) return r;
-    uint8_t* rest = (uint8_t*)s + fp8_s_bytes(M, k);
-    return exl3_fp8_matmul(q, s, M, k, n, w, sw, bias, out, out_dtype, out_stride, rest,
-                           workspace_bytes - (size_t)(rest - q), stream);
+    return fp8_rows_product("fp8_linear", x, x_dtype, x_stride, false, false, M, k, n, w, sw, bias, out, out_dtype, out_stride,
+                            workspace, stream);
+}
+
+size_t exl3_fp8_mlp_workspace(int M, int k, int I, int n, int dtype) {
+    if (M <= 0 || k <= 0 || I <= 0 || I > 1 << 26 || n <= 0 || !dt_ok(dtype)) return 0;
+    return align256((size_t)M * 2 * I * dt_size(dtype)) +
+           std::max(exl3_fp8_linear_workspace(M, k, 2 * I), exl3_fp8_linear_workspace(M, I, n));
+}
+
+int exl3_fp8_mlp(const void* x, int dtype, int64_t x_stride, int M, int k, int I, int n, const void* gu,
+                 const float* gu_scale, const float* gu_bias, const void* dn, const float* dn_scale, const float* dn_bias,
+                 void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    if (I <= 0 || I > 1 << 26) return fail(EXL3_EINVAL, "fp8_mlp: I=%d", I);
+    const size_t need = exl3_fp8_mlp_workspace(M, k, I, n, dtype);
+    uint8_t* rest = (uint8_t*)workspace + (M > 0 && dt_ok(dtype) ? align256((size_t)M * 2 * I * dt_size(dtype)) : 0);
+    if (int r = fp8_product_checks("fp8_mlp (gate|up)", M, k, 2 * I, gu, gu_scale, gu_bias, workspace, dtype, 2 * (int64_t)I))
+        return r;
+    if (int r = fp8_product_checks("fp8_mlp (down)", M, I, n, dn, dn_scale, dn_bias, out, dtype, out_stride)) return r;
+    if (M == 0) return EXL3_OK;
+    if (!x || x_stride < k || !aligned(x, dt_size(dtype)))
+        return fail(EXL3_EINVAL, "fp8_mlp: x null, its alignment or row stride %lld", (long long)x_stride);
+    if (workspace_bytes < need || !aligned(workspace, 16))
+        return fail(EXL3_EWORKSPACE, "fp8_mlp: workspace of %zu bytes on 16, got %zu", need, workspace_bytes);
+    // (gate|up sums are quantised again)
+    if (int r = fp8_rows_product("fp8_mlp (gate|up)", x, dtype, x_stride, false, true, M, k, 2 * I, gu, gu_scale, gu_bias,
+                                 workspace, dtype, 2 * (int64_t)I, rest, stream))
+        return r;
+    return fp8_rows_product("fp8_mlp (down)", workspace, dtype, 2 * (int64_t)I, true, false, M, I, n, dn, dn_scale, dn_bias,
+                            out, dtype, out_stride, rest, stream);
 }
 
 }  // extern "C"

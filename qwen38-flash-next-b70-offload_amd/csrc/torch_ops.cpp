@@ -584,6 +584,35 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor
     return out;
 }
 
+at::Tensor fp8_mlp(const at::Tensor& x, const at::Tensor& gu, const at::Tensor& gu_scale,
+                   const std::optional<at::Tensor>& gu_bias, const at::Tensor& dn, const at::Tensor& dn_scale,
+                   const std::optional<at::Tensor>& dn_bias) {
+    const c10::DeviceGuard guard(x.device());
+    const int dt = dtype_code(x);
+    auto x2 = rows_of(x, "fp8_mlp");
+    const int M = (int)x2.size(0), k = (int)x2.size(1);
+    fp8_weight_checks(x, gu, gu_scale, k, "fp8_mlp (gate|up)");
+    TORCH_CHECK(gu.size(0) % 2 == 0, "fp8_mlp: gate|up weights of an even number of rows, got ", gu.sizes());
+    const int64_t I = gu.size(0) / 2, n = dn.size(0);
+    fp8_weight_checks(x, dn, dn_scale, I, "fp8_mlp (down)");
+    const float* gb = f32_or_null(gu_bias, x, 2 * I, "fp8_mlp (gate|up)");
+    const float* db = f32_or_null(dn_bias, x, n, "fp8_mlp (down)");
+    auto out = at::empty(with_last(x.sizes(), n), x.options());
+    if (M == 0) return out;
+    const size_t ws = exl3_fp8_mlp_workspace(M, k, (int)I, (int)n, dt);
+    auto buf = at::empty({(int64_t)ws}, x.options().dtype(at::kByte));
+    check(exl3_fp8_mlp(x2.data_ptr(), dt, row_stride(x2), M, k, (int)I, (int)n, gu.data_ptr(), gu_scale.data_ptr<float>(),
+                       gb, dn.data_ptr(), dn_scale.data_ptr<float>(), db, out.data_ptr(), n, buf.data_ptr(), ws,
+                       cur_stream(x)),
+          "fp8_mlp");
+    return out;
+}
+
+at::Tensor fp8_mlp_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
+                        const at::Tensor& dn, const at::Tensor&, const std::optional<at::Tensor>&) {
+    return at::empty(with_last(x.sizes(), dn.size(0)), x.options());
+}
+
 at::Tensor fp8_linear_meta(const at::Tensor& x, const at::Tensor& w, const at::Tensor&, const std::optional<at::Tensor>&) {
     return at::empty(with_last(x.sizes(), w.size(0)), x.options());
 }
@@ -645,6 +674,10 @@ TORCH_LIBRARY(exl3xpu_C, m) {
     m.def("fp8_linear(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias=None) -> Tensor");
     m.impl("fp8_linear", c10::DispatchKey::CUDA, &fp8_linear);
     m.impl("fp8_linear", c10::DispatchKey::Meta, &fp8_linear_meta);
+    m.def("fp8_mlp(Tensor x, Tensor gate_up, Tensor gate_up_scale, Tensor? gate_up_bias, Tensor down, Tensor down_scale, "
+          "Tensor? down_bias) -> Tensor");
+    m.impl("fp8_mlp", c10::DispatchKey::CUDA, &fp8_mlp);
+    m.impl("fp8_mlp", c10::DispatchKey::Meta, &fp8_mlp_meta);
     m.def("fp8_matmul(Tensor q, Tensor s, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType dtype) -> Tensor");
     m.impl("fp8_matmul", c10::DispatchKey::CUDA, &fp8_matmul);
     m.impl("fp8_matmul", c10::DispatchKey::Meta, &fp8_matmul_meta);

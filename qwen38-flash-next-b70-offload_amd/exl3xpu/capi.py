@@ -90,6 +90,9 @@ SIGNATURES = {
     "exl3_fp8_linear_workspace": (c_sz, [c_i32, c_i32, c_i32]),
     "exl3_fp8_linear": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_i32, c_p, c_p, c_p, c_p, c_i32, c_i64, c_p, c_sz,
                                 c_p]),
+    "exl3_fp8_mlp_workspace": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "exl3_fp8_mlp": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_p,
+                             c_sz, c_p]),
     "exl3_had_out_q8": (c_i32, [c_p, c_i32, c_i32, c_p, ctypes.c_float, c_p, c_p, c_i32, c_i64, c_p]),
 }
 

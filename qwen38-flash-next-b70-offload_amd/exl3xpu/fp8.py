@@ -52,17 +52,17 @@ class Fp8Linear:
         self.weight = (torch.nn.functional.pad(raw, (0, pad)) if pad else raw.contiguous()).view(torch.float8_e4m3fn)
         self.weight_scale = weight_scale.detach().to(device, torch.float32).contiguous()
         self.bias = None if bias is None else bias.detach().to(device, torch.float32).contiguous()
-        self._op = _C()
+        self._linear, self._matmul = _C().fp8_linear.default, _C().fp8_matmul.default
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         """x [..., k] fp16 / bf16 / fp32 -> [..., n] of x's dtype."""
         if x.size(-1) != self.k:                  # (the op takes any k that the padded weight has room for)
             raise ValueError(f"exl3xpu: rows of {self.k}, got {tuple(x.shape)}")
-        return self._op.fp8_linear(x, self.weight, self.weight_scale, self.bias)
+        return self._linear(x, self.weight, self.weight_scale, self.bias)
 
     def quantised(self, q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         """The product of rows that are quantised already (q, s of quant or silu_mul_quant) -> [..., n] of dtype."""
-        return self._op.fp8_matmul(q, s, self.weight, self.weight_scale, self.bias, dtype)
+        return self._matmul(q, s, self.weight, self.weight_scale, self.bias, dtype)
 
 
 class Fp8Mlp:
@@ -73,9 +73,11 @@ class Fp8Mlp:
         if gate_up.n != 2 * down.k:
             raise ValueError(f"exl3xpu: gate|up of {gate_up.n} columns does not fit a down of {down.k} inputs")
         self.gate_up, self.down = gate_up, down
-        self._op = _C()
+        self._weights = [t for lin in (gate_up, down) for t in (lin.weight, lin.weight_scale, lin.bias)]
+        self._op = _C().fp8_mlp.default
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         """x [..., k] -> [..., n] of x's dtype; gate|up is rounded to x's dtype between the two products."""
-        q, s = self._op.fp8_silu_mul_quant(self.gate_up(x))
-        return self.down.quantised(q, s, x.dtype)
+        if x.size(-1) != self.gate_up.k:
+            raise ValueError(f"exl3xpu: rows of {self.gate_up.k}, got {tuple(x.shape)}")
+        return self._op(x, *self._weights)

@@ -25,6 +25,11 @@ def _fp8():
     return fp8
 
 
+def linear_ops():
+    from exl3xpu.linear import C
+    return C()
+
+
 def _gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
@@ -283,7 +288,7 @@ def test_refusals():
     g = _gen(27)
     w, sw = _weight(g, 256, 256)
     lin = _fp8().Fp8Linear(w, sw)
-    C = lin._op
+    C = linear_ops()
     x = torch.randn(4, 256, generator=g, device="cuda").bfloat16()
     q, s = _fp8().quant(x)
     bad = [lambda: lin(x[:, :255]), lambda: lin(x.double()), lambda: lin(x.to(torch.float8_e4m3fn)),
@@ -295,6 +300,9 @@ def test_refusals():
            lambda: C.fp8_matmul(q[:, :200], s, w, sw, None, torch.bfloat16),
            lambda: C.fp8_matmul(q, s, w, sw, None, torch.int32),
            lambda: C.fp8_matmul(q.view(torch.float8_e5m2), s, w, sw, None, torch.bfloat16),
+           lambda: C.fp8_mlp(x, w, sw, None, w, sw, None), lambda: C.fp8_mlp(x, w[:255], sw, None, w[:, :128], sw[:, :1], None),
+           lambda: C.fp8_mlp(x, w, sw, None, w[:, :128].contiguous(), sw[:, :1], None),
+           lambda: _fp8().Fp8Mlp(lin, _fp8().Fp8Linear(w[:, :128], sw[:, :1]))(x[:, :200]),
            lambda: _fp8().quant(x.int()), lambda: _fp8().quant(x[:, :0]), lambda: _fp8().silu_mul_quant(x[:, :255])]
     for i, f in enumerate(bad):
         with pytest.raises((RuntimeError, ValueError)):
@@ -313,11 +321,18 @@ def _mlp(g, k, I):  # noqa: E741
 def test_mlp_is_its_parts(M):
     g = _gen(31)
     for k, I in ((2048, 512), (512, 640), (300, 200)):  # noqa: E741
-        mlp = _mlp(g, k, I)
-        x = torch.randn(M, k, generator=g, device="cuda").bfloat16()
-        gu = mlp.gate_up(x)
-        q, s = _fp8().silu_mul_quant(gu)
-        assert torch.equal(mlp(x), mlp.down.quantised(q, s, x.dtype))
+        fp8 = _fp8()
+        for bias in (False, True):
+            b = [torch.randn(n, generator=g, device="cuda") if bias else None for n in (2 * I, k)]
+            mlp = fp8.Fp8Mlp(fp8.Fp8Linear(*_weight(g, 2 * I, k), b[0]), fp8.Fp8Linear(*_weight(g, k, I), b[1]))
+            for dtype in DTYPES:
+                print(f"case fp8 mlp M={M} k={k} I={I} bias={bias} {dtype}", flush=True)
+                x = torch.randn(M, k, generator=g, device="cuda").to(dtype)
+                # gate|up with the sums of fp32 outputs, rounded to the type once
+                gu = mlp.gate_up.quantised(*fp8.quant(x), torch.float32).to(dtype)
+                want = mlp.down.quantised(*fp8.silu_mul_quant(gu), dtype)
+                assert torch.equal(mlp(x), want) and torch.equal(mlp(_odd(x)), want)
+                assert mlp(x[:0]).shape == (0, k) and torch.equal(mlp(x[None]), want[None])
 
 
 def _layer(g, M):

@@ -60,6 +60,22 @@ def test_products_refuse(k, code):
     assert _linear(**k) == code
 
 
+def _mlp(x=P, dt=1, xs=256, M=4, k=256, I=128, n=256, gu=P, gs=P, gb=None, dn=P, ds=P, db=None, out=P, stride=256, ws=P,  # noqa: E741
+         size=1 << 40):
+    return capi.lib().exl3_fp8_mlp(x, dt, xs, M, k, I, n, gu, gs, gb, dn, ds, db, out, stride, ws, size, None)
+
+
+@pytest.mark.parametrize("k,code", [
+    (dict(k=0), BAD), (dict(I=0), BAD), (dict(I=1 << 27), BAD), (dict(n=0), BAD), (dict(M=-1), BAD), (dict(dt=3), BAD),
+    (dict(dt=-1), BAD), (dict(x=None), BAD), (dict(x=P + 1), BAD), (dict(xs=255), BAD), (dict(gu=None), BAD),
+    (dict(gu=P + 8), BAD), (dict(gs=None), BAD), (dict(gb=P + 2), BAD), (dict(dn=None), BAD), (dict(dn=P + 4), BAD),
+    (dict(ds=P + 1), BAD), (dict(db=P + 2), BAD), (dict(out=None), BAD), (dict(out=P + 1), BAD), (dict(stride=255), BAD),
+    (dict(ws=None), BAD), (dict(ws=P + 2), WORKSPACE), (dict(size=100), WORKSPACE), (dict(k=1 << 23, xs=1 << 23), UNSUPPORTED),
+    (dict(M=0, x=None, ws=None), 0)])
+def test_mlp_refuses(k, code):
+    assert _mlp(**k) == code
+
+
 def test_products_refuse_their_own():
     assert [_matmul(q=None), _matmul(s=None), _matmul(q=P + 8), _matmul(s=P + 2)] == [BAD] * 4
     assert [_linear(x=None), _linear(dtype=3), _linear(xs=255), _linear(x=P + 1)] == [BAD] * 4
@@ -76,6 +92,14 @@ def test_workspaces_never_fall_as_the_rows_grow(k, n):
         assert [f(0, k, n), f(-5, k, n), f(4, 0, n), f(4, k, -1)] == [0] * 4
 
 
+def test_mlp_workspace():
+    f = capi.lib().exl3_fp8_mlp_workspace
+    for dt in (0, 1, 2):
+        b = [f(M, 2048, 512, 2048, dt) for M in [*range(1, 300), 1024, 60000]]
+        assert all(x <= y for x, y in zip(b, b[1:])) and b[0] >= 1024 * (4 if dt == 2 else 2)
+    assert [f(0, 8, 8, 8, 0), f(1, 0, 8, 8, 0), f(1, 8, -1, 8, 0), f(1, 8, 8, 0, 0), f(1, 8, 8, 8, 5), f(1, 8, 1 << 27, 8, 0)] == [0] * 6
+
+
 def test_shapes_without_a_device():
     m = torch.device("meta")
     ids, w = ops().moe_route(torch.empty(3, 5, 64, device=m), None, 6, "softmax", 1, 1, True, 1.0)
@@ -87,6 +111,9 @@ def test_shapes_without_a_device():
     w8, sw = torch.empty(130, 384, device=m, dtype=torch.float8_e4m3fn), torch.empty(2, 3, device=m)
     y = C().fp8_linear(torch.empty(2, 7, 300, device=m, dtype=torch.float16), w8, sw, None)
     assert y.shape == (2, 7, 130) and y.dtype == torch.float16
+    m = C().fp8_mlp(torch.empty(2, 7, 300, device=m), w8, sw, None, torch.empty(90, 128, device=m, dtype=w8.dtype),
+                    torch.empty(1, 1, device=m), None)
+    assert m.shape == (2, 7, 90) and m.dtype == torch.float32
     y = C().fp8_matmul(q, s, w8, sw, None, torch.bfloat16)
     assert y.shape == (2, 7, 130) and y.dtype == torch.bfloat16
 
