@@ -18,7 +18,6 @@ void launch_fp8_tile_e4m3(int tile, bool few, const Fp8ProductArgs& a, int out_d
 void launch_fp8_tile_exact(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st);
 
 namespace {
-constexpr int kCus = 256;
 // rows up to which the product quantises them itself, and their blocks of 128: as many as a workgroup quantises at once
 constexpr int kOwnRows = 16, kOwnBlocks = 128;
 }  // namespace

@@ -51,7 +51,8 @@ __device__ __forceinline__ float silu_times(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(p, e * kLn2, p)) * u;
 }
 
-// 8 consecutive elements of a row as fp32. WIDE: 16-byte aligned and all inside the row; else one by one, 0 from `n` on
+// 8 consecutive elements of a row as fp32. WIDE: 16-byte aligned and all inside the row; else one by one, from the `n`-th on
+// (n > 0) the last one again
 template <int DT, bool WIDE>
 __device__ __forceinline__ void load8(const void* x, size_t at, int n, float (&v)[8]) {
     if constexpr (WIDE) {
@@ -77,10 +78,10 @@ __device__ __forceinline__ void load8(const void* x, size_t at, int n, float (&v
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (j >= n) v[j] = 0.0f;
-            else if constexpr (DT == 0) v[j] = (float)((const _Float16*)x)[at + j];
-            else if constexpr (DT == 1) v[j] = __builtin_bit_cast(float, (uint32_t)((const uint16_t*)x)[at + j] << 16);
-            else v[j] = ((const float*)x)[at + j];
+            const size_t i = at + min(j, n - 1);
+            if constexpr (DT == 0) v[j] = (float)((const _Float16*)x)[i];
+            else if constexpr (DT == 1) v[j] = __builtin_bit_cast(float, (uint32_t)((const uint16_t*)x)[i] << 16);
+            else v[j] = ((const float*)x)[i];
         }
     }
 }
@@ -98,18 +99,18 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
 // number, also negative) lie inside the row, the others are 0
 template <int DT, bool SILU, bool WIDE>
 __device__ __forceinline__ void block_values(const void* x, size_t at, int k, int n, float (&v)[8]) {
-    // (no branch where a whole group of 8 is loaded or none: the row before any other takes the place of none)
-    if (WIDE) at = n > 0 ? at : 0;
-    load8<DT, WIDE>(x, at, n, v);
+    // (no branches: the rows' first elements are loaded for none)
+    at = n > 0 ? at : 0;
+    const int some = max(n, 1);
+    load8<DT, WIDE>(x, at, some, v);
     if constexpr (SILU) {
         float u[8];
-        load8<DT, WIDE>(x, at + k, n, u);
+        load8<DT, WIDE>(x, at + k, some, u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = silu_times(v[j], u[j]);
     }
-    if (WIDE)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = n > 0 ? v[j] : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = (WIDE ? 0 : j) < n ? v[j] : 0.0f;
 }
 
 // the 8 values' e4m3 and the scale of the block that the 16 lanes of a DPP row hold
