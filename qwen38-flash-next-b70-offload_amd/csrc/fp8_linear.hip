@@ -10,7 +10,6 @@
 // - / -, 16 x 32 5.1 / 5.4 / 8.2 / - / -, 32 x 32 6.0 / 6.4 / 6.6 / 17.3 / -, 64 x 64 9.3 / 9.6 / 9.6 / 11.3 / 34,
 // 128 x 128 17 / 18 / 18 / 22 / 27, 256 x 256 40 / 40 / 41 / 43 / 45.
 #include "exl3_kernels.h"
-#include "fp8_tiles.cuh"
 
 namespace exl3 {
 
@@ -18,29 +17,38 @@ void launch_fp8_tile_e4m3(int tile, bool few, const Fp8ProductArgs& a, int out_d
 void launch_fp8_tile_exact(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st);
 
 namespace {
-// rows up to which the product quantises them itself, and their blocks of 128: as many as a workgroup quantises at once
-constexpr int kOwnRows = 16, kOwnBlocks = 128;
+
+struct Pick {
+    int tile;
+    bool few;                                        // at most one workgroup per CU
+};
+Pick pick_tile(int M, int n, int largest) {
+    constexpr int kSizes[][2] = {{16, 16}, {16, 32}, {32, 32}, {64, 64}, {128, 128}, {256, 256}};
+    Pick best{};
+    int64_t least = 0;
+    for (int i = 0; i <= largest; ++i) {
+        const int bm = kSizes[i][0], bn = kSizes[i][1];
+        const int64_t tiles = (int64_t)((M - 1) / bm + 1) * ((n - 1) / bn + 1);
+        const int64_t bytes = (tiles > kCus ? tiles : kCus) * (bm + bn);
+        if (i == 0 || bytes < least) least = bytes, best = {i, tiles <= kCus};
+    }
+    return best;
+}
+
 }  // namespace
 
+// As many blocks of 128 as the workgroup has in hand at once (4 for each 16 lanes): 8 of 512 threads at 16 columns, 4 of 256
+// at 32. More rows are quantised by a launch of their own: 2048 -> 1024, 8 rows 5.1 us, by two launches 6.1; 4096 -> 2048, 8
+// rows 8.0 us, by two launches 7.4.
 bool fp8_product_quantises(int M, int k, int n) {
-    (void)n;
-    const int kb = fp8_blocks(k);
-    return M <= kOwnRows && (int64_t)M * kb <= kOwnBlocks;
+    return M <= 16 && (int64_t)M * fp8_blocks(k) <= (pick_tile(M, n, kTile16x32).tile == kTile16 ? 128 : 64);
 }
 
 hipError_t launch_fp8_product(const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
-    constexpr int kSizes[][2] = {{16, 16}, {16, 32}, {32, 32}, {64, 64}, {128, 128}, {256, 256}};
     const bool exact = a.exact || out_dt == 2;
-    int tile = 0;
-    bool few = true;
-    for (int64_t i = 0, least = 0; i < (!a.q ? kTile16x32 : exact ? kTile128 : kTile256) + 1; ++i) {
-        const int bm = kSizes[i][0], bn = kSizes[i][1];
-        const int64_t tiles = (int64_t)((a.M - 1) / bm + 1) * ((a.n - 1) / bn + 1);
-        const int64_t bytes = (tiles > kCus ? tiles : kCus) * (bm + bn);
-        if (i == 0 || bytes < least) least = bytes, tile = (int)i, few = tiles <= kCus;
-    }
-    if (exact) launch_fp8_tile_exact(tile, few, a, out_dt, st);
-    else launch_fp8_tile_e4m3(tile, few, a, out_dt, st);
+    const Pick p = pick_tile(a.M, a.n, !a.q ? kTile16x32 : exact ? kTile128 : kTile256);
+    if (exact) launch_fp8_tile_exact(p.tile, p.few, a, out_dt, st);
+    else launch_fp8_tile_e4m3(p.tile, p.few, a, out_dt, st);
     return hipGetLastError();
 }
 
