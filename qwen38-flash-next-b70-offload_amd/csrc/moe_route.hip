@@ -143,7 +143,6 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
     using Key = std::conditional_t<BIAS, double, uint32_t>;
     using Val = std::conditional_t<BIAS, double, float>;
     __shared__ Key lkeys[kRouteWaves][64 * NPL];
-    __shared__ Key gkeys[kRouteWaves][kRouteMaxGroups];
     const int l = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x * kRouteWaves + wv;
     if (row >= A.M) return;
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
             if (e0 + j < A.E) lg[j] = logit_at<DT>(A.logits, base + e0 + j);
     }
     // the row's softmax where the keys or the weights need it
-    Val top = 0, total = 1;
+    Val top = 0, total = 1, e[NPL];
     if (!A.sigmoid && (BIAS || !A.renormalize)) {
         uint32_t most = 0;
 #pragma unroll
@@ -170,7 +169,11 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
         top = top_or_0((Val)value_of(wave_max(most)));
         total = 0;
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) total += BIAS ? exp((double)lg[j] - top) : (Val)expf(lg[j] - (float)top);
+        for (int j = 0; j < NPL; ++j) {
+            if constexpr (BIAS) e[j] = exp((double)lg[j] - top);
+            else e[j] = expf(lg[j] - top);
+            total += e[j];
+        }
         total = wave_sum(total);
         if (total == 0) total = 1;
     }
@@ -179,8 +182,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
     for (int j = 0; j < NPL; ++j) {
         const bool there = e0 + j < A.E;
         if constexpr (BIAS) {
-            const double v = lg[j];
-            const double sc = A.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - top) / total;
+            const double sc = A.sigmoid ? 1.0 / (1.0 + exp(-(double)lg[j])) : e[j] / total;
             const Key k = key_of(sc + (double)A.bias[there ? e0 + j : 0]);
             key[j] = there ? k : kNone<Key>;
         } else {
@@ -196,38 +198,53 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
     lds_ready();
 
     if (A.n_group > 1) {
-        const int G = A.n_group, gs = A.E / G;
-        Key* gk = gkeys[wv];
-        // P = the power of two up to 64 / G lanes per group; each lane the two largest of its share, then of the group's
-        const int P = 1 << (31 - __builtin_clz(64 / G)), g = l / P;
+        // The lanes P g .. P g + P - 1 find group g's two largest keys. Where the lanes' own shares make up whole groups, the
+        // power of two of them that does; else (aligned false) the power of two up to 64 / G, by way of LDS
+        const int G = A.n_group, gs = A.E / G, share = gs / NPL;
+        const bool aligned = gs % NPL == 0 && (share & (share - 1)) == 0;
+        const int P = aligned ? share : 1 << (31 - __builtin_clz(64 / G)), g = l / P;
         Key t1 = kNone<Key>, t2 = kNone<Key>;
-        if (g < G)
+        if (aligned) {
+            sort_descending(key);
+            t1 = key[0];
+            if constexpr (NPL > 1) t2 = key[1];
+        } else if (g < G) {
             for (int i = l & (P - 1); i < gs; i += P) {
                 const Key k = lk[g * gs + i];
                 t2 = larger(t2, smaller(t1, k));
                 t1 = larger(t1, k);
             }
-        for (int d = 1; d < P; d *= 2) {
-            const Key o1 = __shfl_xor(t1, d), o2 = __shfl_xor(t2, d);
+        }
+        auto join = [&](Key o1, Key o2) {
             t2 = larger(smaller(t1, o1), larger(t2, o2));
             t1 = larger(t1, o1);
+        };
+        // the neighbour, the other pair of four, the other four of eight, the other eight of sixteen (a mirror reaches them:
+        // they all have the same two by then)
+        if (P > 1) join(dpp<0xB1>(t1, t1), dpp<0xB1>(t2, t2));
+        if (P > 2) join(dpp<0x4E>(t1, t1), dpp<0x4E>(t2, t2));
+        if (P > 4) join(dpp<0x141>(t1, t1), dpp<0x141>(t2, t2));
+        if (P > 8) join(dpp<0x140>(t1, t1), dpp<0x140>(t2, t2));
+        for (int d = 16; d < P; d *= 2) join(__shfl_xor(t1, d), __shfl_xor(t2, d));
+        Key value = t1;
+        if constexpr (BIAS) {
+            const Key sum = key_of(value_of(t1) + value_of(t2));
+            value = gs > 1 ? sum : t1;
         }
-        if (g < G && (l & (P - 1)) == 0) {
-            if constexpr (BIAS) gk[g] = gs > 1 ? key_of(value_of(t1) + value_of(t2)) : t1;
-            else gk[g] = t1;
-        }
-        lds_ready();
-        const Key mine = l < G ? gk[l] : kNone<Key>;
         int rank = 0;
         for (int h = 0; h < G; ++h) {
-            const Key o = gk[h];
-            rank += o > mine || (o == mine && h < l);
+            const Key o = lane_value(value, h * P);
+            rank += o > value || (o == value && h < g);
         }
-        const uint64_t kept = __ballot(l < G && rank < A.topk_group);
+        const uint64_t kept = __ballot(g < G && rank < A.topk_group);        // (bit P i: group i)
         const uint32_t magic = ((1u << 20) + gs - 1) / gs;      // e / gs for e < 1024 (e * gs < 2^20)
 #pragma unroll
-        for (int j = 0; j < NPL; ++j)
-            if (!(kept >> (((uint32_t)(e0 + j) * magic) >> 20) & 1)) lk[e0 + j] = key[j] = kNone<Key>;
+        for (int j = 0; j < NPL; ++j) {
+            const int of = (int)((uint32_t)(e0 + j) * magic >> 20);
+            const bool out = of >= G || !(kept >> (of * P) & 1);
+            if (out) lk[e0 + j] = kNone<Key>;
+            key[j] = out ? kNone<Key> : key[j];      // (sorted keys of a lane are all of one group)
+        }
         lds_ready();
     }
 
@@ -236,8 +253,23 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
     Key picked = kNone<Key>, last = kNone<Key>;
     int from = 0, nth = 0, last_from = -1, n = 0;
     for (int r = 0; r < A.topk; ++r) {
-        const Key most = wave_max(key[0]);
-        const uint64_t have = __ballot(key[0] == most);
+        Key most;
+        uint64_t have;
+        if constexpr (BIAS) {
+            // the upper halves first, as whole numbers in the values' order: most often only one lane has the largest
+            const int hi = (int)(__builtin_bit_cast(uint64_t, key[0]) >> 32);
+            const uint32_t h = (uint32_t)hi ^ ((uint32_t)(hi >> 31) | 0x80000000u), top_h = wave_max(h);
+            have = __ballot(h == top_h);
+            if (have & (have - 1)) {
+                most = wave_max(h == top_h ? key[0] : kNone<Key>);
+                have = __ballot(key[0] == most);
+            } else {
+                most = lane_value(key[0], __builtin_ctzll(have));
+            }
+        } else {
+            most = wave_max(key[0]);
+            have = __ballot(key[0] == most);
+        }
         const int win = __builtin_ctzll(have);
         n = win == last_from && most == last ? n + 1 : 0;
         last = most;
