@@ -284,6 +284,80 @@ def test_c_abi_leaves_what_is_behind_a_row():
         assert (out[M:] == 7).all() and (out[:, n:] == 7).all()
 
 
+def test_rows_and_weights_past_32_bits():
+    """Rows, quantised rows, weights and outputs whose bytes lie past 2^32."""
+    g = _gen(41)
+    k, M = 4096, 1_050_000
+    x = torch.zeros(M, k, dtype=torch.bfloat16, device="cuda")
+    x[-300:] = torch.randn(300, k, generator=g, device="cuda").bfloat16()
+    print("case fp8 rows past 32 bits", flush=True)
+    q, s = _fp8().quant(x)
+    rq, rs = _quant_ref(x[-300:].double())
+    assert torch.equal(q[-300:].double(), rq) and torch.equal(s[-300:].double(), rs)
+    w, sw = _weight(g, 200, k)
+    lin = _fp8().Fp8Linear(w, sw)
+    y = lin.quantised(q, s, torch.float16)
+    _check_product(y[-300:], rq, rs, w, sw, None)
+    assert not y[:1000].any() and not y[M // 2:M // 2 + 1000].any()
+    del x, q, s, y
+    n = 1_050_000
+    raw = torch.zeros(n, k, dtype=torch.uint8, device="cuda")
+    raw[-200:] = w.view(torch.uint8)
+    sw = torch.ones(-(-n // 128), k // 128, device="cuda")
+    lin = _fp8().Fp8Linear(raw.view(torch.float8_e4m3fn), sw)
+    for M in (1, 20, 300):
+        print(f"case fp8 weights past 32 bits M={M}", flush=True)
+        x = torch.randn(M, k, generator=g, device="cuda").bfloat16()
+        y = lin(x)
+        _check_product(y[:, -200:], *_quant_ref(x.double()), w, torch.ones(2, k // 128, device="cuda"), None)
+        assert not y[:, :1000].any()
+    far = torch.zeros((1 << 31) + 2000, dtype=torch.bfloat16, device="cuda")      # rows 2^31 elements apart
+    x = far.as_strided((2, 1000), (1 << 31, 1))
+    x.copy_(torch.randn(2, 1000, generator=g, device="cuda"))
+    w, sw = _weight(g, 48, 1000)
+    lin = _fp8().Fp8Linear(w, sw)
+    print("case fp8 rows 2^32 bytes apart", flush=True)
+    assert torch.equal(lin(x), lin(x.contiguous()))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(_fp8().quant(x), _fp8().quant(x.contiguous())))
+
+
+@pytest.mark.parametrize("k,n", [(128, 64), (384, 40), (2048, 256), (4096, 80), (640, 7000)])
+def test_rows_quantised_within_the_product(k, n):
+    """The rows up to which the product quantises them itself, and one more, also at strides and odd addresses."""
+    g = _gen(43 + k)
+    w, sw = _weight(g, n, k)
+    lin = _fp8().Fp8Linear(w, sw)
+    for M in range(1, 19):
+        for dtype in DTYPES:
+            print(f"case fp8 own rows k={k} n={n} M={M} {dtype}", flush=True)
+            x = (torch.randn(M, k, generator=g, device="cuda") * 3).to(dtype)
+            x[M // 2, : k // 2] = 0
+            y = lin(x)
+            torch.cuda.synchronize()
+            _check_product(y, *_quant_ref(x.double()), w, sw, None)
+            assert torch.equal(lin(_odd(x)), y) and torch.equal(lin(torch.nn.functional.pad(x, (0, 3))[:, :k]), y)
+
+
+def test_a_workspace_of_a_larger_call():
+    """One workspace for calls of every size, the largest first, and the smallest: nothing of a call is left in it."""
+    from exl3xpu import capi
+    L, st = capi.lib(), torch.cuda.current_stream().cuda_stream
+    g = _gen(45)
+    k, I, n = 512, 256, 384  # noqa: E741
+    gu, gs = _weight(g, 2 * I, k)
+    dn, ds = _weight(g, n, I)
+    mlp = _fp8().Fp8Mlp(_fp8().Fp8Linear(gu, gs), _fp8().Fp8Linear(dn, ds))
+    ws = torch.full((L.exl3_fp8_mlp_workspace(400, k, I, n, 1),), 0x7F, dtype=torch.uint8, device="cuda")
+    for M in (400, 1, 33, 4, 130, 2, 400):
+        x = torch.randn(M, k, generator=g, device="cuda").bfloat16()
+        out = torch.full((M, n + 3), 9.0, dtype=torch.bfloat16, device="cuda")
+        print(f"case fp8 mlp c-abi M={M}", flush=True)
+        capi.check(L.exl3_fp8_mlp(x.data_ptr(), 1, k, M, k, I, n, gu.data_ptr(), gs.data_ptr(), None, dn.data_ptr(),
+                                  ds.data_ptr(), None, out.data_ptr(), n + 3, ws.data_ptr(), ws.numel(), st))
+        torch.cuda.synchronize()
+        assert torch.equal(out[:, :n], mlp(x)) and (out[:, n:] == 9).all()
+
+
 def test_refusals():
     g = _gen(27)
     w, sw = _weight(g, 256, 256)

@@ -162,6 +162,40 @@ def test_route_strides_and_shapes():
     assert [t.shape for t in _router(2)(wide.view(3, 4, 300)[:, :0])] == [(3, 0, 2)] * 2
 
 
+def test_route_rows_past_32_bits():
+    g = torch.Generator(device="cuda").manual_seed(15)
+    far = torch.zeros((1 << 31) + 600, dtype=torch.bfloat16, device="cuda")
+    lg = far.as_strided((2, 512), (1 << 31, 1))
+    lg.copy_(torch.randn(2, 512, generator=g, device="cuda"))
+    print("case route rows 2^32 bytes apart", flush=True)
+    _check(lg, 10)
+    _check(lg, 10, scoring="sigmoid", bias=0.1 * torch.randn(512, generator=g, device="cuda"))
+
+
+def test_route_feeds_the_experts_of_two_streams():
+    """Two routers at once, each with its experts, on two streams."""
+    from exl3xpu.moe_offload import ExpertStore
+    from exl3xpu.synth import expert_blob
+    g = torch.Generator(device="cuda").manual_seed(17)
+    store = ExpertStore(256, 128, 3, 8, 8, max_layers=1)
+    store.add_layer("layer0", torch.stack([expert_blob(7, e, 256, 128, 3) for e in range(8)]))
+    store.make_resident("layer0", range(8))
+    torch.cuda.synchronize()
+    routers = [_router(2), _router(3, scoring="sigmoid", bias=0.1 * torch.randn(8, generator=g, device="cuda"))]
+    lg = [torch.randn(m, 8, generator=g, device="cuda") for m in (3, 70)]
+    want = [[t.clone() for t in r(x)] for r, x in zip(routers, lg)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in routers], [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(routers[i](lg[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in range(2) for pair in got[i] for a, b in zip(pair, want[i]))
+    x = torch.randn(3, 256, generator=g, device="cuda").bfloat16()
+    assert torch.equal(store.forward_routed("layer0", x, lg[0], routers[0], cached=False), store.forward("layer0", x, *want[0]))
+
+
 def test_route_keys_closer_than_32_bits():
     """Scores + bias that differ by less than 32 bits hold: the choice is that of 64."""
     E, M = 256, 512
