@@ -249,6 +249,8 @@ struct RouteArgs {
 hipError_t launch_route(const RouteArgs& a, int dtype, hipStream_t s);
 
 // The 8-bit float linear: rows in e4m3 with one fp32 scale per 128 columns, weights in e4m3 with one per 128 x 128 block
+// (a launch holds fewer than 2^32 threads)
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;
 constexpr int kFp8Block = 128;
 __host__ __device__ static inline int fp8_blocks(int n) { return n / kFp8Block + (n % kFp8Block != 0); }
 // fp8_rows.hip. silu: x holds gate|up rows of 2 k values and the rows written are silu(gate) * up
@@ -257,6 +259,19 @@ struct Fp8RowsArgs {
     int M, k;
     uint8_t* q; float* s;                          // [M, 128 ceil(k / 128)] (zeros behind k), [M, ceil(k / 128)]
 };
+// Its workgroups of 256 threads cover 16 >> shift rows of 1 << shift blocks each, in `chunks` steps along the row
+struct Fp8RowsGrid {
+    int shift, chunks;
+    int64_t workgroups;
+};
+static inline Fp8RowsGrid fp8_rows_grid(int M, int k) {
+    const int kb = fp8_blocks(k);
+    Fp8RowsGrid g{};
+    while (g.shift < 4 && (1 << g.shift) < kb) ++g.shift;
+    g.chunks = (kb + (1 << g.shift) - 1) >> g.shift;
+    g.workgroups = (int64_t)((M - 1) / (16 >> g.shift) + 1) * g.chunks;
+    return g;
+}
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, int x_dt, bool silu, hipStream_t st);
 // 16-byte loads of such rows: every row starts on 16 bytes and no group of 8 elements crosses its end
 static inline bool fp8_rows_wide(const void* x, int64_t x_stride, int k, int x_dt) {

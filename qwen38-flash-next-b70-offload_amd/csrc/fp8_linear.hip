@@ -30,7 +30,9 @@ Pick pick_tile(int M, int n, int largest) {
         const int bm = kSizes[i][0], bn = kSizes[i][1];
         const int64_t tiles = (int64_t)((M - 1) / bm + 1) * ((n - 1) / bn + 1);
         const int64_t bytes = (tiles > kCus ? tiles : kCus) * (bm + bn);
-        if (i == 0 || bytes < least) least = bytes, best = {i, tiles <= kCus};
+        // (of up to 512 threads, in eighths; the callers' limit is that of the largest)
+        if (i < largest && (tiles + 7) * 512 >= kMaxThreads) continue;
+        if (least == 0 || bytes < least) least = bytes, best = {i, tiles <= kCus};
     }
     return best;
 }

@@ -10,7 +10,7 @@ namespace {
 
 constexpr int kRowsThreads = 256;                    // 16 blocks of 128 columns
 
-// A workgroup covers 16 >> shift rows of 1 << shift blocks each, the column chunks of a row next to each other
+// (Fp8RowsGrid; the column chunks of a row are next to each other)
 template <int DT, bool SILU, bool WIDE>
 __global__ void __launch_bounds__(kRowsThreads) fp8_rows_kernel(Fp8RowsArgs A, int kb, int shift, int chunks) {
     const int t = threadIdx.x >> 4, i = threadIdx.x & 15;
@@ -27,10 +27,8 @@ __global__ void __launch_bounds__(kRowsThreads) fp8_rows_kernel(Fp8RowsArgs A, i
 template <bool SILU, bool WIDE>
 void launch_rows(const Fp8RowsArgs& a, int x_dt, hipStream_t st) {
     const int kb = fp8_blocks(a.k);
-    int shift = 0;
-    while (shift < 4 && (1 << shift) < kb) ++shift;
-    const int chunks = (kb + (1 << shift) - 1) >> shift, rows = 16 >> shift;
-    const dim3 grid((unsigned)((int64_t)((a.M - 1) / rows + 1) * chunks));
+    const auto [shift, chunks, workgroups] = fp8_rows_grid(a.M, a.k);
+    const dim3 grid((unsigned)workgroups);
     if (x_dt == 0) hipLaunchKernelGGL((fp8_rows_kernel<0, SILU, WIDE>), grid, kRowsThreads, 0, st, a, kb, shift, chunks);
     else if (x_dt == 1) hipLaunchKernelGGL((fp8_rows_kernel<1, SILU, WIDE>), grid, kRowsThreads, 0, st, a, kb, shift, chunks);
     else hipLaunchKernelGGL((fp8_rows_kernel<2, SILU, WIDE>), grid, kRowsThreads, 0, st, a, kb, shift, chunks);

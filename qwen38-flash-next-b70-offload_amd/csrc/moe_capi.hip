@@ -1261,8 +1261,6 @@ namespace {
 bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
 size_t dt_size(int dt) { return dt == EXL3_DT_F32 ? 4 : 2; }
 bool dt_ok(int dt) { return dt >= EXL3_DT_F16 && dt <= EXL3_DT_F32; }
-// a launch holds fewer than 2^32 threads
-constexpr int64_t kMaxThreads = (int64_t)1 << 32;
 
 // the sizes every entry point of the 8-bit float linear takes
 int fp8_dims(const char* what, int M, int k, int n) {
@@ -1280,7 +1278,7 @@ int fp8_rows(const char* what, const void* x, int x_dtype, int64_t x_stride, int
     if (!x || !q || !s) return fail(EXL3_EINVAL, "%s: null pointer", what);
     if (x_stride < (silu ? 2 : 1) * (int64_t)k) return fail(EXL3_EINVAL, "%s: row stride %lld", what, (long long)x_stride);
     if (!aligned(x, dt_size(x_dtype)) || !aligned(q, 16) || !aligned(s, 4)) return fail(EXL3_EINVAL, "%s: alignment", what);
-    if ((M + (int64_t)16) * (fp8_blocks(k) + (int64_t)16) * 16 >= kMaxThreads)
+    if (fp8_rows_grid(M, k).workgroups * 256 >= kMaxThreads)
         return fail(EXL3_EUNSUPPORTED, "%s: M=%d rows of k=%d exceed one launch", what, M, k);
     Fp8RowsArgs a{};
     a.x = x;

@@ -482,6 +482,7 @@ at::Tensor rows_of(const at::Tensor& x, const char* what) {
 int64_t row_stride(const at::Tensor& x2) { return x2.size(0) > 1 ? x2.stride(0) : x2.size(1); }
 
 std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t n) {
+    TORCH_CHECK(!sizes.empty(), "a tensor of at least one dimension, got a scalar");
     auto v = sizes.vec();
     v.back() = n;
     return v;

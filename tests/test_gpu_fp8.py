@@ -321,6 +321,18 @@ def test_rows_and_weights_past_32_bits():
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(_fp8().quant(x), _fp8().quant(x.contiguous())))
 
 
+def test_more_small_tiles_than_one_launch_holds():
+    """2^27 rows of 128 to 16 columns: 16 x 16 tiles, which would be the ones, would take 2^32 threads."""
+    g = _gen(37)
+    M = 1 << 17
+    q, s = _fp8().quant(torch.randn(M, 128, generator=g, device="cuda"))
+    lin = _fp8().Fp8Linear(*_weight(g, 16, 128))
+    want = lin.quantised(q, s, torch.bfloat16)
+    print("case fp8 product of 2^27 rows", flush=True)
+    got = lin.quantised(q.view(torch.uint8).repeat(1024, 1).view(q.dtype), s.repeat(1024, 1), torch.bfloat16)
+    assert all(torch.equal(t, want) for t in got.split(M))
+
+
 @pytest.mark.parametrize("k,n", [(128, 64), (384, 40), (2048, 256), (4096, 80), (640, 7000)])
 def test_rows_quantised_within_the_product(k, n):
     """The rows up to which the product quantises them itself, and one more, also at strides and odd addresses."""

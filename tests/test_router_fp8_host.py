@@ -118,6 +118,22 @@ def test_shapes_without_a_device():
     assert y.shape == (2, 7, 130) and y.dtype == torch.bfloat16
 
 
+def test_scalars_have_no_rows():
+    m = torch.device("meta")
+    w8, sw, x = torch.empty(130, 384, device=m, dtype=torch.float8_e4m3fn), torch.empty(2, 3, device=m), torch.empty((), device=m)
+    for f in (lambda: ops().moe_route(x, None, 1, "softmax", 1, 1, True, 1.0), lambda: C().fp8_linear(x, w8, sw, None),
+              lambda: C().fp8_matmul(x, x, w8, sw, None, torch.bfloat16), lambda: C().fp8_mlp(x, w8, sw, None, w8, sw, None),
+              lambda: C().fp8_quant(x), lambda: C().fp8_silu_mul_quant(x)):
+        with pytest.raises((RuntimeError, IndexError)):
+            f()
+
+
+@pytest.mark.parametrize("M,k", [(1 << 28, 128), (1 << 27, 200), (1 << 24, 2048), (1 << 16, 1 << 21)])
+def test_rows_of_one_launch(M, k):
+    """16 lanes a block of 128, rounded up to whole workgroups: 2^32 threads and more are refused."""
+    assert _rows("exl3_fp8_quant", M=M, k=k, stride=k) == UNSUPPORTED
+
+
 def test_classes_refuse():
     w, s = torch.zeros(256, 300).to(torch.float8_e4m3fn), torch.ones(2, 3)
     lin = fp8.Fp8Linear(w, s)
