@@ -147,8 +147,11 @@ __device__ __forceinline__ void quant_rows(const Fp8ProductArgs& A, uint8_t* q, 
 // and brings them to LDS by direct loads, ST stages of its own. The groups' sums join at the end, in the groups' order. OWN:
 // the workgroup quantises its (up to 16) rows itself while its first weights are on their way, and `own` is their LDS.
 // EXACT: sums without the e4m3 MFMA's losses, outputs in fp16, bf16 or fp32 (out_dt 0, 1, 2); else fp16 or bf16 outputs.
+// Two waves per SIMD at least: with more registers than that leaves, MFMAs write accumulation registers, which the multiply-adds
+// cannot read (8,192 rows, 2048 -> 12,288, fp32 outputs: 412 us with the copies, 390 without).
 template <bool EXACT, bool OWN, int BM, int BN, int WM, int WN, int KG, int ST>
-__global__ void __launch_bounds__(64 * WM * WN * KG) fp8_tile_kernel(Fp8ProductArgs A, int mt, int nt, int per, int out_dt) {
+__global__ void __launch_bounds__(64 * WM * WN * KG, WM * WN * KG <= 4 ? 2 : 1)
+    fp8_tile_kernel(Fp8ProductArgs A, int mt, int nt, int per, int out_dt) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, QB = OWN ? 0 : BM;
     static_assert(!OWN || BM == 16, "one fragment of rows");
     union Lds {
@@ -257,11 +260,14 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp8_tile_kernel(Fp8ProductA
                 for (int i = 0; i < TN; ++i) x[j & 1][i] = block_sum(wf[i], qf[j & 1]);
                 add(j ? j - 1 : TM - 1);
                 sc[j & 1] = st.s[wm + j * 16 + r] * sw;
+                // (the exact sums' conversions between their MFMAs too where there are 8 of those: 777 rows, 2000 -> 1000, 10.4 ->
+                // 9.9 us; with 4 of them, 256 rows, 5.8 against 5.7)
+                constexpr bool kThrees = EXACT && TN > 1;
                 __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
-                for (int i = 0; i < TN; ++i) {
+                for (int i = 0; i < (kThrees ? 4 : 1) * TN; ++i) {
                     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x2, kThrees ? 3 : 5, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }

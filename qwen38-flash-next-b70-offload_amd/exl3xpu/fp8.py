@@ -13,6 +13,8 @@ can be captured into a graph.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .linear import C as _C
@@ -22,14 +24,19 @@ __all__ = ["BLOCK", "Fp8Linear", "Fp8Mlp", "quant", "silu_mul_quant"]
 BLOCK = 128
 
 
+@functools.cache
+def _op(name: str):
+    return getattr(_C(), name).default
+
+
 def quant(x: torch.Tensor):
     """x [..., k] fp16 / bf16 / fp32 -> (q, s)."""
-    return _C().fp8_quant(x)
+    return _op("fp8_quant")(x)
 
 
 def silu_mul_quant(gate_up: torch.Tensor):
     """gate|up rows [..., 2 k] -> (q, s) of silu(gate) * up, computed in fp32."""
-    return _C().fp8_silu_mul_quant(gate_up)
+    return _op("fp8_silu_mul_quant")(gate_up)
 
 
 class Fp8Linear:
@@ -52,7 +59,7 @@ class Fp8Linear:
         self.weight = (torch.nn.functional.pad(raw, (0, pad)) if pad else raw.contiguous()).view(torch.float8_e4m3fn)
         self.weight_scale = weight_scale.detach().to(device, torch.float32).contiguous()
         self.bias = None if bias is None else bias.detach().to(device, torch.float32).contiguous()
-        self._linear, self._matmul = _C().fp8_linear.default, _C().fp8_matmul.default
+        self._linear, self._matmul = _op("fp8_linear"), _op("fp8_matmul")
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         """x [..., k] fp16 / bf16 / fp32 -> [..., n] of x's dtype."""
@@ -74,7 +81,7 @@ class Fp8Mlp:
             raise ValueError(f"exl3xpu: gate|up of {gate_up.n} columns does not fit a down of {down.k} inputs")
         self.gate_up, self.down = gate_up, down
         self._weights = [t for lin in (gate_up, down) for t in (lin.weight, lin.weight_scale, lin.bias)]
-        self._op = _C().fp8_mlp.default
+        self._op = _op("fp8_mlp")
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         """x [..., k] -> [..., n] of x's dtype; gate|up is rounded to x's dtype between the two products."""
