@@ -10,7 +10,12 @@
 //   weight  the pick's score (renormalised: over the picks' sum, the softmax taken over the picks' own logits, so that
 //           nothing underflows), times scale; a sum of 0 (every pick at -inf) gives weights of 0
 //
-// One wave per row. Lane i holds the E / 64 neighbouring experts from i * NPL, so the lowest lane of a tie holds the
+// One wave per row; the instructions of 8 waves per SIMD bound 8,192 rows (logits arrive at 2.2 TB/s), the chain of the picks
+// one row. GPU time, us, for 1 / 200 / 8,192 rows: 512 experts, top 10: 3.2 / 3.7 / 7.7, with a bias 5.0 / 5.6 / 15.4; 256 in
+// 8 groups of which 4 compete, top 8: 3.4 / 3.8 / 7.5, with a bias 4.6 / 5.2 / 12.9; 128, top 8: 2.8 / 3.3 / 5.9, with a bias
+// 3.7 / 4.1 / 9.0.
+//
+// Lane i holds the E / 64 neighbouring experts from i * NPL, so the lowest lane of a tie holds the
 // lowest index; it sorts their keys (a network of max and min, without the indices). A pick is then one maximum over the
 // lanes' first keys (six DPP steps), the first lane that has it, and that lane's keys move up. What the picks were is found
 // at the end, all at once: lane r looks up the place of pick r's key among the keys of the lane that it came from. Nothing is
@@ -36,8 +41,9 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __builtin_bit_cast(float, (k & 0x80000000u) ? (k == 0xFFFFFFFFu ? 0x7FC00000u : k & 0x7FFFFFFFu) : ~k);
 }
 constexpr double kInf = 1e300, kNan = 2e300;
-__device__ __forceinline__ double key_of(double v) {
-    return v != v ? kNan : v == INFINITY ? kInf : v == -INFINITY ? -kInf : v + 0.0;
+__device__ __forceinline__ double key_of(double v) {      // (no -0: a score is never one, and a sum of others is +0)
+    const double k = __builtin_fmin(__builtin_fmax(v, -kInf), kInf);
+    return v != v ? kNan : k;
 }
 __device__ __forceinline__ double value_of(double k) {
     return k == kNan ? __builtin_nan("") : k == kInf ? INFINITY : k == -kInf ? -INFINITY : k;
@@ -134,6 +140,16 @@ __device__ __forceinline__ void logits_wide(const void* p, size_t at, float (&v)
     for (int j = 0; j < NPL; ++j) v[j] = logit_at<DT>(u.x, j);
 }
 
+// 1 / (1 + e^-l), 0 below -700: the hardware's reciprocal (2^-23) and two steps of Newton's
+__device__ __forceinline__ double sigmoid64(float l) {
+    const bool low = l < -700.0f;
+    const double d = 1.0 + exp(low ? 700.0 : -(double)l);
+    double r = __builtin_amdgcn_rcp(d);
+    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+    return low ? 0.0 : r;
+}
+
 // the softmax is taken relative to the row's largest logit (to 0 where that is -inf, so that exp gives 0)
 template <class T>
 __device__ __forceinline__ T top_or_0(T top) { return top == -(T)INFINITY ? (T)0 : top; }
@@ -153,12 +169,28 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
     float lg[NPL];
 #pragma unroll
     for (int j = 0; j < NPL; ++j) lg[j] = -INFINITY;
-    if (wide) {
+    if (wide & 1) {
         if (e0 < A.E) logits_wide<DT>(A.logits, base + e0, lg);
     } else {
 #pragma unroll
-        for (int j = 0; j < NPL; ++j)
-            if (e0 + j < A.E) lg[j] = logit_at<DT>(A.logits, base + e0 + j);
+        for (int j = 0; j < NPL; ++j) {
+            const float v = logit_at<DT>(A.logits, base + min(e0 + j, A.E - 1));
+            lg[j] = e0 + j < A.E ? v : -INFINITY;
+        }
+    }
+    [[maybe_unused]] float bias[NPL];
+    if constexpr (BIAS) {                            // (all of it before the first score is needed)
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) bias[j] = -INFINITY;
+        if (wide & 2) {
+            if (e0 < A.E) logits_wide<2>(A.bias, e0, bias);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) {
+                const float v = A.bias[min(e0 + j, A.E - 1)];
+                bias[j] = e0 + j < A.E ? v : -INFINITY;
+            }
+        }
     }
     // the row's softmax where the keys or the weights need it
     Val top = 0, total = 1, e[NPL];
@@ -177,18 +209,23 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
         total = wave_sum(total);
         if (total == 0) total = 1;
     }
+    if constexpr (BIAS) {                            // (now the scores)
+        if (A.sigmoid) {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) e[j] = sigmoid64(lg[j]);
+        } else {
+            const double each = 1.0 / total;
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) e[j] *= each;
+        }
+    }
+    // (places behind the last expert have the key of -inf, or, as every expert of a row with a NaN, of NaN: with no expert's are
+    // theirs smaller, but where keys are equal the experts come first, and there are topk of them)
     Key key[NPL];
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
-        const bool there = e0 + j < A.E;
-        if constexpr (BIAS) {
-            const double sc = A.sigmoid ? 1.0 / (1.0 + exp(-(double)lg[j])) : e[j] / total;
-            const Key k = key_of(sc + (double)A.bias[there ? e0 + j : 0]);
-            key[j] = there ? k : kNone<Key>;
-        } else {
-            const Key k = key_of(lg[j]);
-            key[j] = there ? k : kNone<Key>;
-        }
+        if constexpr (BIAS) key[j] = key_of(e[j] + (double)bias[j]);
+        else key[j] = key_of(lg[j]);
         lk[e0 + j] = key[j];
     }
     auto lds_ready = [] {                            // (a wave's own part of LDS)
@@ -197,6 +234,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
     };
     lds_ready();
 
+    bool sorted = false;
     if (A.n_group > 1) {
         // The lanes P g .. P g + P - 1 find group g's two largest keys. Where the lanes' own shares make up whole groups, the
         // power of two of them that does; else (aligned false) the power of two up to 64 / G, by way of LDS
@@ -236,22 +274,30 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
             const Key o = lane_value(value, h * P);
             rank += o > value || (o == value && h < g);
         }
-        const uint64_t kept = __ballot(g < G && rank < A.topk_group);        // (bit P i: group i)
-        const uint32_t magic = ((1u << 20) + gs - 1) / gs;      // e / gs for e < 1024 (e * gs < 2^20)
+        const bool keeps = g < G && rank < A.topk_group;
+        if (aligned) {
+            // (a lane's keys are all of its own group)
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-            const int of = (int)((uint32_t)(e0 + j) * magic >> 20);
-            const bool out = of >= G || !(kept >> (of * P) & 1);
-            if (out) lk[e0 + j] = kNone<Key>;
-            key[j] = out ? kNone<Key> : key[j];      // (sorted keys of a lane are all of one group)
+            for (int j = 0; j < NPL; ++j) key[j] = keeps ? key[j] : kNone<Key>;
+            sorted = true;
+        } else {
+            const uint64_t kept = __ballot(keeps);              // (bit P i: group i)
+            const uint32_t magic = ((1u << 20) + gs - 1) / gs;  // e / gs for e < 1024 (e * gs < 2^20)
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) {
+                const int of = (int)((uint32_t)(e0 + j) * magic >> 20);
+                const bool out = of >= G || !(kept >> (of * P) & 1);
+                if (out) lk[e0 + j] = kNone<Key>;
+                key[j] = out ? kNone<Key> : key[j];
+            }
+            lds_ready();
         }
-        lds_ready();
     }
 
     // the picks: lane r keeps pick r's key, the lane it came from, and how many picks before it took that key from that lane
-    sort_descending(key);
+    if (!sorted) sort_descending(key);
     Key picked = kNone<Key>, last = kNone<Key>;
-    int from = 0, nth = 0, last_from = -1, n = 0;
+    int source = 0, last_from = -1, n = 0;
     for (int r = 0; r < A.topk; ++r) {
         Key most;
         uint64_t have;
@@ -276,17 +322,25 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
         last_from = win;
         const bool here = l == r;
         picked = here ? most : picked;
-        from = here ? win : from;
-        nth = here ? n : nth;
-        const bool mine = l == win;
+        source = here ? n << 8 | win : source;
+        if constexpr (BIAS && NPL > 1) {
+            if (l == win) {
+                asm volatile("");                    // (a branch: 64 bits move at once, and are chosen by halves)
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-            const Key here = key[j], next = j + 1 < NPL ? key[j + 1] : kNone<Key>;
-            key[j] = mine ? next : here;
+                for (int j = 0; j < NPL; ++j) key[j] = j + 1 < NPL ? key[j + 1] : kNone<Key>;
+            }
+        } else {
+            const bool mine = l == win;
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) {
+                const Key here = key[j], next = j + 1 < NPL ? key[j + 1] : kNone<Key>;
+                key[j] = mine ? next : here;
+            }
         }
     }
     const bool live = l < A.topk;
-    int id = from * NPL;
+    const int from = source & 255;
+    int nth = source >> 8, id = from * NPL;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {                  // the place of the nth (from 0) key of this value
         const bool same = lk[from * NPL + j] == picked;
@@ -315,7 +369,10 @@ template <int NPL, bool BIAS>
 void route_dt(const RouteArgs& a, int dtype, hipStream_t s) {
     const dim3 grid((unsigned)((a.M + (int64_t)kRouteWaves - 1) / kRouteWaves)), block(64 * kRouteWaves);
     const int esz = dtype == 2 ? 4 : 2, each = NPL * esz < 16 ? NPL * esz : 16;
-    const int wide = a.E % NPL == 0 && (uintptr_t)a.logits % each == 0 && a.stride * esz % each == 0;
+    // (a lane's logits, and its biases, in wide loads)
+    constexpr int kBiasEach = NPL * 4 < 16 ? NPL * 4 : 16;
+    const int wide = (a.E % NPL == 0 && (uintptr_t)a.logits % each == 0 && a.stride * esz % each == 0) |
+                     (BIAS && a.E % NPL == 0 && (uintptr_t)a.bias % kBiasEach == 0) << 1;
     if (dtype == 0) hipLaunchKernelGGL((route_kernel<NPL, BIAS, 0>), grid, block, 0, s, a, wide);
     else if (dtype == 1) hipLaunchKernelGGL((route_kernel<NPL, BIAS, 1>), grid, block, 0, s, a, wide);
     else hipLaunchKernelGGL((route_kernel<NPL, BIAS, 2>), grid, block, 0, s, a, wide);

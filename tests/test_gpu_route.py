@@ -148,6 +148,38 @@ def test_route_masks_infinities_and_ties(scoring, bias):
         assert ids[0].tolist() == list(range(topk)) and w[0].abs().max() == 0
 
 
+@pytest.mark.parametrize("E,topk,n_group,topk_group", [(60, 60, 1, 1), (130, 9, 1, 1), (250, 12, 1, 1), (512, 10, 1, 1),
+                                                       (256, 8, 8, 4), (160, 6, 8, 3)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_biases_without_an_end(E, topk, n_group, topk_group, scoring):
+    """Experts that the bias rules out, forces or spoils, biases that start anywhere, scores at both ends of sigmoid's range."""
+    g = torch.Generator(device="cuda").manual_seed(E)
+    lg = torch.randn(12, E, generator=g, device="cuda")
+    lg[1] = -math.inf
+    lg[2] = math.nan
+    lg[3, ::3] = math.nan
+    lg[4] *= 30
+    lg[5, 5:] = -800.0
+    lg[6, :-3] = -math.inf
+    lg[7, 1::2] = 800.0
+    room = torch.empty(E + 1, device="cuda")
+    for at in (0, 1):
+        bias = room[at:at + E]
+        for kind in range(5):
+            bias.copy_(0.1 * torch.randn(E, generator=g, device="cuda"))
+            if kind == 1:
+                bias[::4] = -math.inf
+            elif kind == 2:
+                bias.fill_(-math.inf)
+            elif kind == 3:
+                bias[[1, E - 1]] = math.inf
+                bias[E // 2] = math.nan
+            elif kind == 4:
+                bias.zero_()
+            print(f"case route bias E={E} groups={n_group} {scoring} at={at} kind={kind}", flush=True)
+            _check(lg, topk, scoring=scoring, bias=bias, n_group=n_group, topk_group=topk_group)
+
+
 def test_route_strides_and_shapes():
     g = torch.Generator(device="cuda").manual_seed(9)
     wide = torch.randn(12, 300, generator=g, device="cuda")
