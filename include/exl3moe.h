@@ -368,33 +368,37 @@ int exl3_table_update(int64_t* ptrs_all, int32_t* slot_of, int32_t* slot_key, in
  * compete (by their largest score; with a bias, by the sum of their two largest). Picks come in descending order of what
  * they are chosen by, equal ones by index; a NaN counts as the largest. w: the picks' scores, over their sum with
  * renormalize (0 where that sum is 0: a row of -inf), times scale. The ids of a row are always topk different experts.
- * 1 <= E <= 1024, topk <= 64 and <= topk_group * E / n_group, n_group <= 64 and a divisor of E. ids int32, w fp32 [M, topk]. */
+ * 1 <= E <= 1024, topk <= 64 and <= topk_group * E / n_group, n_group <= 64 and a divisor of E, M < 2^26 - 64. ids: int32,
+ * w: fp32 [M, topk]. */
 int exl3_moe_route(const void* logits, int dtype, int64_t stride, int M, int E, const float* bias, int topk, int scoring,
                    int n_group, int topk_group, int renormalize, float scale, int32_t* ids, float* w, void* stream);
 
 /* Rows of 8-bit floats (e4m3, OCP) with one fp32 scale per 128 columns: s = max(amax / 448, 2^-80), q = x / s rounded to
  * the nearest, halves to even (scale and quotient are rounded to 32 bits first). kp = k rounded up to 128. x: [M, k] of
  * x_dtype with x_stride elements between rows; q: [M, kp], zeros behind column k; s: fp32 [M, kp / 128]. An infinite or
- * NaN element makes its block's scale infinite or NaN. */
+ * NaN element makes its block's scale infinite or NaN. k <= 2^22, and rows for fewer than 2^28 blocks (EXL3_EUNSUPPORTED). */
 int exl3_fp8_quant(const void* x, int x_dtype, int64_t x_stride, int M, int k, void* q, float* s, void* stream);
 /* the same of silu(gate) * up (in fp32) of gate|up rows [M, 2 k] */
 int exl3_fp8_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int M, int k, void* q, float* s, void* stream);
 /* out[m][n] = sum over blocks b of s[m][b] sw[n / 128][b] (sum over k in b of q[m][k] w[n][k]) + bias[n], fp32 sums, rounded
  * once to out_dtype. q, s as above; w: e4m3 [n, kp], zeros behind column k; sw: fp32 [ceil(n / 128), kp / 128]; bias: fp32
- * [n] or NULL; q and w start on 16 bytes. For fp16 and bf16 outputs the sums of 128 products may be off by 7 * 2^-13 of
- * their products' magnitudes at most (1.5e-5 of the output's size for normal values), for fp32 by no more than fp32 sums. workspace: exl3_fp8_matmul_workspace bytes, no state between calls; its size
- * never falls as M grows. */
+ * [n] or NULL; q and w start on 16 bytes; k <= 2^22, n <= 2^27. For fp16 and bf16 outputs the sums of 128 products may be off
+ * by 7 * 2^-13 of their products' magnitudes at most (1.5e-5 of the output's size for normal values), for fp32 by no more than
+ * fp32 sums. workspace: exl3_fp8_matmul_workspace bytes (none at present), no state between calls; its size never falls as M
+ * grows. */
 size_t exl3_fp8_matmul_workspace(int M, int k, int n);
 int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
                     void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
-/* the same of x [M, k], quantised within the call */
+/* the same of x [M, k], quantised within the call; its workspace starts on 16 bytes and is not shared by calls that run at
+ * the same time */
 size_t exl3_fp8_linear_workspace(int M, int k, int n);
 int exl3_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const float* sw,
                     const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                     size_t workspace_bytes, void* stream);
 /* A gated MLP: exl3_fp8_linear of x [M, k] with gate|up weights of 2 I rows (gu: [2 I, k up to a multiple of 128], scales
- * gu_scale, gu_bias fp32 [2 I] or NULL) whose sums are as exact as those of fp32 outputs, rounded to `dtype`, then silu(gate) * up quantised and multiplied with the down
- * weights (dn: [n, I up to a multiple of 128], dn_scale, dn_bias fp32 [n] or NULL). x and out are of `dtype`. */
+ * gu_scale, gu_bias fp32 [2 I] or NULL) whose sums are as exact as those of fp32 outputs, rounded to `dtype`, then silu(gate)
+ * * up quantised and multiplied with the down weights (dn: [n, I up to a multiple of 128], dn_scale, dn_bias fp32 [n] or
+ * NULL). x and out are of `dtype`. The workspace as exl3_fp8_linear's. */
 size_t exl3_fp8_mlp_workspace(int M, int k, int I, int n, int dtype);
 int exl3_fp8_mlp(const void* x, int dtype, int64_t x_stride, int M, int k, int I, int n, const void* gu,
                  const float* gu_scale, const float* gu_bias, const void* dn, const float* dn_scale, const float* dn_bias,
