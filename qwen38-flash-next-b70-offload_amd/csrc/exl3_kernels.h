@@ -288,8 +288,9 @@ struct Fp8ProductArgs {
     bool silu, x_wide;
     bool exact;                                    // sums without the e4m3 MFMA's losses (fp32 outputs always have them)
 };
-// the product's tiles (rows x columns); 256 x 256 without `exact`, the first two where the product quantises its rows itself
-enum { kTile16, kTile16x32, kTile32, kTile64, kTile128, kTile256 };
+// the product's tiles (rows x columns); 128 x 64 and 256 x 256 without `exact`, the first two where the product quantises its
+// rows itself
+enum { kTile16, kTile16x32, kTile32, kTile64, kTile128x64, kTile128, kTile256 };
 constexpr int kCus = 256;
 // whether the product quantises its rows itself (no launch_fp8_rows before it)
 bool fp8_product_quantises(int M, int k, int n);

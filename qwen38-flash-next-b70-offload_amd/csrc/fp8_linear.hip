@@ -6,7 +6,8 @@
 //
 //     max(1, tiles / 256 CUs) (BM + BN)
 //
-// the smaller one where two are equal. 4096 -> 2048, us for 16 / 64 / 128 / 512 / 2,048 rows: 16 x 16 tiles 4.0 / 5.5 / 10.2 /
+// the smaller one where two are equal. 128 x 64 only where each CU has one at most and without exact sums (1,024 rows, 4096 ->
+// 2048: 17.0 us, 64 x 64 18.6; two for some CUs, 1,100 rows: 27.8, 128 x 128 25.1; exact 26.0 against 25.4). 4096 -> 2048, us for 16 / 64 / 128 / 512 / 2,048 rows: 16 x 16 tiles 4.0 / 5.5 / 10.2 /
 // - / -, 16 x 32 5.1 / 5.4 / 8.2 / - / -, 32 x 32 6.0 / 6.4 / 6.6 / 17.3 / -, 64 x 64 9.3 / 9.6 / 9.6 / 11.3 / 34,
 // 128 x 128 17 / 18 / 18 / 22 / 27, 256 x 256 40 / 40 / 41 / 43 / 45.
 #include "exl3_kernels.h"
@@ -22,14 +23,15 @@ struct Pick {
     int tile;
     bool few;                                        // at most one workgroup per CU
 };
-Pick pick_tile(int M, int n, int largest) {
-    constexpr int kSizes[][2] = {{16, 16}, {16, 32}, {32, 32}, {64, 64}, {128, 128}, {256, 256}};
+Pick pick_tile(int M, int n, int largest, bool exact) {
+    constexpr int kSizes[][2] = {{16, 16}, {16, 32}, {32, 32}, {64, 64}, {128, 64}, {128, 128}, {256, 256}};
     Pick best{};
     int64_t least = 0;
     for (int i = 0; i <= largest; ++i) {
         const int bm = kSizes[i][0], bn = kSizes[i][1];
         const int64_t tiles = (int64_t)((M - 1) / bm + 1) * ((n - 1) / bn + 1);
         const int64_t bytes = (tiles > kCus ? tiles : kCus) * (bm + bn);
+        if (tiles > kCus && (i == kTile16 || i == kTile128x64) || exact && i == kTile128x64) continue;
         // (of up to 512 threads, in eighths; the callers' limit is that of the largest)
         if (i < largest && (tiles + 7) * 512 >= kMaxThreads) continue;
         if (least == 0 || bytes < least) least = bytes, best = {i, tiles <= kCus};
@@ -43,12 +45,12 @@ Pick pick_tile(int M, int n, int largest) {
 // at 32. More rows are quantised by a launch of their own: 2048 -> 1024, 8 rows 5.1 us, by two launches 6.1; 4096 -> 2048, 8
 // rows 8.0 us, by two launches 7.4.
 bool fp8_product_quantises(int M, int k, int n) {
-    return M <= 16 && (int64_t)M * fp8_blocks(k) <= (pick_tile(M, n, kTile16x32).tile == kTile16 ? 128 : 64);
+    return M <= 16 && (int64_t)M * fp8_blocks(k) <= (pick_tile(M, n, kTile16x32, false).tile == kTile16 ? 128 : 64);
 }
 
 hipError_t launch_fp8_product(const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
     const bool exact = a.exact || out_dt == 2;
-    const Pick p = pick_tile(a.M, a.n, !a.q ? kTile16x32 : exact ? kTile128 : kTile256);
+    const Pick p = pick_tile(a.M, a.n, !a.q ? kTile16x32 : exact ? kTile128 : kTile256, exact);
     if (exact) launch_fp8_tile_exact(p.tile, p.few, a, out_dt, st);
     else launch_fp8_tile_e4m3(p.tile, p.few, a, out_dt, st);
     return hipGetLastError();

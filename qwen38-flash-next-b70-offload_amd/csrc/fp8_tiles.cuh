@@ -371,15 +371,28 @@ void launch_fp8_tiles(const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
 // `few`: at most one workgroup per CU, so that it may have the CU's LDS
 template <bool EXACT>
 void launch_fp8_tile(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
-    if (!a.q) {
+    if (!a.q) {                                      // (no other tile may have these: their rows come from q)
         if (tile == kTile16) launch_fp8_tiles<EXACT, true, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
         else launch_fp8_tiles<EXACT, true, 16, 32, 1, 2, 2, 4>(a, out_dt, st);
-    } else if (tile == kTile16) launch_fp8_tiles<EXACT, false, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
+        return;
+    }
+    if constexpr (EXACT) {
+        if (few && tile == kTile128) return launch_fp8_tiles<EXACT, false, 128, 128, 2, 2, 2, 2>(a, out_dt, st);
+    } else {
+        // e4m3 MFMAs leave the loads to wait for, so that more stages pay where the CU's LDS is there for them: up to 32 x 32
+        // from three steps on (4096 -> 2048, 64 rows 5.9 -> 5.2 us, 128 rows 6.7 -> 6.2; k 512, one step: 3.4 -> 3.8), and 128 x
+        // 128 as one group of 8 waves, whose registers allow it (2,048 rows, 27.5 -> 25.5 us, 1,500 rows 25.9 -> 22.9). Exact
+        // sums lose: 128 rows 7.3 -> 7.9 us, 2,048 rows 38.7 -> 42.7
+        if (few && tile == kTile16x32 && a.kb > 8) return launch_fp8_tiles<EXACT, false, 16, 32, 1, 2, 4, 4>(a, out_dt, st);
+        if (few && tile == kTile32 && a.kb > 8) return launch_fp8_tiles<EXACT, false, 32, 32, 1, 2, 4, 4>(a, out_dt, st);
+        if (few && tile == kTile128) return launch_fp8_tiles<EXACT, false, 128, 128, 2, 4, 1, 4>(a, out_dt, st);
+        if (tile == kTile128x64) return launch_fp8_tiles<EXACT, false, 128, 64, 4, 2, 1, 4>(a, out_dt, st);
+    }
+    if (tile == kTile16) launch_fp8_tiles<EXACT, false, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
     else if (tile == kTile16x32) launch_fp8_tiles<EXACT, false, 16, 32, 1, 2, 4, 2>(a, out_dt, st);
     else if (tile == kTile32) launch_fp8_tiles<EXACT, false, 32, 32, 1, 2, 4, 2>(a, out_dt, st);
     else if (tile == kTile64 && few) launch_fp8_tiles<EXACT, false, 64, 64, 2, 2, 2, 4>(a, out_dt, st);
     else if (tile == kTile64) launch_fp8_tiles<EXACT, false, 64, 64, 2, 2, 2, 2>(a, out_dt, st);
-    else if (tile == kTile128 && few) launch_fp8_tiles<EXACT, false, 128, 128, 2, 2, 2, 2>(a, out_dt, st);
     else launch_fp8_tiles<EXACT, false, 128, 128, 2, 2, 1, 2>(a, out_dt, st);
 }
 

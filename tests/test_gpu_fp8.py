@@ -229,6 +229,25 @@ def test_linear_larger(M, n, k):
         assert torch.equal(lin(x), y)                        # the same sums in the same order
 
 
+@pytest.mark.parametrize("n,k,Ms", [(2000, 1300, (33, 40, 47, 64, 90, 100, 127, 300)), (2050, 4000, (64, 97, 128)),
+                                    (1990, 640, (770, 1000, 1090, 1500, 2200)), (5000, 2048, (1, 3, 4, 5, 8, 16, 17)),
+                                    (1100, 1152, (80, 2030)), (12200, 200, (100, 1100))])
+def test_linear_tiles(n, k, Ms):
+    """Sizes of every tile, with one workgroup per CU at most and with more, and edges inside a tile."""
+    g = _gen(n + k)
+    w, sw = _weight(g, n, k)
+    bias = torch.randn(n, generator=g, device="cuda")
+    lin = _fp8().Fp8Linear(w, sw, bias)
+    for M in Ms:
+        for dtype in DTYPES:
+            print(f"case fp8 linear tiles n={n} k={k} M={M} {dtype}", flush=True)
+            x = torch.randn(M, k, generator=g, device="cuda").to(dtype)
+            y = lin(x)
+            torch.cuda.synchronize()
+            _check_product(y, *_quant_ref(x.double()), w, sw, bias)
+            assert torch.equal(lin(_odd(x)), y)
+
+
 def test_linear_rows_do_not_see_each_other():
     """A NaN or an infinity stays in its row, and a NaN weight in its column."""
     g = _gen(21)
