@@ -6,10 +6,13 @@
 //
 //     max(1, tiles / 256 CUs) (BM + BN)
 //
-// the smaller one where two are equal. 128 x 64 only where each CU has one at most and without exact sums (1,024 rows, 4096 ->
-// 2048: 17.0 us, 64 x 64 18.6; two for some CUs, 1,100 rows: 27.8, 128 x 128 25.1; exact 26.0 against 25.4). 4096 -> 2048, us for 16 / 64 / 128 / 512 / 2,048 rows: 16 x 16 tiles 4.0 / 5.5 / 10.2 /
-// - / -, 16 x 32 5.1 / 5.4 / 8.2 / - / -, 32 x 32 6.0 / 6.4 / 6.6 / 17.3 / -, 64 x 64 9.3 / 9.6 / 9.6 / 11.3 / 34,
-// 128 x 128 17 / 18 / 18 / 22 / 27, 256 x 256 40 / 40 / 41 / 43 / 45.
+// the smaller one where two are equal. 16 x 16 only where each CU has one at most (two for some: 40 rows, 4096 -> 2048, 7.7 us,
+// 16 x 32 6.9), and 128 x 64 too, without exact sums (1,024 rows: 20.2 us, 64 x 64 23.3; two for some CUs, 1,100 rows: 27.8, 128 x
+// 128 20.8; exact 26.0 against 25.4). 4096 -> 2048, us, weights from HBM: 16 rows 6.6 and 32 rows 6.5 (16 x 16), 64 rows 7.2 (16 x
+// 32), 128 rows 8.6 and 256 rows 12.1 (32 x 32), 1,500 rows 25.0 (128 x 128). Every tile at every size, in an earlier form with
+// fewer stages, weights in the caches, us for 16 / 64 / 128 / 512 / 2,048 rows: 16 x 16 4.0 / 5.5 / 10.2 / - / -, 16 x 32 5.1 / 5.4 /
+// 8.2 / - / -, 32 x 32 6.0 / 6.4 / 6.6 / 17.3 / -, 64 x 64 9.3 / 9.6 / 9.6 / 11.3 / 34, 128 x 128 17 / 18 / 18 / 22 / 27, 256 x 256
+// 40 / 40 / 41 / 43 / 45.
 #include "exl3_kernels.h"
 
 namespace exl3 {
@@ -41,9 +44,9 @@ Pick pick_tile(int M, int n, int largest, bool exact) {
 
 }  // namespace
 
-// As many blocks of 128 as the workgroup has in hand at once (4 for each 16 lanes): 8 of 512 threads at 16 columns, 4 of 256
-// at 32. More rows are quantised by a launch of their own: 2048 -> 1024, 8 rows 5.1 us, by two launches 6.1; 4096 -> 2048, 8
-// rows 8.0 us, by two launches 7.4.
+// As many blocks of 128 as the workgroup has in hand at once (4 for each 16 lanes of up to 512 threads at 16 columns, of 256 at
+// 32). More rows are quantised by a launch of their own: 2048 -> 1024, 8 rows 5.1 us, by two launches 6.1; 4096 -> 2048, 8 rows
+// 8.0 us, by two launches 7.4.
 bool fp8_product_quantises(int M, int k, int n) {
     return M <= 16 && (int64_t)M * fp8_blocks(k) <= (pick_tile(M, n, kTile16x32, false).tile == kTile16 ? 128 : 64);
 }

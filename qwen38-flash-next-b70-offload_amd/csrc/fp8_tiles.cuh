@@ -368,28 +368,35 @@ void launch_fp8_tiles(const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
                        own, st, a, mt, nt, per, out_dt);
 }
 
-// `few`: at most one workgroup per CU, so that it may have the CU's LDS
+// `few`: at most one workgroup per CU, so that it may have the CU's LDS. More stages pay where more than two steps follow each
+// other (weights from HBM, us: 4096 -> 2048, 16 rows 7.2 -> 6.6, 64 rows 9.5 -> 7.2, exact 9.8 -> 7.3, 128 rows 10.6 -> 8.6, exact
+// 11.2 -> 9.2; with one step, k 512, 17 rows 3.2 -> 3.7), and e4m3's 128 x 128 as one group of 8 waves, whose registers allow it
+// (1,500 rows 28.0 -> 25.0; exact, whose waves would convert more, 36.0 -> 40.2).
+// Rows quantised inside: as many blocks of 128 as 256 threads have in hand at once, else 512 threads (4096 -> 2048, 1 row 6.0
+// us, with 512 7.0; 2048 -> 1024, 8 rows 6.0 and 5.2). As few rows that were quantised before take the same groups of waves, so
+// that the product is the same to the last bit.
 template <bool EXACT>
 void launch_fp8_tile(int tile, bool few, const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
+    const bool little = a.M <= 16 && (int64_t)a.M * a.kb <= 64;
     if (!a.q) {                                      // (no other tile may have these: their rows come from q)
-        if (tile == kTile16) launch_fp8_tiles<EXACT, true, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
+        if (tile == kTile16 && little) launch_fp8_tiles<EXACT, true, 16, 16, 1, 1, 4, 4>(a, out_dt, st);
+        else if (tile == kTile16) launch_fp8_tiles<EXACT, true, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
         else launch_fp8_tiles<EXACT, true, 16, 32, 1, 2, 2, 4>(a, out_dt, st);
         return;
     }
     if constexpr (EXACT) {
         if (few && tile == kTile128) return launch_fp8_tiles<EXACT, false, 128, 128, 2, 2, 2, 2>(a, out_dt, st);
     } else {
-        // e4m3 MFMAs leave the loads to wait for, so that more stages pay where the CU's LDS is there for them: up to 32 x 32
-        // from three steps on (4096 -> 2048, 64 rows 5.9 -> 5.2 us, 128 rows 6.7 -> 6.2; k 512, one step: 3.4 -> 3.8), and 128 x
-        // 128 as one group of 8 waves, whose registers allow it (2,048 rows, 27.5 -> 25.5 us, 1,500 rows 25.9 -> 22.9). Exact
-        // sums lose: 128 rows 7.3 -> 7.9 us, 2,048 rows 38.7 -> 42.7
-        if (few && tile == kTile16x32 && a.kb > 8) return launch_fp8_tiles<EXACT, false, 16, 32, 1, 2, 4, 4>(a, out_dt, st);
-        if (few && tile == kTile32 && a.kb > 8) return launch_fp8_tiles<EXACT, false, 32, 32, 1, 2, 4, 4>(a, out_dt, st);
         if (few && tile == kTile128) return launch_fp8_tiles<EXACT, false, 128, 128, 2, 4, 1, 4>(a, out_dt, st);
         if (tile == kTile128x64) return launch_fp8_tiles<EXACT, false, 128, 64, 4, 2, 1, 4>(a, out_dt, st);
     }
-    if (tile == kTile16) launch_fp8_tiles<EXACT, false, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
+    if (tile == kTile16 && little) launch_fp8_tiles<EXACT, false, 16, 16, 1, 1, 4, 4>(a, out_dt, st);
+    else if (tile == kTile16x32 && little) launch_fp8_tiles<EXACT, false, 16, 32, 1, 2, 2, 4>(a, out_dt, st);
+    else if (tile == kTile16 && few && a.kb > 16) launch_fp8_tiles<EXACT, false, 16, 16, 1, 1, 8, 4>(a, out_dt, st);
+    else if (tile == kTile16) launch_fp8_tiles<EXACT, false, 16, 16, 1, 1, 8, 2>(a, out_dt, st);
+    else if (tile == kTile16x32 && few && a.kb > 8) launch_fp8_tiles<EXACT, false, 16, 32, 1, 2, 4, 4>(a, out_dt, st);
     else if (tile == kTile16x32) launch_fp8_tiles<EXACT, false, 16, 32, 1, 2, 4, 2>(a, out_dt, st);
+    else if (tile == kTile32 && few && a.kb > 8) launch_fp8_tiles<EXACT, false, 32, 32, 1, 2, 4, 4>(a, out_dt, st);
     else if (tile == kTile32) launch_fp8_tiles<EXACT, false, 32, 32, 1, 2, 4, 2>(a, out_dt, st);
     else if (tile == kTile64 && few) launch_fp8_tiles<EXACT, false, 64, 64, 2, 2, 2, 4>(a, out_dt, st);
     else if (tile == kTile64) launch_fp8_tiles<EXACT, false, 64, 64, 2, 2, 2, 2>(a, out_dt, st);

@@ -230,7 +230,7 @@ def test_linear_larger(M, n, k):
 
 
 @pytest.mark.parametrize("n,k,Ms", [(2000, 1300, (33, 40, 47, 64, 90, 100, 127, 300)), (2050, 4000, (64, 97, 128)),
-                                    (1990, 640, (770, 1000, 1090, 1500, 2200)), (5000, 2048, (1, 3, 4, 5, 8, 16, 17)),
+                                    (1990, 640, (770, 1000, 1090, 1500, 2200)), (5000, 2048, (1, 3, 4, 5, 8, 16, 17)), (1000, 4096, (1, 2, 3, 4, 5, 16, 17, 31)),
                                     (1100, 1152, (80, 2030)), (12200, 200, (100, 1100))])
 def test_linear_tiles(n, k, Ms):
     """Sizes of every tile, with one workgroup per CU at most and with more, and edges inside a tile."""
@@ -246,6 +246,7 @@ def test_linear_tiles(n, k, Ms):
             torch.cuda.synchronize()
             _check_product(y, *_quant_ref(x.double()), w, sw, bias)
             assert torch.equal(lin(_odd(x)), y)
+            assert torch.equal(lin.quantised(*_fp8().quant(x), dtype), y)
 
 
 def test_linear_rows_do_not_see_each_other():
