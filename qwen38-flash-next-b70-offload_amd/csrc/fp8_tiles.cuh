@@ -3,7 +3,7 @@
 // e4m3 operands, fp32 sums) and its two scales applied in fp32.
 //
 // What bounds it, by size: few rows, the weights' way from HBM and the steps of one workgroup, which are few and each waits for
-// its loads (1 row, 2048 -> 12,288: 7.4 us, 3.4 TB/s; 40 rows, 4096 -> 2048: 7.0 us); more, what a CU takes in (fp8_linear.hip);
+// its loads (1 row, 2048 -> 12,288: 7.4 us, 3.4 TB/s; 40 rows, 4096 -> 2048: 6.0 us); more, what a CU takes in (fp8_linear.hip);
 // the largest, MFMAs and the power they draw (fp8_tiles_e4m3.hip).
 //
 // The weights are the MFMA's A operand and the rows its B operand, so a lane's accumulators are four neighbouring columns
