@@ -6,13 +6,16 @@
 //
 //     max(1, tiles / 256 CUs) (BM + BN)
 //
-// the smaller one where two are equal. 16 x 16 only where each CU has one at most (two for some: 40 rows, 4096 -> 2048, 7.7 us,
-// 16 x 32 6.9), and 128 x 64 too, without exact sums (1,024 rows: 20.2 us, 64 x 64 23.3; two for some CUs, 1,100 rows: 27.8, 128 x
-// 128 20.8; exact 26.0 against 25.4). 4096 -> 2048, us, weights from HBM: 16 rows 6.6 and 32 rows 6.5 (16 x 16), 64 rows 7.2 (16 x
-// 32), 128 rows 8.6 and 256 rows 12.1 (32 x 32), 1,500 rows 25.0 (128 x 128). Every tile at every size, in an earlier form with
-// fewer stages, weights in the caches, us for 16 / 64 / 128 / 512 / 2,048 rows: 16 x 16 4.0 / 5.5 / 10.2 / - / -, 16 x 32 5.1 / 5.4 /
-// 8.2 / - / -, 32 x 32 6.0 / 6.4 / 6.6 / 17.3 / -, 64 x 64 9.3 / 9.6 / 9.6 / 11.3 / 34, 128 x 128 17 / 18 / 18 / 22 / 27, 256 x 256
-// 40 / 40 / 41 / 43 / 45.
+// the smaller one where two are equal, but for these, since a CU with one tile has its LDS for more stages (us, weights from HBM):
+// 16 x 16 and, of more than 16 rows, 16 x 32 only where each CU has one at most (4096 -> 2048, 40 rows 7.7, 16 x 32 6.9; 80 rows
+// 10.0, 32 x 32 7.9), 64 x 64 only so where 128 x 64 is (700 rows 20.4, 128 x 64 17.1), and that only so and without exact sums
+// (1,100 rows 27.8, 128 x 128 20.8; 1,024 rows, exact 26.0, 64 x 64 25.4).
+//
+// 4096 -> 2048, weights from HBM, us: 16 rows 6.6 and 32 rows 6.5 (16 x 16), 64 rows 7.2 (16 x 32), 128 rows 8.6 and 256 rows 12.1
+// (32 x 32), 700 rows 17.1 (128 x 64), 1,500 rows 25.0 (128 x 128). Every tile at every size, in an earlier form with fewer stages,
+// weights in the caches, us for 16 / 64 / 128 / 512 / 2,048 rows: 16 x 16 4.0 / 5.5 / 10.2 / - / -, 16 x 32 5.1 / 5.4 / 8.2 / - / -,
+// 32 x 32 6.0 / 6.4 / 6.6 / 17.3 / -, 64 x 64 9.3 / 9.6 / 9.6 / 11.3 / 34, 128 x 128 17 / 18 / 18 / 22 / 27, 256 x 256 40 / 40 / 41 /
+// 43 / 45.
 #include "exl3_kernels.h"
 
 namespace exl3 {
@@ -28,13 +31,14 @@ struct Pick {
 };
 Pick pick_tile(int M, int n, int largest, bool exact) {
     constexpr int kSizes[][2] = {{16, 16}, {16, 32}, {32, 32}, {64, 64}, {128, 64}, {128, 128}, {256, 256}};
+    auto tiles_of = [&](int i) { return (int64_t)((M - 1) / kSizes[i][0] + 1) * ((n - 1) / kSizes[i][1] + 1); };
+    const bool one_128x64 = !exact && tiles_of(kTile128x64) <= kCus;
     Pick best{};
     int64_t least = 0;
     for (int i = 0; i <= largest; ++i) {
-        const int bm = kSizes[i][0], bn = kSizes[i][1];
-        const int64_t tiles = (int64_t)((M - 1) / bm + 1) * ((n - 1) / bn + 1);
-        const int64_t bytes = (tiles > kCus ? tiles : kCus) * (bm + bn);
-        if (tiles > kCus && (i == kTile16 || i == kTile128x64) || exact && i == kTile128x64) continue;
+        const int64_t tiles = tiles_of(i), bytes = (tiles > kCus ? tiles : kCus) * (kSizes[i][0] + kSizes[i][1]);
+        if (tiles > kCus && (i == kTile16 || (i == kTile16x32 && M > 16) || (i == kTile64 && one_128x64))) continue;
+        if (i == kTile128x64 && !one_128x64) continue;
         // (of up to 512 threads, in eighths; the callers' limit is that of the largest)
         if (i < largest && (tiles + 7) * 512 >= kMaxThreads) continue;
         if (least == 0 || bytes < least) least = bytes, best = {i, tiles <= kCus};

@@ -231,7 +231,8 @@ def test_linear_larger(M, n, k):
 
 @pytest.mark.parametrize("n,k,Ms", [(2000, 1300, (33, 40, 47, 64, 90, 100, 127, 300)), (2050, 4000, (64, 97, 128)),
                                     (1990, 640, (770, 1000, 1090, 1500, 2200)), (5000, 2048, (1, 3, 4, 5, 8, 16, 17)), (1000, 4096, (1, 2, 3, 4, 5, 16, 17, 31)),
-                                    (1100, 1152, (80, 2030)), (12200, 200, (100, 1100))])
+                                    (1100, 1152, (80, 2030)), (12200, 200, (100, 1100)),
+                                    (8300, 640, (14, 16, 20)), (8200, 300, (128, 129))])
 def test_linear_tiles(n, k, Ms):
     """Sizes of every tile, with one workgroup per CU at most and with more, and edges inside a tile."""
     g = _gen(n + k)
