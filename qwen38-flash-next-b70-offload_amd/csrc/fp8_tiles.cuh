@@ -104,7 +104,7 @@ template <int THREADS, int DT, bool SILU, bool WIDE, class F>
 __device__ __forceinline__ void quant_rows(const Fp8ProductArgs& A, uint8_t* q, float* s, F between) {
     constexpr int kTogether = 4, kGroups = THREADS / 16;
     const int i = threadIdx.x & 15, tasks = A.M * A.kb, rb = own_row_bytes(A.kb);
-    const uint32_t magic = (65536 + A.kb - 1) / A.kb;        // t / kb for t < 65536 / kb (there are few: kOwnBlocks)
+    const uint32_t magic = (65536 + A.kb - 1) / A.kb;        // t / kb for t < 65536 / kb (t is below 128, and so is kb, or 128)
     auto row_of = [&](int t) { return (int)((uint32_t)t * magic >> 16); };
     int t0 = threadIdx.x >> 4;
     float v[kTogether][8];
