@@ -51,6 +51,18 @@ __device__ __forceinline__ float silu_times(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(p, e * kLn2, p)) * u;
 }
 
+// The same of gates below kSiluFar, for which exp(-g) may be beyond fp32 (from -88.8 down): the 1 beside it is less than 2^-57 of
+// it, so the value is g u exp(g), with exp(g) in two halves, 2^(-t / 2) (1 - e ln 2) 2^(-t / 2), so that it is lost only where the
+// product is too; e holds what t lost to log2(e)'s rounding too, 2e-8 of t. g = -inf gives NaN, as 0 times it is.
+constexpr float kSiluFar = -40.0f;
+__device__ __forceinline__ float silu_times_far(float g, float u) {
+    constexpr float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147180559945309f;
+    const float t = -g * kLog2e;
+    const float e = abs_bits(t) < 0x7F800000u ? __builtin_fmaf(-g, kLog2eRest, __builtin_fmaf(-g, kLog2e, -t)) : 0.0f;
+    const float h = __builtin_amdgcn_exp2f(-0.5f * t);
+    return g * h * u * __builtin_fmaf(h, -e * kLn2, h);
+}
+
 // 8 consecutive elements of a row as fp32. WIDE: 16-byte aligned and all inside the row; else one by one, from the `n`-th on
 // (n > 0) the last one again
 template <int DT, bool WIDE>
@@ -96,18 +108,29 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
 }
 
 // 8 of a block's 128 values before they are quantised: those of x at `at`, or silu(x[at]) x[at + k]; `n` of them (any
-// number, also negative) lie inside the row, the others are 0
+// number, also negative) lie inside the row, the others are 0. In two steps, for callers that load several blocks before they need
+// the first: what is in memory (u: only for silu), and the values out of it, in v
 template <int DT, bool SILU, bool WIDE>
-__device__ __forceinline__ void block_values(const void* x, size_t at, int k, int n, float (&v)[8]) {
+__device__ __forceinline__ void block_load(const void* x, size_t at, int k, int n, float (&v)[8], float (&u)[8]) {
     // (no branches: the rows' first elements are loaded for none)
     at = n > 0 ? at : 0;
     const int some = max(n, 1);
     load8<DT, WIDE>(x, at, some, v);
+    if constexpr (SILU) load8<DT, WIDE>(x, at + k, some, u);
+}
+template <bool SILU, bool WIDE>
+__device__ __forceinline__ void block_values(int n, float (&v)[8], const float (&u)[8]) {
     if constexpr (SILU) {
-        float u[8];
-        load8<DT, WIDE>(x, at + k, some, u);
+        float g[8], least = v[0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = silu_times(v[j], u[j]);
+        for (int j = 0; j < 8; ++j) {
+            g[j] = v[j];
+            least = __builtin_fminf(least, g[j]);
+            v[j] = silu_times(g[j], u[j]);
+        }
+        if (least < kSiluFar)                        // (rare, so a branch)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = g[j] < kSiluFar ? silu_times_far(g[j], u[j]) : v[j];
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (WIDE ? 0 : j) < n ? v[j] : 0.0f;

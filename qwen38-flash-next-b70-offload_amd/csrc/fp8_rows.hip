@@ -19,8 +19,9 @@ __global__ void __launch_bounds__(kRowsThreads) fp8_rows_kernel(Fp8RowsArgs A, i
     const int b = (blockIdx.x % chunks << shift) + (t & ((1 << shift) - 1));
     if (row >= A.M || b >= kb) return;               // (whole rows of 16 lanes)
     const int c = b * kFp8Block + i * 8;
-    float v[8], s;
-    block_values<DT, SILU, WIDE>(A.x, (size_t)row * A.x_stride + c, A.k, A.k - c, v);
+    float v[8], u[8], s;
+    block_load<DT, SILU, WIDE>(A.x, (size_t)row * A.x_stride + c, A.k, A.k - c, v, u);
+    block_values<SILU, WIDE>(A.k - c, v, u);
     *(uint2*)(A.q + ((size_t)row * kb + b) * kFp8Block + i * 8) = quant_block(v, s);
     if (i == 0) A.s[(size_t)row * kb + b] = s;
 }

@@ -107,21 +107,22 @@ __device__ __forceinline__ void quant_rows(const Fp8ProductArgs& A, uint8_t* q, 
     const uint32_t magic = (65536 + A.kb - 1) / A.kb;        // t / kb for t < 65536 / kb (t is below 128, and so is kb, or 128)
     auto row_of = [&](int t) { return (int)((uint32_t)t * magic >> 16); };
     int t0 = threadIdx.x >> 4;
-    float v[kTogether][8];
-    auto values = [&] {                              // (the loads of four blocks before the first is needed)
+    float v[kTogether][8], up[kTogether][8];
+    auto load = [&] {                                // (four blocks before the first is needed)
 #pragma unroll
         for (int u = 0; u < kTogether; ++u) {
             const int t = t0 + u * kGroups, m = row_of(t), c = (t - m * A.kb) * kFp8Block + i * 8;
-            block_values<DT, SILU, WIDE>(A.x, (size_t)m * A.x_stride + c, A.k, t < tasks ? A.k - c : 0, v[u]);
+            block_load<DT, SILU, WIDE>(A.x, (size_t)m * A.x_stride + c, A.k, t < tasks ? A.k - c : 0, v[u], up[u]);
         }
     };
-    values();
+    load();
     between();
     while (true) {
 #pragma unroll
         for (int u = 0; u < kTogether; ++u) {
             const int t = t0 + u * kGroups, m = row_of(t), b = t - m * A.kb;
             float sc;
+            block_values<SILU, WIDE>(t < tasks ? A.k - b * kFp8Block - i * 8 : 0, v[u], up[u]);
             const uint2 o = quant_block(v[u], sc);
             if (t >= tasks) continue;
             *(uint2*)(q + m * rb + b * kFp8Block + piece_at(m, i >> 1) * 16 + (i & 1) * 8) = o;
@@ -129,7 +130,7 @@ __device__ __forceinline__ void quant_rows(const Fp8ProductArgs& A, uint8_t* q, 
         }
         t0 += kTogether * kGroups;
         if (t0 >= tasks) break;
-        values();
+        load();
     }
 }
 

@@ -504,3 +504,65 @@ def test_layer_in_two_graphs_and_on_streams():
                 got[i].append(mlp(big[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(t, alone[i]) for i in range(2) for t in got[i])
+
+
+def _check_silu_gates(gates, ups):
+    """silu(gate) * up of single values, each a block of its own, so that its scale shows the value itself: 8 units of 2^-24
+    and the scale's own rounding, at every size of the value down to the smallest scale."""
+    for up in ups:
+        v = gates.double() / (1 + torch.exp(-gates.double())) * up
+        fits = v.abs() < 2.0 ** 127
+        g, v = gates[fits], v[fits]
+        q, s = _fp8().silu_mul_quant(torch.stack([g, torch.full_like(g, up)], 1))
+        torch.cuda.synchronize()
+        rs = (v.abs() / 448).clamp_min(2.0 ** -80)
+        off = (s[:, 0].double() - rs).abs() / rs
+        bad = ~(off <= 9 * 2.0 ** -24)
+        assert not bad.any(), (up, int(bad.sum()), g[bad][:8].tolist(), s[bad][:8, 0].tolist(), float(off.nan_to_num(9).max()) * 2 ** 24)
+        quo, got = v / rs, q[:, 0].double()
+        lo, hi = _e4m3(quo.abs() * (1 - 19 * 2.0 ** -24)), _e4m3(quo.abs() * (1 + 19 * 2.0 ** -24))
+        assert ((got.abs() >= lo) & (got.abs() <= hi) & ((got == 0) | (got.sign() == quo.sign()))).all()
+        assert (q.view(torch.uint8)[:, 1:] == 0).all()
+
+
+def _finite16(dtype):
+    """Every finite value of a 16-bit type."""
+    v = torch.arange(1 << 16, device="cuda").to(torch.uint16).view(dtype)
+    return v[v.isfinite()]
+
+
+def test_silu_of_large_negative_gates():
+    """Gates at which exp(-gate) passes fp32's largest value, every one of the 16-bit types, with ups of 1 and ups for which the
+    product is no zero all the same."""
+    for dtype, ups in ((torch.bfloat16, (1.0, 2.0 ** 40, 2.0 ** 90)), (torch.float16, (1.0, 2.0 ** 15))):
+        print(f"case fp8 silu of large negative gates {dtype}", flush=True)
+        v = _finite16(dtype)
+        _check_silu_gates(v[v <= -40], ups)
+    steps = torch.cat([torch.linspace(-140, -40, 200_001, device="cuda"), -torch.exp2(torch.arange(6, 128, device="cuda").float()),
+                       torch.tensor([-torch.finfo(torch.float32).max], device="cuda")])
+    print("case fp8 silu of large negative gates float32", flush=True)
+    _check_silu_gates(steps, (1.0, 2.0 ** 40, 2.0 ** 100))
+
+
+@pytest.mark.parametrize("M", [1, 4, 37, 300])
+def test_mlp_of_large_negative_gates(M):
+    """Columns whose gate is far below 0 count for nothing, as those with a gate of 0 do, whether the rows are quantised within
+    the products or before."""
+    fp8, g, k, I = _fp8(), _gen(51), 512, 384  # noqa: E741
+    w, sw = _weight(g, 2 * I, k)
+    raw = w.view(torch.uint8).clone()
+    raw[:I] = 0                                              # (the gates are their biases, exactly)
+    down = fp8.Fp8Linear(*_weight(g, k, I))
+    gates = torch.randn(I, generator=g, device="cuda").bfloat16().float()
+    far = torch.tensor([-91.0, -95.0, -110.0, -128.0, -256.0, -1000.0, -90.0, -200.0], device="cuda")
+    biases = []
+    for values in (far, torch.zeros_like(far)):
+        b = torch.cat([gates, torch.zeros(I, device="cuda")])
+        b[3:3 + 40 * 8:8] = values.repeat(5)
+        biases.append(b)
+    for dtype in DTYPES:
+        print(f"case fp8 mlp of large negative gates M={M} {dtype}", flush=True)
+        x = torch.randn(M, k, generator=g, device="cuda").to(dtype)
+        y, want = (fp8.Fp8Mlp(fp8.Fp8Linear(raw.view(w.dtype), sw, b), down)(x) for b in biases)
+        torch.cuda.synchronize()
+        assert y.isfinite().all() and torch.equal(y, want)
