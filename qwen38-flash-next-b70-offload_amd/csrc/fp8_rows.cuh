@@ -41,26 +41,32 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
 
-// silu(g) * u = g u / (1 + exp(-g)). exp(-g) = 2^t (1 + e ln 2) with t = -g log2(e) rounded and e what the rounding lost, on
-// the hardware's exp2 and reciprocal: about 3 units in the last place. g = +-inf has no e.
+// silu(g) * u = g u / (1 + exp(-g)). exp(-g) = 2^t (1 + e ln 2) with t = -g log2(e) rounded and e what that lost, to the
+// product's rounding and to log2(e)'s own (1.3e-8 of t: 9 units of 2^-24 at g = -40), on the hardware's exp2 and
+// reciprocal: within 8 units of 2^-24. g = +-inf has no e.
+constexpr float kLn2 = 0.693147180559945309f;
+struct ExpMinus {
+    float t, e;
+    __device__ __forceinline__ explicit ExpMinus(float g) {
+        constexpr float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299e-8f;
+        t = -g * kLog2e;
+        e = abs_bits(t) < 0x7F800000u ? __builtin_fmaf(-g, kLog2eRest, __builtin_fmaf(-g, kLog2e, -t)) : 0.0f;
+    }
+};
 __device__ __forceinline__ float silu_times(float g, float u) {
-    constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
-    const float t = -g * kLog2e;
-    const float e = abs_bits(t) < 0x7F800000u ? __builtin_fmaf(-g, kLog2e, -t) : 0.0f;
-    const float p = __builtin_amdgcn_exp2f(t);
-    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(p, e * kLn2, p)) * u;
+    const ExpMinus x(g);
+    const float p = __builtin_amdgcn_exp2f(x.t);
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(p, x.e * kLn2, p)) * u;
 }
 
 // The same of gates below kSiluFar, for which exp(-g) may be beyond fp32 (from -88.8 down): the 1 beside it is less than 2^-57 of
 // it, so the value is g u exp(g), with exp(g) in two halves, 2^(-t / 2) (1 - e ln 2) 2^(-t / 2), so that it is lost only where the
-// product is too; e holds what t lost to log2(e)'s rounding too, 2e-8 of t. g = -inf gives NaN, as 0 times it is.
+// product is too. g = -inf gives NaN, as 0 times it is.
 constexpr float kSiluFar = -40.0f;
 __device__ __forceinline__ float silu_times_far(float g, float u) {
-    constexpr float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147180559945309f;
-    const float t = -g * kLog2e;
-    const float e = abs_bits(t) < 0x7F800000u ? __builtin_fmaf(-g, kLog2eRest, __builtin_fmaf(-g, kLog2e, -t)) : 0.0f;
-    const float h = __builtin_amdgcn_exp2f(-0.5f * t);
-    return g * h * u * __builtin_fmaf(h, -e * kLn2, h);
+    const ExpMinus x(g);
+    const float h = __builtin_amdgcn_exp2f(-0.5f * x.t);
+    return g * h * u * __builtin_fmaf(h, -x.e * kLn2, h);
 }
 
 // 8 consecutive elements of a row as fp32. WIDE: 16-byte aligned and all inside the row; else one by one, from the `n`-th on

@@ -566,3 +566,12 @@ def test_mlp_of_large_negative_gates(M):
         y, want = (fp8.Fp8Mlp(fp8.Fp8Linear(raw.view(w.dtype), sw, b), down)(x) for b in biases)
         torch.cuda.synchronize()
         assert y.isfinite().all() and torch.equal(y, want)
+
+
+def test_silu_every_gate():
+    """Every finite gate of the 16-bit types and closely spaced ones of fp32, each value by itself."""
+    for dtype, ups in ((torch.bfloat16, (1.0, -2.0 ** 40)), (torch.float16, (1.0, -2.0 ** 15))):
+        print(f"case fp8 silu of every gate {dtype}", flush=True)
+        _check_silu_gates(_finite16(dtype), ups)
+    print("case fp8 silu of every gate float32", flush=True)
+    _check_silu_gates(torch.linspace(-60, 60, 1_000_001, device="cuda"), (1.0, 3.0))
