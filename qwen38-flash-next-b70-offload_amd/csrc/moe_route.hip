@@ -7,8 +7,9 @@
 //   groups  E / n_group neighbouring experts each; a group's value is its largest key, with a bias the sum of its two
 //           largest; only the experts of the topk_group best groups compete
 //   picks   keys descending, equal keys by index; NaN counts as the largest
-//   weight  the pick's score (renormalised: over the picks' sum, the softmax taken over the picks' own logits, so that
-//           nothing underflows), times scale; a sum of 0 (every pick at -inf) gives weights of 0
+//   weight  the pick's score (renormalised: over the picks' sum, the softmax taken over the picks' own logits, and sigmoids that
+//           are all small relative to the largest pick's, so that nothing underflows), times scale; a sum of 0 (every pick at
+//           -inf, or a sigmoid of less than -700) gives weights of 0
 //
 // One wave per row; the instructions of 8 waves per SIMD bound 8,192 rows (logits arrive at 2.2 TB/s), the chain of the picks
 // one row. GPU time, us, for 1 / 200 / 8,192 rows: 512 experts, top 10: 3.2 / 3.7 / 7.7, with a bias 5.0 / 5.6 / 15.4; 256 in
@@ -140,9 +141,10 @@ __device__ __forceinline__ void logits_wide(const void* p, size_t at, float (&v)
     for (int j = 0; j < NPL; ++j) v[j] = logit_at<DT>(u.x, j);
 }
 
-// 1 / (1 + e^-l), 0 below -700: the hardware's reciprocal (2^-23) and two steps of Newton's
+// 1 / (1 + e^-l), 0 below kLeastLogit: the hardware's reciprocal (2^-23) and two steps of Newton's
+constexpr float kLeastLogit = -700.0f;
 __device__ __forceinline__ double sigmoid64(float l) {
-    const bool low = l < -700.0f;
+    const bool low = l < kLeastLogit;
     const double d = 1.0 + exp(low ? 700.0 : -(double)l);
     double r = __builtin_amdgcn_rcp(d);
     r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
@@ -356,7 +358,12 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs A, in
     else w = (float)((BIAS ? exp((double)x - top) : (Val)expf(x - (float)top)) / total);
     if (!live) w = 0;
     if (A.renormalize) {
-        const float sum = wave_sum(w);
+        float sum = wave_sum(w);
+        if (A.sigmoid && sum < 0x1p-24f) {           // every pick's score is exp(x) to 2^-24, and may be below fp32's smallest
+            const float most = BIAS ? value_of(wave_max(live ? key_of(x) : 0u)) : lane_value(x, 0);
+            w = x < kLeastLogit ? 0.0f : expf(x - most);
+            sum = wave_sum(w);
+        }
         w /= sum == 0 ? 1.0f : sum;
     }
     if (live) {

@@ -9,7 +9,7 @@ balance's) by score + bias; with n_group > 1 only the experts of the topk_group 
 group's value being its largest score, or with a bias the sum of its two largest scores + bias. Picks are in descending
 order, equal ones by index, and always topk different experts. The weights are the picks' scores (without the bias), with
 renormalize over their sum, times scale. An expert whose logit is -inf has score 0: it is picked only where fewer than topk
-others are left, and a row of -inf gets weights of 0. A NaN logit counts as the largest and gives NaN weights.
+others are left, and a row of -inf gets weights of 0. (The sigmoid of a logit below -700 counts as 0.) A NaN logit counts as the largest and gives NaN weights.
 
 The reference's plugin gets ids and weights from its caller's router (plugin/sglang_plugin.tier.py:531-561).
 """

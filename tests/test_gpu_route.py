@@ -278,3 +278,20 @@ def test_route_on_a_stream_and_in_a_graph():
         r(inputs[3 - i])                                    # eager work between the replays
         torch.cuda.synchronize()
         assert torch.equal(ids, want[i][0]) and torch.equal(w, want[i][1])
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_route_sigmoid_weights_far_below(bias):
+    """Renormalised sigmoid weights are those of the scores also where every pick's score is far below fp32's smallest."""
+    g = torch.Generator(device="cuda").manual_seed(19)
+    at = torch.tensor([-10.0, -15.0, -16.0, -16.6, -16.7, -17.0, -18.0, -20.0, -50.0, -80.0, -86.0, -87.5, -88.0, -88.8, -90.0, -100.0,
+                       -200.0, -500.0, -650.0], device="cuda")
+    for E, topk, groups in ((64, 8, {}), (130, 9, {}), (512, 10, {}), (256, 8, dict(n_group=8, topk_group=4))):
+        lg = torch.randn(40, E, generator=g, device="cuda")
+        lg[:19] += at[:, None]
+        lg[19] = -100.0
+        b = 0.1 * torch.randn(E, generator=g, device="cuda") if bias else None
+        for dtype in DTYPES:
+            print(f"case route sigmoid far below E={E} bias={bias} {dtype}", flush=True)
+            ids, w = _check(lg.to(dtype), topk, scoring="sigmoid", bias=b, scale=2.5, **groups)
+            assert torch.allclose(w.sum(-1), torch.full((40,), 2.5, device="cuda"), rtol=1e-5)
