@@ -366,9 +366,11 @@ int exl3_table_update(int64_t* ptrs_all, int32_t* slot_of, int32_t* slot_key, in
  * EXL3_DT_*, `stride` elements between rows. scoring 0: softmax, 1: sigmoid. bias: fp32 [E] or NULL, added to the scores
  * for the choice alone. E / n_group neighbouring experts form a group, and only the experts of the topk_group best groups
  * compete (by their largest score; with a bias, by the sum of their two largest). Picks come in descending order of what
- * they are chosen by, equal ones by index; a NaN counts as the largest. w: the picks' scores, over their sum with
- * renormalize (0 where that sum is 0: a row of -inf; the sigmoid of a logit below -700 counts as 0), times scale. The ids of
- * a row are always topk different experts. 1 <= E <= 1024, topk <= 64 and <= topk_group * E / n_group, n_group <= 64 and a
+ * they are chosen by, equal ones by index; a NaN counts as the largest (a NaN or +inf logit makes every softmax score of its
+ * row NaN: with a bias the first of those that compete are picked). w: the picks' scores, over their sum with renormalize (the
+ * softmax's from the picks' own logits; 0 where that sum is 0: a row of -inf; the sigmoid of a logit below -700 counts as 0),
+ * times scale. A logit of -inf has score 0 and with a bias competes with that alone. The ids of a row are always topk
+ * different experts. 1 <= E <= 1024, topk <= 64 and <= topk_group * E / n_group, n_group <= 64 and a
  * divisor of E, M < 2^26 - 64. ids: int32, w: fp32 [M, topk]. */
 int exl3_moe_route(const void* logits, int dtype, int64_t stride, int M, int E, const float* bias, int topk, int scoring,
                    int n_group, int topk_group, int renormalize, float scale, int32_t* ids, float* w, void* stream);

@@ -8,8 +8,13 @@ Scores are softmax(logits) or sigmoid(logits) over the experts. The choice goes 
 balance's) by score + bias; with n_group > 1 only the experts of the topk_group best groups of neighbours compete, a
 group's value being its largest score, or with a bias the sum of its two largest scores + bias. Picks are in descending
 order, equal ones by index, and always topk different experts. The weights are the picks' scores (without the bias), with
-renormalize over their sum, times scale. An expert whose logit is -inf has score 0: it is picked only where fewer than topk
-others are left, and a row of -inf gets weights of 0. (The sigmoid of a logit below -700 counts as 0.) A NaN logit counts as the largest and gives NaN weights.
+renormalize over their sum, times scale.
+
+An expert whose logit is -inf has score 0. Without a bias it is picked only where fewer than topk others are left; with one it
+competes with its bias alone, so an expert that must not be picked needs a bias of -inf. A row of -inf gets weights of 0. (The
+sigmoid of a logit below -700 counts as 0.) A NaN logit counts as the largest and gives NaN weights, but for softmax with a bias:
+there a NaN or +inf logit makes every score of its row NaN, so the first topk experts of those that compete are picked, and
+with renormalize the weights come from the picks' own logits.
 
 The reference's plugin gets ids and weights from its caller's router (plugin/sglang_plugin.tier.py:531-561).
 """

@@ -295,3 +295,26 @@ def test_route_sigmoid_weights_far_below(bias):
             print(f"case route sigmoid far below E={E} bias={bias} {dtype}", flush=True)
             ids, w = _check(lg.to(dtype), topk, scoring="sigmoid", bias=b, scale=2.5, **groups)
             assert torch.allclose(w.sum(-1), torch.full((40,), 2.5, device="cuda"), rtol=1e-5)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_masked_experts_and_a_bias(scoring):
+    """A logit of -inf leaves the bias alone to compete; a bias of -inf rules the expert out. NaN and +inf with softmax scores and
+    a bias: the first experts that compete, weighed by their own logits."""
+    lg = torch.full((3, 8), -3.0, device="cuda")
+    lg[:, 6] = -math.inf
+    bias = torch.zeros(8, device="cuda")
+    bias[6] = 2.0
+    ids, w = _check(lg, 2, scoring=scoring, bias=bias)
+    assert ids.tolist() == [[6, 0]] * 3 and w.tolist() == [[0.0, 1.0]] * 3
+    bias[6] = -math.inf
+    ids, w = _check(lg, 2, scoring=scoring, bias=bias)
+    assert ids.tolist() == [[0, 1]] * 3 and w.tolist() == [[0.5, 0.5]] * 3
+    lg[1, 7], lg[2, 7] = math.nan, math.inf
+    ids, w = _router(2, scoring=scoring, bias=bias)(lg)
+    torch.cuda.synchronize()
+    if scoring == "softmax":
+        assert ids.tolist() == [[0, 1]] * 3 and w.tolist() == [[0.5, 0.5]] * 3
+        assert _router(2, bias=bias, renormalize=False)(lg)[1][1:].isnan().all()
+    else:
+        assert ids.tolist() == [[0, 1], [7, 0], [7, 0]] and w[1].isnan().all() and w[2].isfinite().all()
