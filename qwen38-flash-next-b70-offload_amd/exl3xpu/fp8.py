@@ -41,7 +41,8 @@ def silu_mul_quant(gate_up: torch.Tensor):
 
 class Fp8Linear:
     """x @ weight^T + bias for weight [n, k] in float8_e4m3fn with weight_scale fp32 [ceil(n / 128), ceil(k / 128)] (the
-    value is weight * its block's scale). A k that is no multiple of 128 is padded with zeros here, once."""
+    value is weight * its block's scale). Weights whose k is no multiple of 128 are padded with zeros here, and those that do not
+    start on 16 bytes copied, once."""
 
     def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None, device=None):
         """Tensors move to `device` (the weight's by default). Raises ValueError on shapes or types that do not fit."""
@@ -56,7 +57,9 @@ class Fp8Linear:
         device = weight.device if device is None else torch.device(device)
         pad = blocks[1] * BLOCK - self.k
         raw = weight.detach().to(device).view(torch.uint8)
-        self.weight = (torch.nn.functional.pad(raw, (0, pad)) if pad else raw.contiguous()).view(torch.float8_e4m3fn)
+        raw = torch.nn.functional.pad(raw, (0, pad)) if pad else raw.contiguous()
+        # (the op takes weights that start on 16 bytes; a view into a larger buffer may not)
+        self.weight = (raw.clone() if raw.data_ptr() % 16 else raw).view(torch.float8_e4m3fn)
         self.weight_scale = weight_scale.detach().to(device, torch.float32).contiguous()
         self.bias = None if bias is None else bias.detach().to(device, torch.float32).contiguous()
         self._linear, self._matmul = _op("fp8_linear"), _op("fp8_matmul")

@@ -575,3 +575,16 @@ def test_silu_every_gate():
         _check_silu_gates(_finite16(dtype), ups)
     print("case fp8 silu of every gate float32", flush=True)
     _check_silu_gates(torch.linspace(-60, 60, 1_000_001, device="cuda"), (1.0, 3.0))
+
+
+def test_linear_of_weights_at_odd_addresses():
+    g = _gen(53)
+    w, sw = _weight(g, 130, 256)
+    x = torch.randn(20, 256, generator=g, device="cuda").bfloat16()
+    want = _fp8().Fp8Linear(w, sw)(x)
+    for at in (1, 8, 15):
+        store = torch.zeros(w.numel() + 16, dtype=torch.uint8, device="cuda")
+        v = store[at:at + w.numel()].view(w.dtype).view(w.shape)
+        v.copy_(w)
+        print(f"case fp8 weights at byte {at}", flush=True)
+        assert torch.equal(_fp8().Fp8Linear(v, sw)(x), want)

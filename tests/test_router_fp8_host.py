@@ -148,3 +148,12 @@ def test_classes_refuse():
         with pytest.raises(ValueError):
             bad()
     assert routing.Router(2, bias=torch.zeros(8, dtype=torch.bfloat16)).bias.dtype == torch.float32
+
+
+def test_weights_at_any_address():
+    """Weights cut out of a larger buffer, as a checkpoint's file is one, are moved to an address that the kernels take."""
+    store = torch.arange(128 * 256 + 16, dtype=torch.int64).remainder(126).to(torch.uint8)
+    for at in range(16):
+        w = store[at:at + 128 * 256].view(torch.float8_e4m3fn).view(128, 256)
+        lin = fp8.Fp8Linear(w, torch.ones(1, 2))
+        assert lin.weight.data_ptr() % 16 == 0 and torch.equal(lin.weight.view(torch.uint8), w.view(torch.uint8))
