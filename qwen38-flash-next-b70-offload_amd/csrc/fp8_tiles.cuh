@@ -87,9 +87,10 @@ __device__ __forceinline__ void to_lds(void* lds, Rsrc from, uint32_t lane_off, 
 // of 16 rows meet every bank once
 __device__ __forceinline__ int piece_at(int row, int c) { return c ^ ((row >> 1) & 7); }
 
-// One block of k of a tile's operands. QB rows of q (none where the workgroup quantises its rows itself)
+// One block of k of a tile's operands. QB rows of q (none where the workgroup quantises its rows itself). On 16 bytes, as the loads
+// to LDS and the fragments' reads are
 template <int QB, int BN>
-struct Stage {
+struct alignas(16) Stage {
     uint8_t w[BN * 128];
     uint8_t q[QB ? QB * 128 : 16];
     float s[QB < 64 ? 64 : QB];
@@ -165,9 +166,10 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, WM * WN * KG <= 4 ? 2 : 1)
         Stage<QB, BN> stage[KG][ST];
         struct {
             v4f sums[KG > 1 ? KG - 1 : 1][KG > 1 ? NW : 1][TM * TN][KG > 1 ? 64 : 1];
-            uint16_t out[NW][TM * 16 * TN * 16];
+            alignas(16) uint16_t out[NW][TM * 16 * TN * 16];
         } last;
     };
+    static_assert(alignof(Lds) >= 16);
     __shared__ Lds lds;
     extern __shared__ __attribute__((aligned(16))) uint8_t own[];
     const int l = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = l >> 4, r = l & 15;

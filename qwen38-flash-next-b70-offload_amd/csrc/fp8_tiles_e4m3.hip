@@ -15,8 +15,9 @@ __global__ void __launch_bounds__(512) fp8_tile256_kernel(Fp8ProductArgs A, int 
     // reads any)
     struct Lds {
         Stage<B, B> stage[2];
-        uint16_t outs[NW][16 * TN * 16];             // 16 rows of a wave's outputs
+        alignas(16) uint16_t outs[NW][16 * TN * 16]; // 16 rows of a wave's outputs
     };
+    static_assert(alignof(Lds) >= 16);
     __shared__ Lds lds;
     const int l = lane_id(), wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = l >> 4, r = l & 15;
     const int first = (blockIdx.x & 7) * per, step = gridDim.x >> 3, end = min(first + per, mt * nt);
