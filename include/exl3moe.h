@@ -386,13 +386,12 @@ int exl3_fp8_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int 
  * once to out_dtype. q, s as above; w: e4m3 [n, kp], zeros behind column k; sw: fp32 [ceil(n / 128), kp / 128]; bias: fp32
  * [n] or NULL; q and w start on 16 bytes; k <= 2^22, n <= 2^27. For fp16 and bf16 outputs the sums of 128 products may be off
  * by 7 * 2^-13 of their products' magnitudes at most (1.5e-5 of the output's size for normal values), for fp32 by no more than
- * fp32 sums. workspace: exl3_fp8_matmul_workspace bytes (none at present), no state between calls; its size never falls as M
- * grows. */
+ * fp32 sums. workspace: none is needed, the query gives 0. No state between calls. */
 size_t exl3_fp8_matmul_workspace(int M, int k, int n);
 int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
                     void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
-/* the same of x [M, k], quantised within the call; its workspace starts on 16 bytes and is not shared by calls that run at
- * the same time */
+/* the same of x [M, k], quantised within the call; its workspace (whose size never falls as M grows) starts on 16 bytes and is
+ * not shared by calls that run at the same time */
 size_t exl3_fp8_linear_workspace(int M, int k, int n);
 int exl3_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const float* sw,
                     const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,

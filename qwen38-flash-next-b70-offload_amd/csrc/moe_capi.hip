@@ -1351,12 +1351,8 @@ int exl3_fp8_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int 
     return fp8_rows("fp8_silu_mul_quant", gate_up, dtype, stride, M, k, true, q, s, stream);
 }
 
-size_t exl3_fp8_matmul_workspace(int M, int k, int n) {
-    (void)M;
-    (void)k;
-    (void)n;
-    return 0;
-}
+// (groups of waves join their sums in LDS)
+size_t exl3_fp8_matmul_workspace(int, int, int) { return 0; }
 
 namespace {
 
@@ -1378,22 +1374,20 @@ int fp8_product(const char* what, Fp8ProductArgs a, int M, int k, int n, const v
 }  // namespace
 
 int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
-                    void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+                    void* out, int out_dtype, int64_t out_stride, void*, size_t, void* stream) {
     if (int r = fp8_product_checks("fp8_matmul", M, k, n, w, sw, bias, out, out_dtype, out_stride)) return r;
     if (M == 0) return EXL3_OK;
     if (!q || !s || !aligned(q, 16) || !aligned(s, 4)) return fail(EXL3_EINVAL, "fp8_matmul: q or s null or not aligned");
-    const size_t need = exl3_fp8_matmul_workspace(M, k, n);
-    if (need && (!workspace || workspace_bytes < need))
-        return fail(EXL3_EWORKSPACE, "fp8_matmul: workspace %zu < %zu bytes", workspace_bytes, need);
     Fp8ProductArgs a{};
     a.q = (const uint8_t*)q;
     a.s = s;
     return fp8_product("fp8_matmul launch", a, M, k, n, w, sw, bias, out, out_dtype, out_stride, stream);
 }
 
+// The quantised rows; asked for also of few rows, which the product quantises in LDS, so that the size never falls as M grows
 size_t exl3_fp8_linear_workspace(int M, int k, int n) {
     if (M <= 0 || k <= 0 || n <= 0) return 0;
-    return fp8_q_bytes(M, k) + fp8_s_bytes(M, k) + exl3_fp8_matmul_workspace(M, k, n);
+    return fp8_q_bytes(M, k) + fp8_s_bytes(M, k);
 }
 
 namespace {

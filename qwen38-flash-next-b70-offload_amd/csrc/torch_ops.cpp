@@ -635,11 +635,8 @@ at::Tensor fp8_matmul(const at::Tensor& q, const at::Tensor& s, const at::Tensor
     auto out = at::empty(with_last(q.sizes(), n), q.options().dtype(dtype));
     const int dt = dtype_code(out);
     if (M == 0) return out;
-    const size_t ws = exl3_fp8_matmul_workspace(M, k, (int)n);
-    at::Tensor buf;
-    if (ws) buf = at::empty({(int64_t)ws}, q.options().dtype(at::kByte));
     check(exl3_fp8_matmul(q.data_ptr(), s.data_ptr<float>(), M, k, (int)n, w.data_ptr(), sw.data_ptr<float>(), b,
-                          out.data_ptr(), dt, n, ws ? buf.data_ptr() : nullptr, ws, cur_stream(q)),
+                          out.data_ptr(), dt, n, nullptr, 0, cur_stream(q)),
           "fp8_matmul");
     return out;
 }
