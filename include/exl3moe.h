@@ -385,8 +385,9 @@ int exl3_fp8_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int 
 /* out[m][n] = sum over blocks b of s[m][b] sw[n / 128][b] (sum over k in b of q[m][k] w[n][k]) + bias[n], fp32 sums, rounded
  * once to out_dtype. q, s as above; w: e4m3 [n, kp], zeros behind column k; sw: fp32 [ceil(n / 128), kp / 128]; bias: fp32
  * [n] or NULL; q and w start on 16 bytes; k <= 2^22, n <= 2^27. For fp16 and bf16 outputs the sums of 128 products may be off
- * by 7 * 2^-13 of their products' magnitudes at most (1.5e-5 of the output's size for normal values), for fp32 by no more than
- * fp32 sums. workspace: none is needed, the query gives 0. No state between calls. */
+ * by 7 * 2^-13 of their products' magnitudes at most (1.5e-5 of the outputs' root mean square for normal values: small beside
+ * their rounding, but not for an output that cancels to a hundredth of the others), for fp32 by no more than fp32 sums: a
+ * caller who needs those asks for fp32 outputs and rounds them. workspace: none is needed, the query gives 0. No state between calls. */
 size_t exl3_fp8_matmul_workspace(int M, int k, int n);
 int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
                     void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);

@@ -588,3 +588,32 @@ def test_linear_of_weights_at_odd_addresses():
         v.copy_(w)
         print(f"case fp8 weights at byte {at}", flush=True)
         assert torch.equal(_fp8().Fp8Linear(v, sw)(x), want)
+
+
+@pytest.mark.parametrize("M,n,k", [(3, 200, 512), (40, 200, 512), (300, 256, 1024), (1100, 1000, 384), (2100, 2100, 256)])
+def test_products_of_every_size_and_sums_that_cancel(M, n, k):
+    """Operands spread evenly over e4m3's values, from 2^-9 to 448, and products that cancel in pairs: fp16 and bf16 outputs within
+    what the e4m3 MFMA may lose, fp32 outputs within fp32 sums; fp32 outputs rounded by the caller have neither loss."""
+    g = _gen(57 + M)
+
+    def codes(rows, cols):
+        c = torch.randint(0, 127, (rows, cols), generator=g, device="cuda") + 128 * torch.randint(0, 2, (rows, cols), generator=g, device="cuda")
+        return c.to(torch.uint8)
+    q, w = codes(M, k), codes(n, k)
+    s, sw = (torch.rand(a, b, generator=g, device="cuda") + 0.5 for a, b in ((M, k // 128), (-(-n // 128), k // 128)))
+    for cancel in (False, True):
+        if cancel:                                           # (neighbours with the same weight and opposite signs)
+            q[:, 1::2] = q[:, ::2] ^ 128
+            w[:, 1::2] = w[:, ::2]
+        qv, wv = q.view(torch.float8_e4m3fn), w.view(torch.float8_e4m3fn)
+        lin = _fp8().Fp8Linear(wv, sw)
+        for dtype in DTYPES:
+            print(f"case fp8 products of every size M={M} cancel={cancel} {dtype}", flush=True)
+            y = lin.quantised(qv, s, dtype)
+            torch.cuda.synchronize()
+            ref, mag = _product_ref(qv, s, wv, sw, None)
+            half, loss = torch.finfo(dtype).eps / 2, 0.0 if dtype == torch.float32 else 7 * 2.0 ** -13
+            tol = ((128 + 3 * s.size(-1) + 4) * 2.0 ** -23 + loss) * mag
+            tol = tol + half * (ref.abs() + tol)
+            fits = ref.abs() + tol < torch.finfo(dtype).max
+            assert fits.sum() > 50 and ((y.double() - ref).abs() <= tol)[fits].all()      # (fp16 cannot hold the others)
