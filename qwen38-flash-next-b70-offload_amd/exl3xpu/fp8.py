@@ -1,6 +1,7 @@
 """The 8-bit float linear beside the EXL3 one: weights in e4m3 with one fp32 scale per 128 x 128 block, rows quantised to
-e4m3 with one fp32 scale per 128 columns, fp32 sums (torch.ops.exl3xpu_C.fp8_*). What a checkpoint keeps in that form
-next to its EXL3 experts: projections, and the shared expert of an MoE layer.
+e4m3 with one fp32 scale per 128 columns, fp32 sums (torch.ops.exl3xpu_C.fp8_*). For layers whose weights are in that form
+next to EXL3 experts: projections, and the shared expert of an MoE layer. The caller's model builds and calls them; no loader
+here makes them out of a checkpoint.
 
   y = Fp8Linear(weight, weight_scale, bias=None)(x)        x [..., k] -> [..., n] of x's dtype
   y = Fp8Mlp(gate_up, down)(x)                             down(silu(gate) * up) of two Fp8Linear
@@ -9,7 +10,8 @@ next to its EXL3 experts: projections, and the shared expert of an MoE layer.
 
 q is float8_e4m3fn [..., k rounded up to 128] (zeros behind k), s fp32 [..., ceil(k / 128)], q s the value: s = max(amax /
 448, 2^-80), q = x / s rounded to the nearest, halves to even. Calls run on the device's current stream, keep no state and
-can be captured into a graph.
+can be captured into a graph. How many rows a call has picks the order of a product's sums: a row alone and the same row
+in a batch may differ in the last bits.
 """
 from __future__ import annotations
 
