@@ -1,21 +1,34 @@
 // Which tile computes an 8-bit float product (fp8_tiles.cuh has the kernel).
 //
-// A tile of BM rows x BN columns brings (BM + BN) 128 bytes to its CU per block of k, and a CU takes them in at 60-70 GB/s
-// whatever the tile (512 KB of a 64 x 64 tile at k 4096: 8.8 us; 256 KB of a 32 x 32 one: 4.0 us): what a CU has to bring in
-// is what takes the time, and the tile is the one for which that is least,
+// A tile of BM rows x BN columns brings (BM + BN) 128 bytes to its CU per block of k, and a CU takes them in at 42-46 GB/s
+// whatever the tile (4096 -> 2048, one tile per CU, weights from HBM: 256 KB of 32 x 32 in 8.8 us, 512 KB of 64 x 64 in 13.8, 1 MB
+// of 128 x 128 in 27.1, of each 2.4 any launch's): what a CU has to bring in is what takes the time, and the tile is the one for
+// which that is least,
 //
 //     max(1, tiles / 256 CUs) (BM + BN)
 //
-// the smaller one where two are equal, but for these, since a CU with one tile has its LDS for more stages (us, weights from HBM):
-// 16 x 16 and, of more than 16 rows, 16 x 32 only where each CU has one at most (4096 -> 2048, 40 rows 7.7, 16 x 32 6.9; 80 rows
-// 10.0, 32 x 32 7.9), 64 x 64 only so where 128 x 64 is (700 rows 20.4, 128 x 64 17.1), and that only so and without exact sums
-// (1,100 rows 27.8, 128 x 128 20.8; 1,024 rows, exact 26.0, 64 x 64 25.4).
+// the smaller one where two are equal, but for these, since a CU with one tile has its LDS for more stages: 16 x 16 and, of more
+// than 16 rows, 16 x 32 only where each CU has one at most (100 rows below), 64 x 64 only so where 128 x 64 is (700 rows), and that
+// only so (1,500 rows) and without exact sums (1,024 rows of those, in an earlier form: 26.0, 64 x 64 25.4).
 //
-// 4096 -> 2048, weights from HBM, us: 16 rows 6.6 and 32 rows 6.5 (16 x 16), 64 rows 7.2 (16 x 32), 128 rows 8.6 and 256 rows 12.1
-// (32 x 32), 700 rows 17.1 (128 x 64), 1,500 rows 25.0 (128 x 128). Every tile at every size, in an earlier form with fewer stages,
-// weights in the caches, us for 16 / 64 / 128 / 512 / 2,048 rows: 16 x 16 4.0 / 5.5 / 10.2 / - / -, 16 x 32 5.1 / 5.4 / 8.2 / - / -,
-// 32 x 32 6.0 / 6.4 / 6.6 / 17.3 / -, 64 x 64 9.3 / 9.6 / 9.6 / 11.3 / 34, 128 x 128 17 / 18 / 18 / 22 / 27, 256 x 256 40 / 40 / 41 /
-// 43 / 45.
+// Every tile, quantised rows, bf16 outputs, weights from HBM, us per call out of a graph; * is what the rule takes. With fp32
+// outputs, and at 2000 -> 1000, the rule's tile is the fastest as well, or within 7 % of it (the runs' own differences).
+//   4096 -> 2048, rows   16    64   100   128   256   512   700  1,000  1,500  2,048  4,096
+//   16 x 16            6.7*   8.2  13.0  13.5  24.4  45.7  53.8
+//   16 x 32            7.5    7.3* 10.0  10.3  19.7  29.8  33.5   48.3
+//   32 x 32            8.0    8.9   7.7*  8.8* 12.5* 22.2  27.1   38.8   50.4   71.9  131.4
+//   64 x 64           11.3   15.8  12.7  15.4  14.6  13.8* 20.3   22.0   34.9   43.9   75.4
+//   128 x 64                 16.7  21.2  24.1  22.8  21.3  17.1*  20.0*  33.4   39.5   77.5
+//   128 x 128                      26.5  29.3  27.5  26.4  22.6   25.1   25.4*  27.1*  45.9*
+//   256 x 256                                  57.7  53.9  54.9   56.2   52.5   53.1   53.4
+//   2048 -> 12,288
+//   16 x 16           10.8   25.2  40.4  45.3
+//   16 x 32            9.1*  16.0  23.8  26.4
+//   32 x 32            9.4   14.9  19.2  21.0  37.5  70.6
+//   64 x 64            8.6   10.4* 13.1  14.8  24.2  34.9  49.1   65.5   84.9  129.8  225.3
+//   128 x 64          10.1   10.7  12.2* 13.5* 22.4  32.5  45.5   58.8   79.1  119.4  233.5
+//   128 x 128         12.7   13.6  15.3  16.5  16.3* 26.6* 36.9   43.6   56.4   73.0  140.7
+//   256 x 256                28.4  30.0  30.2  31.4  30.2  29.9*  31.0*  54.6*  59.2*  96.4*
 #include "exl3_kernels.h"
 
 namespace exl3 {
@@ -49,8 +62,8 @@ Pick pick_tile(int M, int n, int largest, bool exact) {
 }  // namespace
 
 // As many blocks of 128 as the workgroup has in hand at once (4 for each 16 lanes of up to 512 threads at 16 columns, of 256 at
-// 32). More rows are quantised by a launch of their own: 2048 -> 1024, 8 rows 5.1 us, by two launches 6.1; 4096 -> 2048, 8 rows
-// 8.0 us, by two launches 7.4.
+// 32). More rows are quantised by a launch of their own (measured side by side: 2048 -> 1024, 8 rows 5.1 us, by two launches 6.1;
+// 4096 -> 2048, 8 rows 8.0 us, by two launches 7.4).
 bool fp8_product_quantises(int M, int k, int n) {
     return M <= 16 && (int64_t)M * fp8_blocks(k) <= (pick_tile(M, n, kTile16x32, false).tile == kTile16 ? 128 : 64);
 }

@@ -1,8 +1,8 @@
 // Quantised rows of the 8-bit float linear (fp8_rows.cuh), of x or of silu(gate) * up of fused gate|up rows.
 //
 // 16 lanes hold a block of 128 columns, 8 elements each (16 bytes of bf16 in, 8 bytes out), so the block's amax is four DPP
-// steps and each element is read once. One pass over the data: bound by memory. 8,192 x 2,048 bf16 11.0 us (4.6 TB/s; a copy
-// of that size 5.2), gate|up 8,192 x 2 x 512 6.4 us (3.3 TB/s); 301 x 1,000 fp16 2.5 us, of which 2.4 are any launch's.
+// steps and each element is read once. One pass over the data: bound by memory. us per call out of a graph: 8,192 x 2,048 bf16
+// 10.9 (4.7 TB/s; a large copy 5.2), gate|up 8,192 x 2 x 512 6.2 (3.4 TB/s); 301 x 1,000 fp16 2.4, any launch's.
 #include "exl3_kernels.h"
 #include "fp8_rows.cuh"
 

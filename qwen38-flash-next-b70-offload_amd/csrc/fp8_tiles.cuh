@@ -3,7 +3,7 @@
 // e4m3 operands, fp32 sums) and its two scales applied in fp32.
 //
 // What bounds it, by size: few rows, the weights' way from HBM and the steps of one workgroup, which are few and each waits for
-// its loads (1 row, 2048 -> 12,288: 7.4 us, 3.4 TB/s; 40 rows, 4096 -> 2048: 6.0 us); more, what a CU takes in (fp8_linear.hip);
+// its loads (medians of a kernel trace: 1 row, 2048 -> 12,288: 7.2 us, 3.5 TB/s; 40 rows, 4096 -> 2048: 5.8 us); more, what a CU takes in (fp8_linear.hip);
 // the largest, MFMAs and the power they draw (fp8_tiles_e4m3.hip).
 //
 // The weights are the MFMA's A operand and the rows its B operand, so a lane's accumulators are four neighbouring columns
@@ -160,7 +160,7 @@ __device__ __forceinline__ void quant_rows(const Fp8ProductArgs& A, uint8_t* q, 
 // the workgroup quantises its (up to 16) rows itself while its first weights are on their way, and `own` is their LDS.
 // EXACT: sums without the e4m3 MFMA's losses, outputs in fp16, bf16 or fp32 (out_dt 0, 1, 2); else fp16 or bf16 outputs.
 // Two waves per SIMD at least: with more registers than that leaves, MFMAs write accumulation registers, which the multiply-adds
-// cannot read (8,192 rows, 2048 -> 12,288, fp32 outputs: 412 us with the copies, 390 without).
+// cannot read (8,192 rows, 2048 -> 12,288, fp32 outputs, side by side: 412 us with the copies, 390 without).
 template <bool EXACT, bool OWN, int BM, int BN, int WM, int WN, int KG, int ST>
 __global__ void __launch_bounds__(64 * WM * WN * KG, WM * WN * KG <= 4 ? 2 : 1)
     fp8_tile_kernel(Fp8ProductArgs A, int mt, int nt, int per, int out_dt) {
@@ -273,8 +273,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, WM * WN * KG <= 4 ? 2 : 1)
                 for (int i = 0; i < TN; ++i) x[j & 1][i] = block_sum(wf[i], qf[j & 1]);
                 add(j ? j - 1 : TM - 1);
                 sc[j & 1] = st.s[wm + j * 16 + r] * sw;
-                // (the exact sums' conversions between their MFMAs too where there are 8 of those: 777 rows, 2000 -> 1000, 10.4 ->
-                // 9.9 us; with 4 of them, 256 rows, 5.8 against 5.7)
+                // (the exact sums' conversions between their MFMAs too where there are 8 of those: 777 rows, 2000 -> 1000, side by
+                // side, 10.4 -> 9.9 us; with 4 of them, 256 rows, 5.8 against 5.7)
                 constexpr bool kThrees = EXACT && TN > 1;
                 __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
@@ -376,7 +376,7 @@ void launch_fp8_tiles(const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
 }
 
 // `few`: at most one workgroup per CU, so that it may have the CU's LDS. More stages pay where more than two steps follow each
-// other (weights from HBM, us: 4096 -> 2048, 16 rows 7.2 -> 6.6, 64 rows 9.5 -> 7.2, exact 9.8 -> 7.3, 128 rows 10.6 -> 8.6, exact
+// other (weights from HBM, us per call out of a graph, side by side: 4096 -> 2048, 16 rows 7.2 -> 6.6, 64 rows 9.5 -> 7.2, exact 9.8 -> 7.3, 128 rows 10.6 -> 8.6, exact
 // 11.2 -> 9.2; with one step, k 512, 17 rows 3.2 -> 3.7), and e4m3's 128 x 128 as one group of 8 waves, whose registers allow it
 // (1,500 rows 28.0 -> 25.0; exact, whose waves would convert more, 36.0 -> 40.2).
 // Rows quantised inside: as many blocks of 128 as 256 threads have in hand at once, else 512 threads (4096 -> 2048, 1 row 6.0

@@ -6,8 +6,8 @@ namespace exl3 {
 // ---- 256 x 256 tiles, one after the other ---------------------------------------------------------------------------------
 // For the large products: as many workgroups as CUs, each with every 32nd tile of its XCD's run (its 32 CUs have neighbouring
 // ones at a time). A block's loads are issued while the block before is multiplied, the next tile's first among them, so that
-// they are on their way while this tile's outputs are stored. 8,192 rows, 2048 -> 12,288: 180 to 217 us over cards and values,
-// 1.9-2.3 PFLOP/s. MFMAs alone reach 4.6 (4.3 with the scales' multiply-adds); they are at work 69 % of a wave's time, at the
+// they are on their way while this tile's outputs are stored. 8,192 rows, 2048 -> 12,288, kernel trace: 217 us at the median, 181 to
+// 234 (1.9 PFLOP/s, 1.8-2.3), as the power allows. MFMAs alone reach 4.6 (4.3 with the scales' multiply-adds); they are at work 69 % of a wave's time, at the
 // 1.95 GHz that the power leaves.
 __global__ void __launch_bounds__(512) fp8_tile256_kernel(Fp8ProductArgs A, int mt, int nt, int per, int out_dt) {
     constexpr int B = 256, WM = 2, WN = 4, NW = WM * WN, TM = B / WM / 16, TN = B / WN / 16, kPieces = TN * 2;
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(512) fp8_tile256_kernel(Fp8ProductArgs A, int 
                     const v8u v = *(const v8u*)(o + (row * kPieces + (piece ^ (row & (kPieces - 1)))) * 8);
                     uint16_t* p = (uint16_t*)A.out + (size_t)m * A.out_stride + n;
                     if constexpr (decltype(full)::value) {
-                        // (past the caches: 178 us against 185 at 8,192 rows, 2048 -> 12,288)
+                        // (past the caches: 178 us against 185 in one run, 8,192 rows, 2048 -> 12,288)
                         __builtin_nontemporal_store(v, (v8u*)p);
                     } else if (m < A.M && n < A.n) {
                         if (wide && n + 8 <= A.n) *(v8u*)p = v;

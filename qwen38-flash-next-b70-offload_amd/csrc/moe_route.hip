@@ -11,10 +11,11 @@
 //           are all small relative to the largest pick's, so that nothing underflows), times scale; a sum of 0 (every pick at
 //           -inf, or a sigmoid of less than -700) gives weights of 0
 //
-// One wave per row; the instructions of 8 waves per SIMD bound 8,192 rows (logits arrive at 2.2 TB/s), the chain of the picks
-// one row. GPU time, us, for 1 / 200 / 8,192 rows: 512 experts, top 10: 3.2 / 3.7 / 7.7, with a bias 5.0 / 5.6 / 15.4; 256 in
-// 8 groups of which 4 compete, top 8: 3.4 / 3.8 / 7.5, with a bias 4.6 / 5.2 / 12.9; 128, top 8: 2.8 / 3.3 / 5.9, with a bias
-// 3.7 / 4.1 / 9.0.
+// One wave per row; the instructions of 8 waves per SIMD bound 8,192 rows (logits arrive at 1.9 TB/s), the chain of the picks
+// one row. us per call out of a graph, medians, for 1 / 200 / 8,192 rows of fp32: 512 experts, top 10: 3.3 / 3.8 / 8.9, with a bias
+// 5.0 / 5.6 / 17.0; 256 in 8 groups of which 4 compete, top 8, sigmoid: 3.4 / 3.8 / 7.3, with a bias 4.7 / 5.2 / 12.4; 128, top 8:
+// 2.8 / 3.1 / 5.2, with a bias and sigmoid 3.6 / 4.1 / 8.0. (8,192 rows took 7.7 to 8.9 and with a bias 15.4 to 17.0 on the cards
+// measured.)
 //
 // Lane i holds the E / 64 neighbouring experts from i * NPL, so the lowest lane of a tie holds the
 // lowest index; it sorts their keys (a network of max and min, without the indices). A pick is then one maximum over the
