@@ -370,8 +370,8 @@ int exl3_table_update(int64_t* ptrs_all, int32_t* slot_of, int32_t* slot_key, in
  * row NaN: with a bias the first of those that compete are picked). w: the picks' scores, over their sum with renormalize (the
  * softmax's from the picks' own logits; 0 where that sum is 0: a row of -inf; the sigmoid of a logit below -700 counts as 0),
  * times scale. A logit of -inf has score 0 and with a bias competes with that alone. The ids of a row are always topk
- * different experts. 1 <= E <= 1024, topk <= 64 and <= topk_group * E / n_group, n_group <= 64 and a
- * divisor of E, M < 2^26 - 64. ids: int32, w: fp32 [M, topk]. */
+ * different experts. 1 <= E <= 1024, topk <= 64 and <= topk_group * E / n_group, n_group <= 64 and a divisor of E, M < 2^26 - 64.
+ * ids: int32, w: fp32 [M, topk]. */
 int exl3_moe_route(const void* logits, int dtype, int64_t stride, int M, int E, const float* bias, int topk, int scoring,
                    int n_group, int topk_group, int renormalize, float scale, int32_t* ids, float* w, void* stream);
 
@@ -387,7 +387,8 @@ int exl3_fp8_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int 
  * [n] or NULL; q and w start on 16 bytes; k <= 2^22, n <= 2^27. For fp16 and bf16 outputs the sums of 128 products may be off
  * by 7 * 2^-13 of their products' magnitudes at most (1.5e-5 of the outputs' root mean square for normal values: small beside
  * their rounding, but not for an output that cancels to a hundredth of the others), for fp32 by no more than fp32 sums: a
- * caller who needs those asks for fp32 outputs and rounds them. workspace: none is needed, the query gives 0. No state between calls. */
+ * caller who needs those asks for fp32 outputs and rounds them. workspace: none is needed, the query gives 0. No state between
+ * calls. */
 size_t exl3_fp8_matmul_workspace(int M, int k, int n);
 int exl3_fp8_matmul(const void* q, const float* s, int M, int k, int n, const void* w, const float* sw, const float* bias,
                     void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);

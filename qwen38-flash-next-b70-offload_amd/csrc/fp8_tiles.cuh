@@ -3,8 +3,8 @@
 // e4m3 operands, fp32 sums) and its two scales applied in fp32.
 //
 // What bounds it, by size: few rows, the weights' way from HBM and the steps of one workgroup, which are few and each waits for
-// its loads (medians of a kernel trace: 1 row, 2048 -> 12,288: 7.2 us, 3.5 TB/s; 40 rows, 4096 -> 2048: 5.8 us); more, what a CU takes in (fp8_linear.hip);
-// the largest, MFMAs and the power they draw (fp8_tiles_e4m3.hip).
+// its loads (medians of a kernel trace: 1 row, 2048 -> 12,288: 7.2 us, 3.5 TB/s; 40 rows, 4096 -> 2048: 5.8 us); more, what a CU
+// takes in (fp8_linear.hip); the largest, MFMAs and the power they draw (fp8_tiles_e4m3.hip).
 //
 // The weights are the MFMA's A operand and the rows its B operand, so a lane's accumulators are four neighbouring columns
 // of one row: one row scale per lane.
@@ -376,9 +376,9 @@ void launch_fp8_tiles(const Fp8ProductArgs& a, int out_dt, hipStream_t st) {
 }
 
 // `few`: at most one workgroup per CU, so that it may have the CU's LDS. More stages pay where more than two steps follow each
-// other (weights from HBM, us per call out of a graph, side by side: 4096 -> 2048, 16 rows 7.2 -> 6.6, 64 rows 9.5 -> 7.2, exact 9.8 -> 7.3, 128 rows 10.6 -> 8.6, exact
-// 11.2 -> 9.2; with one step, k 512, 17 rows 3.2 -> 3.7), and e4m3's 128 x 128 as one group of 8 waves, whose registers allow it
-// (1,500 rows 28.0 -> 25.0; exact, whose waves would convert more, 36.0 -> 40.2).
+// other (weights from HBM, us per call out of a graph, side by side: 4096 -> 2048, 16 rows 7.2 -> 6.6, 64 rows 9.5 -> 7.2, exact
+// 9.8 -> 7.3, 128 rows 10.6 -> 8.6, exact 11.2 -> 9.2; with one step, k 512, 17 rows 3.2 -> 3.7), and e4m3's 128 x 128 as one group
+// of 8 waves, whose registers allow it (1,500 rows 28.0 -> 25.0; exact, whose waves would convert more, 36.0 -> 40.2).
 // Rows quantised inside: as many blocks of 128 as 256 threads have in hand at once, else 512 threads (4096 -> 2048, 1 row 6.0
 // us, with 512 7.0; 2048 -> 1024, 8 rows 6.0 and 5.2). As few rows that were quantised before take the same groups of waves, so
 // that the product is the same to the last bit.

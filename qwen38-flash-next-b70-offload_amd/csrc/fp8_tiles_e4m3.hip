@@ -6,9 +6,9 @@ namespace exl3 {
 // ---- 256 x 256 tiles, one after the other ---------------------------------------------------------------------------------
 // For the large products: as many workgroups as CUs, each with every 32nd tile of its XCD's run (its 32 CUs have neighbouring
 // ones at a time). A block's loads are issued while the block before is multiplied, the next tile's first among them, so that
-// they are on their way while this tile's outputs are stored. 8,192 rows, 2048 -> 12,288, kernel trace: 217 us at the median, 181 to
-// 234 (1.9 PFLOP/s, 1.8-2.3), as the power allows. MFMAs alone reach 4.6 (4.3 with the scales' multiply-adds); they are at work 69 % of a wave's time, at the
-// 1.95 GHz that the power leaves.
+// they are on their way while this tile's outputs are stored. 8,192 rows, 2048 -> 12,288, kernel trace: 217 us at the median, 181
+// to 234 (1.9 PFLOP/s, 1.8-2.3), as the power allows. MFMAs alone reach 4.6 (4.3 with the scales' multiply-adds); they are at work
+// 69 % of a wave's time, at the 1.95 GHz that the power leaves.
 __global__ void __launch_bounds__(512) fp8_tile256_kernel(Fp8ProductArgs A, int mt, int nt, int per, int out_dt) {
     constexpr int B = 256, WM = 2, WN = 4, NW = WM * WN, TM = B / WM / 16, TN = B / WN / 16, kPieces = TN * 2;
     // (one variable: where there are two the compiler tells their accesses apart, and waits for all loads to LDS before it
