@@ -407,6 +407,55 @@ int exl3_fp8_mlp(const void* x, int dtype, int64_t x_stride, int M, int k, int I
                  const float* gu_scale, const float* gu_bias, const void* dn, const float* dn_scale, const float* dn_bias,
                  void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- the norm, and the 4-bit float linear (none of these has a counterpart in the reference's op libraries) ----------- */
+
+/* h = x + residual, added in fp32 and rounded to the residual's type (x itself without a residual); y = h / sqrt(mean(h^2) +
+ * eps) * weight in fp32. x: [M, k] of x_dtype, row m at (m / inner) * x_outer + (m % inner) * x_stride elements (inner 1: at m *
+ * x_stride). residual: x_dtype or fp32, or NULL; held: h, [M, k] of the residual's type, which may be the residual itself (NULL
+ * without one). weight: fp32 [k] or NULL. y: [M, k] of x_dtype, or NULL. form 1: q and s as exl3_fp8_quant's, form 2: as
+ * exl3_fp4_quant's (s_stage as there), both of the fp32 values; 0: none. At least one of y and a form. eps is positive. Squares are
+ * summed in fp32: a row whose sum passes 3.4e38 gives 0 (NaN where it is infinite). k <= 2^22 and, by k, up to 2^22 rows. */
+int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64_t x_outer, const void* residual,
+                  int residual_dtype, int64_t residual_stride, void* held, const float* weight, float eps, int M, int k,
+                  void* y, int form, void* q, void* s, int64_t s_stage, void* stream);
+
+/* Rows of microscaled 4-bit floats (OCP MX: e2m1 with one power of two per 32 columns): scale 2^(floor(log2(amax)) - 2), 2^-126
+ * at the least, quotients rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, halves to even, 6 at the most. x: [M, k] of
+ * x_dtype with x_stride elements between rows. q: [M, kp / 2] bytes with kp = k rounded up to 128, two codes to a byte, the first
+ * in the low half, zeros behind column k. s: exponent + 127 in a byte, in ceil(k / 256) stages of [M, 8], s_stage bytes apart
+ * (a multiple of 8, M * 8 at the least): byte j of row m in stage b is for columns 256 b + 32 j; 0 behind column k. An infinite or
+ * NaN element makes its block's byte 255, which is NaN. q starts on 16 bytes, s on 8. k <= 2^22, and M ceil(k / 256) < 2^27. */
+int exl3_fp4_quant(const void* x, int x_dtype, int64_t x_stride, int M, int k, void* q, void* s, int64_t s_stage, void* stream);
+/* the same of silu(gate) * up (in fp32) of gate|up rows [M, 2 k] */
+int exl3_fp4_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int M, int k, void* q, void* s, int64_t s_stage,
+                            void* stream);
+/* the values of such rows, [M, k] of out_dtype */
+int exl3_fp4_dequant(const void* q, const void* s, int64_t s_stage, int M, int k, void* out, int out_dtype, void* stream);
+/* out[m][n] = sum over k of q[m][k] w[n][k], each times its block's scale, + bias[n], fp32 sums, rounded once to out_dtype. q, s
+ * as above; w, sw: the weights' rows [n, k] in the same form, their stages n * 8 bytes apart; bias: fp32 [n] or NULL; k <= 2^22, n
+ * <= 2^27. No state between calls, no workspace. */
+int exl3_fp4_matmul(const void* q, const void* s, int64_t s_stage, int M, int k, int n, const void* w, const void* sw,
+                    const float* bias, void* out, int out_dtype, int64_t out_stride, void* stream);
+/* the same of x [M, k], quantised within the call; its workspace (whose size never falls as M grows) starts on 16 bytes and is
+ * not shared by calls that run at the same time */
+size_t exl3_fp4_linear_workspace(int M, int k, int n);
+int exl3_fp4_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const void* sw,
+                    const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
+                    size_t workspace_bytes, void* stream);
+/* A gated MLP of quantised rows: silu(gate) * up of their product with gate|up weights, which stays in fp32 until it is quantised,
+ * multiplied with the down weights. Ip = I rounded up to 128. gu: [2 Ip, k] in the form above with its rows in another order: for
+ * each 32 of the I gates, those 32 rows and then their 32 ups (zeros for rows behind I); gu_scale and gu_bias (fp32 [2 Ip] or
+ * NULL) in the same order. dn: [n, I]; dn_bias fp32 [n] or NULL. The workspace as exl3_fp4_linear's. */
+size_t exl3_fp4_mlp_matmul_workspace(int M, int I);
+int exl3_fp4_mlp_matmul(const void* q, const void* s, int64_t s_stage, int M, int k, int I, int n, const void* gu,
+                        const void* gu_scale, const float* gu_bias, const void* dn, const void* dn_scale, const float* dn_bias,
+                        void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+/* the same of x [M, k], quantised within the call */
+size_t exl3_fp4_mlp_workspace(int M, int k, int I);
+int exl3_fp4_mlp(const void* x, int x_dtype, int64_t x_stride, int M, int k, int I, int n, const void* gu, const void* gu_scale,
+                 const float* gu_bias, const void* dn, const void* dn_scale, const float* dn_bias, void* out, int out_dtype,
+                 int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -296,4 +296,50 @@ constexpr int kCus = 256;
 bool fp8_product_quantises(int M, int k, int n);
 hipError_t launch_fp8_product(const Fp8ProductArgs& a, int out_dt, hipStream_t st);
 
+// The 4-bit float linear (fp4_rows.cuh has the rows' form): scales per 32 columns, in stages of 256 columns
+constexpr int kFp4Stage = 256;
+__host__ __device__ static inline int fp4_cols(int k) { return fp8_blocks(k) * 128; }
+__host__ __device__ static inline int fp4_stages(int k) { return k / kFp4Stage + (k % kFp4Stage != 0); }
+// fp4_rows.hip. silu: x holds gate|up rows of 2 k values and the rows written are silu(gate) * up
+struct Fp4RowsArgs {
+    const void* x; int64_t x_stride;
+    int M, k;
+    uint8_t* q; uint8_t* s;                        // [M, fp4_cols(k) / 2], [fp4_stages(k)] stages of [M, 8]
+    int64_t s_stage;                               // bytes from one stage to the next
+};
+hipError_t launch_fp4_rows(const Fp4RowsArgs& a, int x_dt, bool silu, hipStream_t st);
+struct Fp4DequantArgs {
+    const uint8_t* q; const uint8_t* s; int64_t s_stage;
+    int M, k;
+    void* out;                                     // [M, k]
+};
+hipError_t launch_fp4_dequant(const Fp4DequantArgs& a, int dt, hipStream_t st);
+// fp4_linear.hip: out[m][n] = sum_k q[m][k] w[n][k], each times its block's scale, + bias[n]
+struct Fp4ProductArgs {
+    const uint8_t* q; const uint8_t* s; int64_t s_stage;
+    const uint8_t* w; const uint8_t* sw;           // [n, fp4_cols(k) / 2], [kb] stages of [n, 8]
+    const float* bias;                             // [n] or null
+    int M, n, kp, kb;                              // kp = fp4_cols(k), kb = fp4_stages(k)
+    void* out; int64_t out_stride;
+    uint8_t* hq; uint8_t* hs;                      // launch_fp4_gate_up: its rows [M, n / 4], stages of [M, 8] next to each other
+};
+hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t st);
+// silu(gate) * up as 4-bit rows. The weights' rows are 32 gates and their 32 ups by turns, n a multiple of 256
+hipError_t launch_fp4_gate_up(const Fp4ProductArgs& a, hipStream_t st);
+
+// rms_norm.hip. Row m of x starts at (m / inner) x_outer + (m % inner) x_stride
+enum { kFormNone, kFormFp8, kFormFp4 };
+struct RmsNormArgs {
+    const void* x; int64_t x_stride, x_outer; int inner;
+    const void* res; int64_t res_stride; void* held;   // null: no residual; held [M, k] of its type
+    const float* w;                                // [k] or null
+    float eps;
+    int M, k;
+    void* y;                                       // [M, k] of x's type, or null
+    int form; uint8_t* q; void* s; int64_t s_stage;    // rows as Fp8RowsArgs or Fp4RowsArgs has them
+};
+// threads that hold a row
+static inline int rms_norm_threads(int k) { return k <= 256 ? 16 : k <= 2048 ? 64 : k <= 8192 ? 256 : 1024; }
+hipError_t launch_rms_norm(const RmsNormArgs& a, int x_dt, int res_dt, hipStream_t st);
+
 }  // namespace exl3

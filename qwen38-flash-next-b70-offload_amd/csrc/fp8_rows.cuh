@@ -104,6 +104,34 @@ __device__ __forceinline__ void load8(const void* x, size_t at, int n, float (&v
     }
 }
 
+// 8 consecutive elements of a row as DT. WIDE as above; else the first `n` of them one by one
+template <int DT, bool WIDE>
+__device__ __forceinline__ void store8(void* y, size_t at, int n, const float (&v)[8]) {
+    if constexpr (DT == 2) {
+        float* p = (float*)y + at;
+        if constexpr (WIDE) {
+            ((float4*)p)[0] = {v[0], v[1], v[2], v[3]};
+            ((float4*)p)[1] = {v[4], v[5], v[6], v[7]};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) p[j] = v[j];
+        }
+    } else {
+        uint16_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = DT == 0 ? __builtin_bit_cast(uint16_t, (_Float16)v[j]) : __builtin_bit_cast(uint16_t, (__bf16)v[j]);
+        uint16_t* p = (uint16_t*)y + at;
+        if constexpr (WIDE) {
+            *(uint4*)p = {u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16, u[6] | (uint32_t)u[7] << 16};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) p[j] = u[j];
+        }
+    }
+}
+
 // the largest over the 16 lanes of a DPP row, in every one of them (row_ror 8, 4, 2, 1)
 template <int CTRL>
 __device__ __forceinline__ uint32_t ror_max(uint32_t v) {

@@ -1460,4 +1460,260 @@ int exl3_fp8_mlp(const void* x, int dtype, int64_t x_stride, int M, int k, int I
                             out, dtype, out_stride, rest, stream);
 }
 
+// ---- the norm, and the 4-bit float linear ----------------------------------------------------------------------------
+
+namespace {
+
+int fp4_dims(const char* what, int M, int k, int n) {
+    if (M < 0 || k <= 0 || n <= 0) return fail(EXL3_EINVAL, "%s: M=%d k=%d n=%d", what, M, k, n);
+    // (a tile's 256 rows of k are one buffer of less than 2^32 bytes)
+    if (k > 1 << 22 || n > 1 << 27) return fail(EXL3_EUNSUPPORTED, "%s: k=%d above 2^22 or n=%d above 2^27", what, k, n);
+    return EXL3_OK;
+}
+
+// quantised rows: codes on 16 bytes, scales on 8, a stage's scales behind the one before
+int fp4_rows_checks(const char* what, const void* q, const void* s, int64_t s_stage, int M) {
+    if (!q || !s) return fail(EXL3_EINVAL, "%s: null pointer", what);
+    if (!aligned(q, 16) || !aligned(s, 8)) return fail(EXL3_EINVAL, "%s: alignment of q or s", what);
+    if (s_stage < (int64_t)M * 8 || s_stage % 8) return fail(EXL3_EINVAL, "%s: s_stage %lld", what, (long long)s_stage);
+    return EXL3_OK;
+}
+
+int fp4_launch_checks(const char* what, int M, int k) {
+    if (((int64_t)M + 7) / 8 * fp4_stages(k) * 256 >= kMaxThreads)
+        return fail(EXL3_EUNSUPPORTED, "%s: M=%d rows of k=%d exceed one launch", what, M, k);
+    return EXL3_OK;
+}
+
+int fp4_rows(const char* what, const void* x, int x_dtype, int64_t x_stride, int M, int k, bool silu, void* q, void* s,
+             int64_t s_stage, void* stream) {
+    if (int r = fp4_dims(what, M, k, 1)) return r;
+    if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "%s: dtype %d", what, x_dtype);
+    if (M == 0) return EXL3_OK;
+    if (!x || !aligned(x, dt_size(x_dtype))) return fail(EXL3_EINVAL, "%s: x null or its alignment", what);
+    if (x_stride < (silu ? 2 : 1) * (int64_t)k) return fail(EXL3_EINVAL, "%s: row stride %lld", what, (long long)x_stride);
+    if (int r = fp4_rows_checks(what, q, s, s_stage, M)) return r;
+    if (int r = fp4_launch_checks(what, M, k)) return r;
+    Fp4RowsArgs a{};
+    a.x = x;
+    a.x_stride = x_stride;
+    a.M = M;
+    a.k = k;
+    a.q = (uint8_t*)q;
+    a.s = (uint8_t*)s;
+    a.s_stage = s_stage;
+    const hipError_t e = launch_fp4_rows(a, x_dtype, silu, (hipStream_t)stream);
+    return e == hipSuccess ? EXL3_OK : hip_fail(e, what);
+}
+
+int fp4_product_checks(const char* what, int M, int k, int n, const void* w, const void* sw, const float* bias) {
+    if (int r = fp4_dims(what, M, k, n)) return r;
+    if (M == 0) return EXL3_OK;
+    if (!w || !sw) return fail(EXL3_EINVAL, "%s: null pointer", what);
+    if (!aligned(w, 16) || !aligned(sw, 8) || !aligned(bias, 4)) return fail(EXL3_EINVAL, "%s: alignment", what);
+    if ((M + (int64_t)255) * (n + (int64_t)255) / 64 >= kMaxThreads)
+        return fail(EXL3_EUNSUPPORTED, "%s: M=%d n=%d exceed one launch", what, M, n);
+    return EXL3_OK;
+}
+
+int fp4_out_checks(const char* what, int M, int n, const void* out, int out_dtype, int64_t out_stride) {
+    if (!dt_ok(out_dtype)) return fail(EXL3_EINVAL, "%s: out dtype %d", what, out_dtype);
+    if (M == 0) return EXL3_OK;
+    if (!out || out_stride < n || !aligned(out, dt_size(out_dtype)))
+        return fail(EXL3_EINVAL, "%s: out null, its alignment or row stride %lld", what, (long long)out_stride);
+    return EXL3_OK;
+}
+
+size_t fp4_q_bytes(int M, int k) { return align256((size_t)M * fp4_cols(k) / 2); }
+size_t fp4_s_bytes(int M, int k) { return align256((size_t)M * fp4_stages(k) * 8); }
+size_t fp4_rows_bytes(int M, int k) { return fp4_q_bytes(M, k) + fp4_s_bytes(M, k); }
+
+Fp4ProductArgs fp4_args(const void* q, const void* s, int64_t s_stage, int M, int k, int n, const void* w, const void* sw,
+                        const float* bias) {
+    Fp4ProductArgs a{};
+    a.q = (const uint8_t*)q;
+    a.s = (const uint8_t*)s;
+    a.s_stage = s_stage;
+    a.w = (const uint8_t*)w;
+    a.sw = (const uint8_t*)sw;
+    a.bias = bias;
+    a.M = M;
+    a.n = n;
+    a.kp = fp4_cols(k);
+    a.kb = fp4_stages(k);
+    return a;
+}
+
+int fp4_product(const char* what, Fp4ProductArgs a, void* out, int out_dtype, int64_t out_stride, void* stream) {
+    a.out = out;
+    a.out_stride = out_stride;
+    const hipError_t e = launch_fp4_product(a, out_dtype, (hipStream_t)stream);
+    return e == hipSuccess ? EXL3_OK : hip_fail(e, what);
+}
+
+// up(silu(gate) * up) of quantised rows, the rows between in `workspace`; arguments checked, M > 0
+int fp4_mlp_products(const char* what, const void* q, const void* s, int64_t s_stage, int M, int k, int I, int n, const void* gu,
+                     const void* gu_scale, const float* gu_bias, const void* dn, const void* dn_scale, const float* dn_bias,
+                     void* out, int out_dtype, int64_t out_stride, void* workspace, void* stream) {
+    Fp4ProductArgs a = fp4_args(q, s, s_stage, M, k, 2 * fp4_cols(I), gu, gu_scale, gu_bias);
+    a.hq = (uint8_t*)workspace;
+    a.hs = a.hq + fp4_q_bytes(M, I);
+    const hipError_t e = launch_fp4_gate_up(a, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, what);
+    return fp4_product(what, fp4_args(a.hq, a.hs, (int64_t)M * 8, M, I, n, dn, dn_scale, dn_bias), out, out_dtype, out_stride,
+                       stream);
+}
+
+int fp4_mlp_checks(const char* what, int M, int k, int I, int n, const void* gu, const void* gu_scale, const float* gu_bias,
+                   const void* dn, const void* dn_scale, const float* dn_bias, const void* out, int out_dtype,
+                   int64_t out_stride, const void* workspace, size_t workspace_bytes, size_t need) {
+    if (I <= 0 || I > 1 << 22) return fail(EXL3_EINVAL, "%s: I=%d", what, I);
+    if (int r = fp4_product_checks(what, M, k, 2 * fp4_cols(I), gu, gu_scale, gu_bias)) return r;
+    if (int r = fp4_product_checks(what, M, I, n, dn, dn_scale, dn_bias)) return r;
+    if (int r = fp4_out_checks(what, M, n, out, out_dtype, out_stride)) return r;
+    if (M > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return fail(EXL3_EWORKSPACE, "%s: workspace of %zu bytes on 16, got %zu", what, need, workspace_bytes);
+    return EXL3_OK;
+}
+
+}  // namespace
+
+int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64_t x_outer, const void* residual,
+                  int residual_dtype, int64_t residual_stride, void* held, const float* weight, float eps, int M, int k,
+                  void* y, int form, void* q, void* s, int64_t s_stage, void* stream) {
+    const char* what = "rms_norm";
+    if (int r = fp4_dims(what, M, k, 1)) return r;
+    if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "%s: dtype %d", what, x_dtype);
+    if (!(eps >= 0x1p-126f) || !(eps <= 3.0e38f)) return fail(EXL3_EINVAL, "%s: eps %g (positive and finite)", what, (double)eps);
+    if (form < kFormNone || form > kFormFp4) return fail(EXL3_EINVAL, "%s: form %d (0 none, 1 e4m3, 2 e2m1)", what, form);
+    if (residual && residual_dtype != x_dtype && residual_dtype != EXL3_DT_F32)
+        return fail(EXL3_EINVAL, "%s: residual dtype %d (x's or fp32)", what, residual_dtype);
+    if (inner < 1) return fail(EXL3_EINVAL, "%s: inner %d", what, inner);
+    if (M == 0) return EXL3_OK;
+    if (!x || x_stride < 0 || x_outer < 0 || !aligned(x, dt_size(x_dtype)))
+        return fail(EXL3_EINVAL, "%s: x null, its alignment or strides", what);
+    if (!residual != !held) return fail(EXL3_EINVAL, "%s: residual and held come together", what);
+    if (residual && (residual_stride < k || !aligned(residual, dt_size(residual_dtype)) || !aligned(held, dt_size(residual_dtype))))
+        return fail(EXL3_EINVAL, "%s: alignment of residual or held, or row stride %lld", what, (long long)residual_stride);
+    if (!aligned(weight, 4) || !aligned(y, dt_size(x_dtype))) return fail(EXL3_EINVAL, "%s: alignment", what);
+    if (!y && form == kFormNone) return fail(EXL3_EINVAL, "%s: no output", what);
+    if (form == kFormFp8 && (!q || !s || !aligned(q, 16) || !aligned(s, 4)))
+        return fail(EXL3_EINVAL, "%s: q or s null or not aligned", what);
+    if (form == kFormFp4)
+        if (int r = fp4_rows_checks(what, q, s, s_stage, M)) return r;
+    if ((M + (int64_t)15) * rms_norm_threads(k) >= kMaxThreads)
+        return fail(EXL3_EUNSUPPORTED, "%s: M=%d rows of k=%d exceed one launch", what, M, k);
+    RmsNormArgs a{};
+    a.x = x;
+    a.x_stride = x_stride;
+    a.x_outer = inner == 1 ? x_stride : x_outer;
+    a.inner = inner;
+    a.res = residual;
+    a.res_stride = residual_stride;
+    a.held = held;
+    a.w = weight;
+    a.eps = eps;
+    a.M = M;
+    a.k = k;
+    a.y = y;
+    a.form = form;
+    a.q = (uint8_t*)q;
+    a.s = s;
+    a.s_stage = s_stage;
+    const hipError_t e = launch_rms_norm(a, x_dtype, residual_dtype, (hipStream_t)stream);
+    return e == hipSuccess ? EXL3_OK : hip_fail(e, what);
+}
+
+int exl3_fp4_quant(const void* x, int x_dtype, int64_t x_stride, int M, int k, void* q, void* s, int64_t s_stage, void* stream) {
+    return fp4_rows("fp4_quant", x, x_dtype, x_stride, M, k, false, q, s, s_stage, stream);
+}
+
+int exl3_fp4_silu_mul_quant(const void* gate_up, int dtype, int64_t stride, int M, int k, void* q, void* s, int64_t s_stage,
+                            void* stream) {
+    return fp4_rows("fp4_silu_mul_quant", gate_up, dtype, stride, M, k, true, q, s, s_stage, stream);
+}
+
+int exl3_fp4_dequant(const void* q, const void* s, int64_t s_stage, int M, int k, void* out, int out_dtype, void* stream) {
+    if (int r = fp4_dims("fp4_dequant", M, k, 1)) return r;
+    if (int r = fp4_out_checks("fp4_dequant", M, k, out, out_dtype, k)) return r;
+    if (M == 0) return EXL3_OK;
+    if (int r = fp4_rows_checks("fp4_dequant", q, s, s_stage, M)) return r;
+    if (int r = fp4_launch_checks("fp4_dequant", M, k)) return r;
+    Fp4DequantArgs a{};
+    a.q = (const uint8_t*)q;
+    a.s = (const uint8_t*)s;
+    a.s_stage = s_stage;
+    a.M = M;
+    a.k = k;
+    a.out = out;
+    const hipError_t e = launch_fp4_dequant(a, out_dtype, (hipStream_t)stream);
+    return e == hipSuccess ? EXL3_OK : hip_fail(e, "fp4_dequant launch");
+}
+
+int exl3_fp4_matmul(const void* q, const void* s, int64_t s_stage, int M, int k, int n, const void* w, const void* sw,
+                    const float* bias, void* out, int out_dtype, int64_t out_stride, void* stream) {
+    if (int r = fp4_product_checks("fp4_matmul", M, k, n, w, sw, bias)) return r;
+    if (int r = fp4_out_checks("fp4_matmul", M, n, out, out_dtype, out_stride)) return r;
+    if (M == 0) return EXL3_OK;
+    if (int r = fp4_rows_checks("fp4_matmul", q, s, s_stage, M)) return r;
+    return fp4_product("fp4_matmul", fp4_args(q, s, s_stage, M, k, n, w, sw, bias), out, out_dtype, out_stride, stream);
+}
+
+size_t exl3_fp4_linear_workspace(int M, int k, int n) {
+    if (M <= 0 || k <= 0 || n <= 0) return 0;
+    return fp4_rows_bytes(M, k);
+}
+
+int exl3_fp4_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const void* sw,
+                    const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+    const char* what = "fp4_linear";
+    if (int r = fp4_product_checks(what, M, k, n, w, sw, bias)) return r;
+    if (int r = fp4_out_checks(what, M, n, out, out_dtype, out_stride)) return r;
+    if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "%s: x dtype %d", what, x_dtype);
+    if (M == 0) return EXL3_OK;
+    const size_t need = exl3_fp4_linear_workspace(M, k, n);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(EXL3_EWORKSPACE, "%s: workspace of %zu bytes on 16, got %zu", what, need, workspace_bytes);
+    uint8_t *q = (uint8_t*)workspace, *s = q + fp4_q_bytes(M, k);
+    if (int r = fp4_rows(what, x, x_dtype, x_stride, M, k, false, q, s, (int64_t)M * 8, stream)) return r;
+    return fp4_product(what, fp4_args(q, s, (int64_t)M * 8, M, k, n, w, sw, bias), out, out_dtype, out_stride, stream);
+}
+
+// the rows between the two products
+size_t exl3_fp4_mlp_matmul_workspace(int M, int I) { return M <= 0 || I <= 0 || I > 1 << 22 ? 0 : fp4_rows_bytes(M, I); }
+
+int exl3_fp4_mlp_matmul(const void* q, const void* s, int64_t s_stage, int M, int k, int I, int n, const void* gu,
+                        const void* gu_scale, const float* gu_bias, const void* dn, const void* dn_scale, const float* dn_bias,
+                        void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "fp4_mlp_matmul";
+    if (int r = fp4_mlp_checks(what, M, k, I, n, gu, gu_scale, gu_bias, dn, dn_scale, dn_bias, out, out_dtype, out_stride,
+                               workspace, workspace_bytes, exl3_fp4_mlp_matmul_workspace(M, I)))
+        return r;
+    if (M == 0) return EXL3_OK;
+    if (int r = fp4_rows_checks(what, q, s, s_stage, M)) return r;
+    return fp4_mlp_products(what, q, s, s_stage, M, k, I, n, gu, gu_scale, gu_bias, dn, dn_scale, dn_bias, out, out_dtype,
+                            out_stride, workspace, stream);
+}
+
+size_t exl3_fp4_mlp_workspace(int M, int k, int I) {
+    if (M <= 0 || k <= 0 || I <= 0 || I > 1 << 22) return 0;
+    return fp4_rows_bytes(M, k) + exl3_fp4_mlp_matmul_workspace(M, I);
+}
+
+int exl3_fp4_mlp(const void* x, int x_dtype, int64_t x_stride, int M, int k, int I, int n, const void* gu, const void* gu_scale,
+                 const float* gu_bias, const void* dn, const void* dn_scale, const float* dn_bias, void* out, int out_dtype,
+                 int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "fp4_mlp";
+    if (int r = fp4_mlp_checks(what, M, k, I, n, gu, gu_scale, gu_bias, dn, dn_scale, dn_bias, out, out_dtype, out_stride,
+                               workspace, workspace_bytes, exl3_fp4_mlp_workspace(M, k, I)))
+        return r;
+    if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "%s: x dtype %d", what, x_dtype);
+    if (M == 0) return EXL3_OK;
+    uint8_t *q = (uint8_t*)workspace, *s = q + fp4_q_bytes(M, k);
+    if (int r = fp4_rows(what, x, x_dtype, x_stride, M, k, false, q, s, (int64_t)M * 8, stream)) return r;
+    return fp4_mlp_products(what, q, s, (int64_t)M * 8, M, k, I, n, gu, gu_scale, gu_bias, dn, dn_scale, dn_bias, out, out_dtype,
+                            out_stride, q + fp4_rows_bytes(M, k), stream);
+}
+
 }  // extern "C"

@@ -646,6 +646,275 @@ at::Tensor fp8_matmul_meta(const at::Tensor& q, const at::Tensor&, const at::Ten
     return at::empty(with_last(q.sizes(), w.size(0)), q.options().dtype(dtype));
 }
 
+// ---- the norm and the 4-bit float linear of exl3xpu_C (no counterpart in the reference) ---------------------------------
+
+void no_gradients(const at::Tensor& x, const char* what) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), what,
+                ": no gradients; detach the input or call it under torch.no_grad()");
+}
+
+int64_t fp4_stages(int64_t k) { return (k + 255) / 256; }
+
+// quantised rows of x's leading sizes and k columns: codes [..., kp / 2] and scales [..., stages, 8], the stages outermost in memory
+std::tuple<at::Tensor, at::Tensor> fp4_rows_empty(const at::Tensor& x, int64_t k) {
+    auto sizes = with_last(x.sizes(), 8);
+    sizes.insert(sizes.begin(), fp4_stages(k));
+    const auto o = x.options().dtype(at::kByte);
+    return {at::empty(with_last(x.sizes(), fp8_up(k) / 2), o), at::empty(sizes, o).movedim(0, -2)};
+}
+
+// Quantised rows as the C-ABI takes them (copies only where the strides or addresses do not fit)
+struct Fp4Rows {
+    at::Tensor q, s;                                 // s with the stages first
+    int M = 0, kp = 0;
+    int64_t s_stage = 0;
+    Fp4Rows(const at::Tensor& q_, const at::Tensor& s_, const char* what) {
+        TORCH_CHECK(q_.scalar_type() == at::kByte && q_.dim() >= 1 && q_.size(-1) > 0 && q_.size(-1) % 64 == 0 &&
+                        q_.size(-1) <= INT32_MAX / 2 && q_.numel() / q_.size(-1) <= INT32_MAX,
+                    what, ": q uint8 [..., a multiple of 64], got ", q_.scalar_type(), " ", q_.sizes());
+        on_device_of(q_, s_, what);
+        kp = (int)(2 * q_.size(-1));
+        M = (int)(q_.numel() / q_.size(-1));
+        auto want = with_last(q_.sizes(), fp4_stages(kp));
+        want.push_back(8);
+        TORCH_CHECK(s_.scalar_type() == at::kByte && s_.sizes().vec() == want, what, ": s uint8 ", want, ", got ",
+                    s_.scalar_type(), " ", s_.sizes());
+        q = q_.contiguous();
+        if ((uintptr_t)q.const_data_ptr() % 16) q = q.clone();
+        s = s_.movedim(-2, 0);
+        const auto rows = s.select(0, 0);
+        if (!rows.is_contiguous() || (s.size(0) > 1 && (s.stride(0) < 8 * (int64_t)M || s.stride(0) % 8))) s = s.contiguous();
+        if ((uintptr_t)s.const_data_ptr() % 8) s = s.clone(at::MemoryFormat::Contiguous);
+        s_stage = s.size(0) > 1 ? s.stride(0) : 8 * (int64_t)M;
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor> fp4_quant_meta(const at::Tensor& x) { return fp4_rows_empty(x, x.size(-1)); }
+std::tuple<at::Tensor, at::Tensor> fp4_silu_mul_quant_meta(const at::Tensor& x) { return fp4_rows_empty(x, x.size(-1) / 2); }
+
+std::tuple<at::Tensor, at::Tensor> fp4_quant(const at::Tensor& x) {
+    const c10::DeviceGuard guard(x.device());
+    no_gradients(x, "fp4_quant");
+    const int dt = dtype_code(x);
+    auto x2 = rows_of(x, "fp4_quant");
+    auto out = fp4_rows_empty(x, x.size(-1));
+    check(exl3_fp4_quant(x2.data_ptr(), dt, row_stride(x2), (int)x2.size(0), (int)x2.size(1), std::get<0>(out).data_ptr(),
+                         std::get<1>(out).data_ptr(), 8 * x2.size(0), cur_stream(x)),
+          "fp4_quant");
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> fp4_silu_mul_quant(const at::Tensor& x) {
+    const c10::DeviceGuard guard(x.device());
+    no_gradients(x, "fp4_silu_mul_quant");
+    const int dt = dtype_code(x);
+    auto x2 = rows_of(x, "fp4_silu_mul_quant");
+    TORCH_CHECK(x2.size(1) % 2 == 0, "fp4_silu_mul_quant: gate|up rows of an even size, got ", x.sizes());
+    const int64_t k = x2.size(1) / 2;
+    auto out = fp4_rows_empty(x, k);
+    check(exl3_fp4_silu_mul_quant(x2.data_ptr(), dt, row_stride(x2), (int)x2.size(0), (int)k, std::get<0>(out).data_ptr(),
+                                  std::get<1>(out).data_ptr(), 8 * x2.size(0), cur_stream(x)),
+          "fp4_silu_mul_quant");
+    return out;
+}
+
+at::Tensor fp4_dequant_meta(const at::Tensor& q, const at::Tensor&, int64_t k, at::ScalarType dtype) {
+    return at::empty(with_last(q.sizes(), k), q.options().dtype(dtype));
+}
+
+at::Tensor fp4_dequant(const at::Tensor& q, const at::Tensor& s, int64_t k, at::ScalarType dtype) {
+    const c10::DeviceGuard guard(q.device());
+    const Fp4Rows r(q, s, "fp4_dequant");
+    TORCH_CHECK(k > 0 && fp8_up(k) == r.kp, "fp4_dequant: rows of ", r.kp, " columns do not hold k=", k);
+    auto out = fp4_dequant_meta(q, s, k, dtype);
+    check(exl3_fp4_dequant(r.q.const_data_ptr(), r.s.const_data_ptr(), r.s_stage, r.M, (int)k, out.data_ptr(), dtype_code(out),
+                           cur_stream(q)),
+          "fp4_dequant");
+    return out;
+}
+
+// weights [n, k] in the rows' form, laid out as the product takes them
+void fp4_weight_checks(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sw, int64_t k, const char* what) {
+    on_device_of(x, w, what);
+    on_device_of(x, sw, what);
+    TORCH_CHECK(w.scalar_type() == at::kByte && w.dim() == 2 && w.is_contiguous() && w.size(1) == fp8_up(k) / 2 && w.size(0) > 0 &&
+                    w.size(0) <= INT32_MAX,
+                what, ": weight uint8 [n, ", fp8_up(k) / 2, "] contiguous, got ", w.scalar_type(), " ", w.sizes());
+    TORCH_CHECK(sw.scalar_type() == at::kByte && sw.dim() == 3 && sw.size(0) == w.size(0) && sw.size(1) == fp4_stages(k) &&
+                    sw.size(2) == 8 && sw.movedim(1, 0).is_contiguous(),
+                what, ": weight_scale uint8 [", w.size(0), ", ", fp4_stages(k), ", 8] with the stages outermost in memory, got ",
+                sw.scalar_type(), " ", sw.sizes());
+}
+
+at::Tensor fp4_linear_meta(const at::Tensor& x, const at::Tensor& w, const at::Tensor&, const std::optional<at::Tensor>&) {
+    return at::empty(with_last(x.sizes(), w.size(0)), x.options());
+}
+
+at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sw, const std::optional<at::Tensor>& bias) {
+    const c10::DeviceGuard guard(x.device());
+    no_gradients(x, "fp4_linear");
+    const int dt = dtype_code(x);
+    auto x2 = rows_of(x, "fp4_linear");
+    const int M = (int)x2.size(0), k = (int)x2.size(1);
+    fp4_weight_checks(x, w, sw, k, "fp4_linear");
+    const int64_t n = w.size(0);
+    const float* b = f32_or_null(bias, x, n, "fp4_linear");
+    auto out = fp4_linear_meta(x, w, sw, bias);
+    if (M == 0) return out;
+    const size_t ws = exl3_fp4_linear_workspace(M, k, (int)n);
+    auto buf = at::empty({(int64_t)ws}, x.options().dtype(at::kByte));
+    check(exl3_fp4_linear(x2.data_ptr(), dt, row_stride(x2), M, k, (int)n, w.const_data_ptr(), sw.const_data_ptr(), b,
+                          out.data_ptr(), dt, n, buf.data_ptr(), ws, cur_stream(x)),
+          "fp4_linear");
+    return out;
+}
+
+at::Tensor fp4_matmul_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor& w, const at::Tensor&,
+                           const std::optional<at::Tensor>&, at::ScalarType dtype) {
+    return at::empty(with_last(q.sizes(), w.size(0)), q.options().dtype(dtype));
+}
+
+at::Tensor fp4_matmul(const at::Tensor& q, const at::Tensor& s, const at::Tensor& w, const at::Tensor& sw,
+                      const std::optional<at::Tensor>& bias, at::ScalarType dtype) {
+    const c10::DeviceGuard guard(q.device());
+    const Fp4Rows r(q, s, "fp4_matmul");
+    fp4_weight_checks(q, w, sw, r.kp, "fp4_matmul");
+    const int64_t n = w.size(0);
+    const float* b = f32_or_null(bias, q, n, "fp4_matmul");
+    auto out = fp4_matmul_meta(q, s, w, sw, bias, dtype);
+    check(exl3_fp4_matmul(r.q.const_data_ptr(), r.s.const_data_ptr(), r.s_stage, r.M, r.kp, (int)n, w.const_data_ptr(),
+                          sw.const_data_ptr(), b, out.data_ptr(), dtype_code(out), n, cur_stream(q)),
+          "fp4_matmul");
+    return out;
+}
+
+struct Fp4MlpSizes {
+    int64_t I, n;
+    const float *gb, *db;
+    Fp4MlpSizes(const at::Tensor& x, int64_t k, int64_t I_, const at::Tensor& gu, const at::Tensor& gu_scale,
+                const std::optional<at::Tensor>& gu_bias, const at::Tensor& dn, const at::Tensor& dn_scale,
+                const std::optional<at::Tensor>& dn_bias, const char* what)
+        : I(I_), n(dn.size(0)) {
+        TORCH_CHECK(I > 0 && I <= (1 << 22), what, ": intermediate size ", I);
+        fp4_weight_checks(x, gu, gu_scale, k, what);
+        TORCH_CHECK(gu.size(0) == 2 * fp8_up(I), what, ": gate|up weights of ", 2 * fp8_up(I), " rows, got ", gu.sizes());
+        fp4_weight_checks(x, dn, dn_scale, I, what);
+        gb = f32_or_null(gu_bias, x, 2 * fp8_up(I), what);
+        db = f32_or_null(dn_bias, x, n, what);
+    }
+};
+
+at::Tensor fp4_mlp(const at::Tensor& x, int64_t I, const at::Tensor& gu, const at::Tensor& gu_scale,
+                   const std::optional<at::Tensor>& gu_bias, const at::Tensor& dn, const at::Tensor& dn_scale,
+                   const std::optional<at::Tensor>& dn_bias) {
+    const c10::DeviceGuard guard(x.device());
+    no_gradients(x, "fp4_mlp");
+    const int dt = dtype_code(x);
+    auto x2 = rows_of(x, "fp4_mlp");
+    const int M = (int)x2.size(0), k = (int)x2.size(1);
+    const Fp4MlpSizes z(x, k, I, gu, gu_scale, gu_bias, dn, dn_scale, dn_bias, "fp4_mlp");
+    auto out = at::empty(with_last(x.sizes(), z.n), x.options());
+    if (M == 0) return out;
+    const size_t ws = exl3_fp4_mlp_workspace(M, k, (int)I);
+    auto buf = at::empty({(int64_t)ws}, x.options().dtype(at::kByte));
+    check(exl3_fp4_mlp(x2.data_ptr(), dt, row_stride(x2), M, k, (int)I, (int)z.n, gu.const_data_ptr(), gu_scale.const_data_ptr(),
+                       z.gb, dn.const_data_ptr(), dn_scale.const_data_ptr(), z.db, out.data_ptr(), dt, z.n, buf.data_ptr(), ws,
+                       cur_stream(x)),
+          "fp4_mlp");
+    return out;
+}
+
+at::Tensor fp4_mlp_meta(const at::Tensor& x, int64_t, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
+                        const at::Tensor& dn, const at::Tensor&, const std::optional<at::Tensor>&) {
+    return at::empty(with_last(x.sizes(), dn.size(0)), x.options());
+}
+
+at::Tensor fp4_mlp_matmul(const at::Tensor& q, const at::Tensor& s, int64_t I, const at::Tensor& gu, const at::Tensor& gu_scale,
+                          const std::optional<at::Tensor>& gu_bias, const at::Tensor& dn, const at::Tensor& dn_scale,
+                          const std::optional<at::Tensor>& dn_bias, at::ScalarType dtype) {
+    const c10::DeviceGuard guard(q.device());
+    const Fp4Rows r(q, s, "fp4_mlp_matmul");
+    const Fp4MlpSizes z(q, r.kp, I, gu, gu_scale, gu_bias, dn, dn_scale, dn_bias, "fp4_mlp_matmul");
+    auto out = at::empty(with_last(q.sizes(), z.n), q.options().dtype(dtype));
+    const int dt = dtype_code(out);
+    if (r.M == 0) return out;
+    const size_t ws = exl3_fp4_mlp_matmul_workspace(r.M, (int)I);
+    auto buf = at::empty({(int64_t)ws}, q.options());
+    check(exl3_fp4_mlp_matmul(r.q.const_data_ptr(), r.s.const_data_ptr(), r.s_stage, r.M, r.kp, (int)I, (int)z.n,
+                              gu.const_data_ptr(), gu_scale.const_data_ptr(), z.gb, dn.const_data_ptr(), dn_scale.const_data_ptr(),
+                              z.db, out.data_ptr(), dt, z.n, buf.data_ptr(), ws, cur_stream(q)),
+          "fp4_mlp_matmul");
+    return out;
+}
+
+at::Tensor fp4_mlp_matmul_meta(const at::Tensor& q, const at::Tensor&, int64_t, const at::Tensor&, const at::Tensor&,
+                               const std::optional<at::Tensor>&, const at::Tensor& dn, const at::Tensor&,
+                               const std::optional<at::Tensor>&, at::ScalarType dtype) {
+    return at::empty(with_last(q.sizes(), dn.size(0)), q.options().dtype(dtype));
+}
+
+// form 0, 1 or 2 as exl3_rms_norm's, `rows`: y too. The outputs there are, in the order q, s, y, held
+std::vector<at::Tensor> rms_norm_empty(const at::Tensor& x, const std::optional<at::Tensor>& residual, int64_t form, bool rows) {
+    TORCH_CHECK(form >= 0 && form <= 2 && (form || rows), "rms_norm: form ", form, " without rows");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "rms_norm: [..., k] with k > 0, got ", x.sizes());
+    std::vector<at::Tensor> out;
+    if (form) {
+        auto [q, s] = form == 1 ? fp8_rows_empty(x, x.size(-1)) : fp4_rows_empty(x, x.size(-1));
+        out.push_back(q);
+        out.push_back(s);
+    }
+    if (rows) out.push_back(at::empty(x.sizes(), x.options()));
+    if (residual) out.push_back(at::empty(x.sizes(), residual->options()));
+    return out;
+}
+
+std::vector<at::Tensor> rms_norm_meta(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                                      const std::optional<at::Tensor>&, double, int64_t form, bool rows) {
+    return rms_norm_empty(x, residual, form, rows);
+}
+
+std::vector<at::Tensor> rms_norm(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                                 const std::optional<at::Tensor>& weight, double eps, int64_t form, bool rows) {
+    const c10::DeviceGuard guard(x.device());
+    no_gradients(x, "rms_norm");
+    const int dt = dtype_code(x);
+    auto out = rms_norm_empty(x, residual, form, rows);
+    const int64_t k = x.size(-1);
+    const float* w = f32_or_null(weight, x, k, "rms_norm (weight)");
+    int rdt = dt;
+    at::Tensor r2;
+    if (residual) {
+        no_gradients(*residual, "rms_norm");
+        on_device_of(x, *residual, "rms_norm");
+        TORCH_CHECK(residual->sizes() == x.sizes(), "rms_norm: residual ", x.sizes(), ", got ", residual->sizes());
+        rdt = dtype_code(*residual);
+        TORCH_CHECK(rdt == dt || rdt == EXL3_DT_F32, "rms_norm: residual of x's dtype or fp32, got ", residual->scalar_type());
+        r2 = rows_of(*residual, "rms_norm");
+    }
+    // rows inside wider ones ([tokens, heads, k] cut out of a fused projection) as they are: a stride within and one between
+    at::Tensor x2;
+    int64_t inner = 1, stride = 0, outer = 0;
+    if (x.dim() == 3 && x.stride(2) == 1 && x.numel() > 0 && x.size(0) > 1 && x.size(1) > 1 && x.stride(1) >= k &&
+        x.stride(0) != x.size(1) * x.stride(1) && x.stride(0) >= 0 && x.size(1) <= INT32_MAX && x.numel() / k <= INT32_MAX) {
+        x2 = x;
+        inner = x.size(1);
+        stride = x.stride(1);
+        outer = x.stride(0);
+    } else {
+        x2 = rows_of(x, "rms_norm");
+        stride = row_stride(x2);
+    }
+    const int M = (int)(x.numel() / k);
+    auto ptr = [&](size_t i) { return out[i].data_ptr(); };
+    const size_t y = form ? 2 : 0, held = y + rows;
+    check(exl3_rms_norm(x2.const_data_ptr(), dt, stride, (int)inner, outer, residual ? r2.const_data_ptr() : nullptr, rdt,
+                        residual ? row_stride(r2) : 0, residual ? ptr(held) : nullptr, w, (float)eps, M, (int)k,
+                        rows ? ptr(y) : nullptr, (int)form, form ? ptr(0) : nullptr, form ? ptr(1) : nullptr, 8 * (int64_t)M,
+                        cur_stream(x)),
+          "rms_norm");
+    return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(exl3xpu_C, m) {
@@ -680,6 +949,32 @@ TORCH_LIBRARY(exl3xpu_C, m) {
     m.def("fp8_matmul(Tensor q, Tensor s, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType dtype) -> Tensor");
     m.impl("fp8_matmul", c10::DispatchKey::CUDA, &fp8_matmul);
     m.impl("fp8_matmul", c10::DispatchKey::Meta, &fp8_matmul_meta);
+    m.def("rms_norm(Tensor x, Tensor? residual, Tensor? weight, float eps, int form, bool rows) -> Tensor[]");
+    m.impl("rms_norm", c10::DispatchKey::CUDA, &rms_norm);
+    m.impl("rms_norm", c10::DispatchKey::Meta, &rms_norm_meta);
+    m.def("fp4_quant(Tensor x) -> (Tensor q, Tensor s)");
+    m.impl("fp4_quant", c10::DispatchKey::CUDA, &fp4_quant);
+    m.impl("fp4_quant", c10::DispatchKey::Meta, &fp4_quant_meta);
+    m.def("fp4_silu_mul_quant(Tensor gate_up) -> (Tensor q, Tensor s)");
+    m.impl("fp4_silu_mul_quant", c10::DispatchKey::CUDA, &fp4_silu_mul_quant);
+    m.impl("fp4_silu_mul_quant", c10::DispatchKey::Meta, &fp4_silu_mul_quant_meta);
+    m.def("fp4_dequant(Tensor q, Tensor s, int k, ScalarType dtype) -> Tensor");
+    m.impl("fp4_dequant", c10::DispatchKey::CUDA, &fp4_dequant);
+    m.impl("fp4_dequant", c10::DispatchKey::Meta, &fp4_dequant_meta);
+    m.def("fp4_linear(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias=None) -> Tensor");
+    m.impl("fp4_linear", c10::DispatchKey::CUDA, &fp4_linear);
+    m.impl("fp4_linear", c10::DispatchKey::Meta, &fp4_linear_meta);
+    m.def("fp4_matmul(Tensor q, Tensor s, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType dtype) -> Tensor");
+    m.impl("fp4_matmul", c10::DispatchKey::CUDA, &fp4_matmul);
+    m.impl("fp4_matmul", c10::DispatchKey::Meta, &fp4_matmul_meta);
+    m.def("fp4_mlp(Tensor x, int I, Tensor gate_up, Tensor gate_up_scale, Tensor? gate_up_bias, Tensor down, "
+          "Tensor down_scale, Tensor? down_bias) -> Tensor");
+    m.impl("fp4_mlp", c10::DispatchKey::CUDA, &fp4_mlp);
+    m.impl("fp4_mlp", c10::DispatchKey::Meta, &fp4_mlp_meta);
+    m.def("fp4_mlp_matmul(Tensor q, Tensor s, int I, Tensor gate_up, Tensor gate_up_scale, Tensor? gate_up_bias, Tensor down, "
+          "Tensor down_scale, Tensor? down_bias, ScalarType dtype) -> Tensor");
+    m.impl("fp4_mlp_matmul", c10::DispatchKey::CUDA, &fp4_mlp_matmul);
+    m.impl("fp4_mlp_matmul", c10::DispatchKey::Meta, &fp4_mlp_matmul_meta);
 }
 
 TORCH_LIBRARY(exl3xpu_moe, m) {

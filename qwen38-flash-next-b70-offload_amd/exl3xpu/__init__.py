@@ -5,6 +5,8 @@ nvtier       -- TierStore, NvTier / NvTierFast / NvTierAsync (RAM tier with admi
 routing      -- Router: logits to the picks and weights that the expert calls take
 linear       -- FusedGroup: the dense EXL3 linear
 fp8          -- Fp8Linear, Fp8Mlp: linears in 8-bit floats with a scale per 128 x 128 block
+fp4          -- Fp4Linear, Fp4Mlp: linears in microscaled 4-bit floats
+norm         -- RmsNorm: the norm before a layer's linears, with the residual's addition and quantised outputs
 capi         -- ctypes binding of the C-ABI library libexl3moe.so (include/exl3moe.h)
 synth        -- seeded synthetic experts and routing traces
 """
