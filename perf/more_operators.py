@@ -222,7 +222,8 @@ def run(st):
     kind, dt = c["kind"], x.dtype
     if own:
         if kind == "norm":
-            return st["norm"].quant(x, st["residual"]) if c["out"] == "fp8" else st["norm"](x, st["residual"])
+            out = st["norm"].quant(x, st["residual"]) if c["out"] == "fp8" else st["norm"](x, st["residual"])
+            return out if isinstance(out, tuple) else (out,)
         if kind == "quant":
             return st["fp4"].dequant(*st["fp4"].quant(x), dt, c["k"])
         if kind == "linear" and c["norm"]:
