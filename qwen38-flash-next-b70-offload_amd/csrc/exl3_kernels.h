@@ -322,9 +322,20 @@ struct Fp4ProductArgs {
     int M, n, kp, kb;                              // kp = fp4_cols(k), kb = fp4_stages(k)
     void* out; int64_t out_stride;
     uint8_t* hq; uint8_t* hs;                      // launch_fp4_gate_up: its rows [M, n / 4], stages of [M, 8] next to each other
+    // q null, few rows: quantised from rows [M, k] of type x_dt, or (silu) from fp32 rows of 32 gates and their 32 ups by turns
+    const void* x; int64_t x_stride; int k, x_dt;
+    bool silu, x_wide;                             // x_wide: every 4 columns start on 4 elements' bytes
 };
 hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t st);
-// silu(gate) * up as 4-bit rows. The weights' rows are 32 gates and their 32 ups by turns, n a multiple of 256
+// whether the product quantises its rows itself (no launch_fp4_rows before it)
+bool fp4_product_quantises(int M, int k, int n);
+static inline bool fp4_rows_wide(const void* x, int64_t x_stride, int k, int x_dt) {
+    const int size = x_dt == 2 ? 4 : 2;
+    return (uintptr_t)x % (4 * size) == 0 && x_stride % 4 == 0 && k % 4 == 0;
+}
+// silu(gate) * up as 4-bit rows, for rows enough (fewer: launch_fp4_product to fp32, and again of those rows). The weights' rows are
+// 32 gates and their 32 ups by turns, n a multiple of 256
+bool fp4_gate_up_in_tiles(int M);
 hipError_t launch_fp4_gate_up(const Fp4ProductArgs& a, hipStream_t st);
 
 // rms_norm.hip. Row m of x starts at (m / inner) x_outer + (m % inner) x_stride

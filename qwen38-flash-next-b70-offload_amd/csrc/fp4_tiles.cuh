@@ -17,12 +17,13 @@
 
 namespace exl3 {
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v2i __attribute__((ext_vector_type(2)));
 
 // 32 codes of a lane as an operand
 __device__ __forceinline__ v8i fp4_operand(v4i v) { return v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
 
 // The scales of a lane's four blocks of a stage (columns 64 j + 32 h) out of its row's eight, byte j for step j
-__device__ __forceinline__ int lane_scales(uint2 row, int h) {
+__device__ __forceinline__ int lane_scales(v2i row, int h) {
     return (int)__builtin_amdgcn_perm(row.y, row.x, h ? 0x07050301u : 0x06040200u);
 }
 
@@ -128,29 +129,51 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
     for (int b = 0; b < steps; ++b) {
         // stage b has arrived for every wave (later ones may be under way), and every wave has read stage b - 1
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * kLoads) : "memory");
+        auto more = [&](int i0, int i1) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(b + ST - 1, i);
-        if (KG > 1 && b * KG + kg >= A.kb) continue; // (the last step)
+            for (int i = i0; i < i1; ++i) load(b + ST - 1, i);
+        };
+        if (KG > 1 && b * KG + kg >= A.kb) {         // (the last step)
+            more(0, kLoads);
+            continue;
+        }
         const Fp4Stage<BM, BN>& st = lds.stage[kg][b % ST];
         // (columns behind kp, in the last stage, count for nothing whatever was loaded)
         const int keep = (b * KG + kg + 1) * kFp4Stage > A.kp ? 0xFFFF : -1;
+        v4i wf[2][TN], qf[2][TM];
+        auto read = [&](int j, int to) {
+            const int at = r * 128 + piece_at(r, j * 2 + h) * 16;
+#pragma unroll
+            for (int i = 0; i < TN; ++i) wf[to][i] = *(const v4i*)(st.w + (wn + i * 32) * 128 + at);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) qf[to][i] = *(const v4i*)(st.q + (wm + i * 32) * 128 + at);
+        };
         int sw[TN], sq[TM];
 #pragma unroll
-        for (int i = 0; i < TN; ++i) sw[i] = lane_scales(*(const uint2*)(st.sw + (wn + i * 32 + r) * 8), h) & keep;
+        for (int i = 0; i < TN; ++i) sw[i] = lane_scales(*(const v2i*)(st.sw + (wn + i * 32 + r) * 8), h) & keep;
 #pragma unroll
-        for (int j = 0; j < TM; ++j) sq[j] = lane_scales(*(const uint2*)(st.sq + (wm + j * 32 + r) * 8), h) & keep;
+        for (int j = 0; j < TM; ++j) sq[j] = lane_scales(*(const v2i*)(st.sq + (wm + j * 32 + r) * 8), h) & keep;
+        read(0, 0);
         four_steps([&](auto step) {
-            constexpr int J = decltype(step)::value;
-            const int at = r * 128 + piece_at(r, J * 2 + h) * 16;
-            v8i wf[TN], qf[TM];
-#pragma unroll
-            for (int i = 0; i < TN; ++i) wf[i] = fp4_operand(*(const v4i*)(st.w + (wn + i * 32) * 128 + at));
-#pragma unroll
-            for (int j = 0; j < TM; ++j) qf[j] = fp4_operand(*(const v4i*)(st.q + (wm + j * 32) * 128 + at));
+            // under a step's MFMAs the next one's fragments are read, and a part of a later stage's loads issued (behind the
+            // reads: the compiler keeps their order)
+            constexpr int J = decltype(step)::value, X = J & 1, kEach = (kLoads + 2) / 3;
+            if constexpr (J < 3) {
+                read(J + 1, X ^ 1);
+                more(J * kEach, min((J + 1) * kEach, kLoads));
+            }
 #pragma unroll
             for (int j = 0; j < TM; ++j)
 #pragma unroll
-                for (int i = 0; i < TN; ++i) acc[j][i] = fp4_mfma<J>(wf[i], qf[j], acc[j][i], sw[i], sq[j]);
+                for (int i = 0; i < TN; ++i) acc[j][i] = fp4_mfma<J>(fp4_operand(wf[X][i]), fp4_operand(qf[X][j]), acc[j][i], sw[i], sq[j]);
+            // (the MFMAs of a step stay in it: nothing else holds them to their place; in the registers that the compiler would choose)
+#pragma unroll
+            for (int j = 0; j < TM; ++j)
+#pragma unroll
+                for (int i = 0; i < TN; ++i) {
+                    if constexpr (TM * TN > 2) asm volatile("" : "+a"(acc[j][i]));
+                    else asm volatile("" : "+v"(acc[j][i]));
+                }
         });
     }
     // no load to LDS may outlive the workgroup, and sums and outputs go through LDS

@@ -1544,6 +1544,25 @@ Fp4ProductArgs fp4_args(const void* q, const void* s, int64_t s_stage, int M, in
     return a;
 }
 
+// the arguments of the product of rows x [M, k], which it quantises itself or (its workspace: q) a launch before it
+int fp4_quantised(const char* what, Fp4ProductArgs& a, const void* x, int x_dtype, int64_t x_stride, int k, uint8_t* q, void* stream) {
+    if (!x || x_stride < k || !aligned(x, dt_size(x_dtype)))
+        return fail(EXL3_EINVAL, "%s: x null, its alignment or row stride %lld", what, (long long)x_stride);
+    if (fp4_product_quantises(a.M, k, a.n)) {
+        a.x = x;
+        a.x_stride = x_stride;
+        a.k = k;
+        a.x_dt = x_dtype;
+        a.x_wide = fp4_rows_wide(x, x_stride, k, x_dtype);
+        return EXL3_OK;
+    }
+    uint8_t* s = q + fp4_q_bytes(a.M, k);
+    a.q = q;
+    a.s = s;
+    a.s_stage = (int64_t)a.M * 8;
+    return fp4_rows(what, x, x_dtype, x_stride, a.M, k, false, q, s, a.s_stage, stream);
+}
+
 int fp4_product(const char* what, Fp4ProductArgs a, void* out, int out_dtype, int64_t out_stride, void* stream) {
     a.out = out;
     a.out_stride = out_stride;
@@ -1551,17 +1570,34 @@ int fp4_product(const char* what, Fp4ProductArgs a, void* out, int out_dtype, in
     return e == hipSuccess ? EXL3_OK : hip_fail(e, what);
 }
 
-// up(silu(gate) * up) of quantised rows, the rows between in `workspace`; arguments checked, M > 0
-int fp4_mlp_products(const char* what, const void* q, const void* s, int64_t s_stage, int M, int k, int I, int n, const void* gu,
-                     const void* gu_scale, const float* gu_bias, const void* dn, const void* dn_scale, const float* dn_bias,
+// down(silu(gate) * up) with gate|up's arguments in `a`, what is between in `workspace`; arguments checked, M > 0
+int fp4_mlp_products(const char* what, Fp4ProductArgs a, int I, int n, const void* dn, const void* dn_scale, const float* dn_bias,
                      void* out, int out_dtype, int64_t out_stride, void* workspace, void* stream) {
-    Fp4ProductArgs a = fp4_args(q, s, s_stage, M, k, 2 * fp4_cols(I), gu, gu_scale, gu_bias);
-    a.hq = (uint8_t*)workspace;
-    a.hs = a.hq + fp4_q_bytes(M, I);
-    const hipError_t e = launch_fp4_gate_up(a, (hipStream_t)stream);
-    if (e != hipSuccess) return hip_fail(e, what);
-    return fp4_product(what, fp4_args(a.hq, a.hs, (int64_t)M * 8, M, I, n, dn, dn_scale, dn_bias), out, out_dtype, out_stride,
-                       stream);
+    Fp4ProductArgs d = fp4_args(nullptr, nullptr, 0, a.M, I, n, dn, dn_scale, dn_bias);
+    if (fp4_gate_up_in_tiles(a.M)) {
+        a.hq = (uint8_t*)workspace;
+        a.hs = a.hq + fp4_q_bytes(a.M, I);
+        const hipError_t e = launch_fp4_gate_up(a, (hipStream_t)stream);
+        if (e != hipSuccess) return hip_fail(e, what);
+        d.q = a.hq;
+        d.s = a.hs;
+        d.s_stage = (int64_t)a.M * 8;
+    } else {
+        if (int r = fp4_product(what, a, workspace, EXL3_DT_F32, a.n, stream)) return r;
+        d.x = workspace;
+        d.x_stride = a.n;
+        d.k = I;
+        d.x_dt = EXL3_DT_F32;
+        d.silu = d.x_wide = true;
+    }
+    return fp4_product(what, d, out, out_dtype, out_stride, stream);
+}
+
+// the rows between the two products: quantised, or fp32 for few of them (one size that never falls as M grows)
+size_t fp4_mlp_bytes(int M, int I) {
+    int few = M;
+    while (few > 0 && fp4_gate_up_in_tiles(few)) few = few > 64 ? 64 : few - 1;
+    return fp4_rows_bytes(M, I) + align256((size_t)few * 2 * fp4_cols(I) * 4);
 }
 
 int fp4_mlp_checks(const char* what, int M, int k, int I, int n, const void* gu, const void* gu_scale, const float* gu_bias,
@@ -1675,13 +1711,13 @@ int exl3_fp4_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, 
     const size_t need = exl3_fp4_linear_workspace(M, k, n);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return fail(EXL3_EWORKSPACE, "%s: workspace of %zu bytes on 16, got %zu", what, need, workspace_bytes);
-    uint8_t *q = (uint8_t*)workspace, *s = q + fp4_q_bytes(M, k);
-    if (int r = fp4_rows(what, x, x_dtype, x_stride, M, k, false, q, s, (int64_t)M * 8, stream)) return r;
-    return fp4_product(what, fp4_args(q, s, (int64_t)M * 8, M, k, n, w, sw, bias), out, out_dtype, out_stride, stream);
+    Fp4ProductArgs a = fp4_args(nullptr, nullptr, 0, M, k, n, w, sw, bias);
+    if (int r = fp4_quantised(what, a, x, x_dtype, x_stride, k, (uint8_t*)workspace, stream)) return r;
+    return fp4_product(what, a, out, out_dtype, out_stride, stream);
 }
 
 // the rows between the two products
-size_t exl3_fp4_mlp_matmul_workspace(int M, int I) { return M <= 0 || I <= 0 || I > 1 << 22 ? 0 : fp4_rows_bytes(M, I); }
+size_t exl3_fp4_mlp_matmul_workspace(int M, int I) { return M <= 0 || I <= 0 || I > 1 << 22 ? 0 : fp4_mlp_bytes(M, I); }
 
 int exl3_fp4_mlp_matmul(const void* q, const void* s, int64_t s_stage, int M, int k, int I, int n, const void* gu,
                         const void* gu_scale, const float* gu_bias, const void* dn, const void* dn_scale, const float* dn_bias,
@@ -1692,8 +1728,8 @@ int exl3_fp4_mlp_matmul(const void* q, const void* s, int64_t s_stage, int M, in
         return r;
     if (M == 0) return EXL3_OK;
     if (int r = fp4_rows_checks(what, q, s, s_stage, M)) return r;
-    return fp4_mlp_products(what, q, s, s_stage, M, k, I, n, gu, gu_scale, gu_bias, dn, dn_scale, dn_bias, out, out_dtype,
-                            out_stride, workspace, stream);
+    return fp4_mlp_products(what, fp4_args(q, s, s_stage, M, k, 2 * fp4_cols(I), gu, gu_scale, gu_bias), I, n, dn, dn_scale, dn_bias,
+                            out, out_dtype, out_stride, workspace, stream);
 }
 
 size_t exl3_fp4_mlp_workspace(int M, int k, int I) {
@@ -1710,10 +1746,10 @@ int exl3_fp4_mlp(const void* x, int x_dtype, int64_t x_stride, int M, int k, int
         return r;
     if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "%s: x dtype %d", what, x_dtype);
     if (M == 0) return EXL3_OK;
-    uint8_t *q = (uint8_t*)workspace, *s = q + fp4_q_bytes(M, k);
-    if (int r = fp4_rows(what, x, x_dtype, x_stride, M, k, false, q, s, (int64_t)M * 8, stream)) return r;
-    return fp4_mlp_products(what, q, s, (int64_t)M * 8, M, k, I, n, gu, gu_scale, gu_bias, dn, dn_scale, dn_bias, out, out_dtype,
-                            out_stride, q + fp4_rows_bytes(M, k), stream);
+    Fp4ProductArgs a = fp4_args(nullptr, nullptr, 0, M, k, 2 * fp4_cols(I), gu, gu_scale, gu_bias);
+    if (int r = fp4_quantised(what, a, x, x_dtype, x_stride, k, (uint8_t*)workspace, stream)) return r;
+    return fp4_mlp_products(what, a, I, n, dn, dn_scale, dn_bias, out, out_dtype, out_stride,
+                            (uint8_t*)workspace + fp4_rows_bytes(M, k), stream);
 }
 
 }  // extern "C"
