@@ -1637,7 +1637,7 @@ int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64
         return fail(EXL3_EINVAL, "%s: q or s null or not aligned", what);
     if (form == kFormFp4)
         if (int r = fp4_rows_checks(what, q, s, s_stage, M)) return r;
-    if ((M + (int64_t)15) * rms_norm_threads(k) >= kMaxThreads)
+    if ((M + (int64_t)15) * rms_norm_threads(M, k) >= kMaxThreads)
         return fail(EXL3_EUNSUPPORTED, "%s: M=%d rows of k=%d exceed one launch", what, M, k);
     RmsNormArgs a{};
     a.x = x;
@@ -1649,6 +1649,7 @@ int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64
     a.held = held;
     a.w = weight;
     a.eps = eps;
+    a.inv_k = 1.0 / k;
     a.M = M;
     a.k = k;
     a.y = y;

@@ -1,6 +1,9 @@
 // The residual's addition and the root-mean-square norm: held = x + residual in the residual's type (fp32 sum, one rounding),
-// y = h / sqrt(mean(h^2) + eps) * w of what is held (x itself without a residual), in fp32. y leaves as rows of x's type, as
-// e4m3 rows with fp32 scales (fp8_rows.cuh) or as 4-bit rows (fp4_rows.cuh), the last two from its fp32 values.
+// y = h / sqrt(mean(h^2) + eps) * w of what is held (x itself without a residual). y leaves as rows of x's type, as e4m3 rows with
+// fp32 scales (fp8_rows.cuh's form) or as 4-bit rows (fp4_rows.cuh).
+//
+// The sum and everything behind it are computed in 64 bits and rounded to 32 once (for e4m3 only its scale and its quotient are):
+// an error of 2^-24 takes one of 10^6 values over a border between two of e4m3's. It costs nothing where memory is the bound.
 //
 // A row is held in registers between its sum and its outputs: T lanes, up to C times 8 elements each, so every input is
 // read once and every output written once. 16 lanes hold 128 neighbouring columns, which is a block of e4m3 and four of the
@@ -8,29 +11,66 @@
 #include "exl3_kernels.h"
 #include "fp4_rows.cuh"
 
+#include <type_traits>
+
 namespace exl3 {
 namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float row16_sum(float v) {
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) v += lane_xor(v, m);
-    return v;
+__device__ __forceinline__ double lane_xor64(double v, int m) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __float_as_uint(lane_xor(__uint_as_float((uint32_t)u), m)), hi = __float_as_uint(lane_xor(__uint_as_float((uint32_t)(u >> 32)), m));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
 // the sum over the T threads of a row, in each of them
 template <int T>
-__device__ __forceinline__ float row_sum(float v) {
-    if constexpr (T == 16) return row16_sum(v);
-    v = wave_sum(v);
+__device__ __forceinline__ double row_sum(double v) {
+#pragma unroll
+    for (int m = 1; m < (T < 64 ? T : 64); m <<= 1) v += lane_xor64(v, m);
     if constexpr (T > 64) {
-        __shared__ float part[T / 64];
+        __shared__ double part[T / 64];
         if (lane_id() == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = row16_sum((lane_id() & 15) < T / 64 ? part[lane_id() & 15] : 0.0f);
+        v = part[0];
+#pragma unroll
+        for (int i = 1; i < T / 64; ++i) v += part[i];
     }
     return v;
+}
+
+// 1 / sqrt(a) for a > 0, to 2^-44: the hardware's 2^-23 and a step of Newton's; 0 for infinity
+__device__ __forceinline__ double root_inverse(double a) {
+    const double y = __builtin_amdgcn_rsq(a), e = __builtin_fma(-a * y, y, 1.0);
+    return a > 1.7e308 ? 0.0 : __builtin_fma(0.5 * y, e, y);
+}
+
+// a block of 128 values, 8 to each of 16 lanes, as quant_block has it, without a rounding before the scale's and the quotient's
+__device__ __forceinline__ uint2 quant_block64(const double (&t)[8], float& s) {
+    double top = 0;
+    uint32_t bits = 0;                               // (a maximum passes over NaN)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        top = __builtin_fmax(top, __builtin_fabs(t[j]));
+        bits = max(bits, abs_bits((float)t[j]));
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) top = __builtin_fmax(top, lane_xor64(top, m));
+    bits = row16_max(bits);
+    s = (float)(top * (1.0 / kE4m3Max));
+    s = s < kFp8MinScale ? kFp8MinScale : s;
+    const double inv0 = (double)__builtin_amdgcn_rcpf(s), inv = __builtin_fma(__builtin_fma(-(double)s, inv0, 1.0), inv0, inv0);
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = (float)(t[j] * inv);
+    if (bits >= 0x7F800000u) {                       // (rare, so a branch)
+        s = fp8_scale(bits);
+        const Fp8Div d(s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = d((float)t[j]);
+    }
+    return {pack_e4m3(q[0], q[1], q[2], q[3]), pack_e4m3(q[4], q[5], q[6], q[7])};
 }
 
 template <int DT, int RDT, bool WIDE>
@@ -70,23 +110,20 @@ struct Row {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = (WIDE ? 0 : j) < n ? v[j] : 0.0f;
     }
-    __device__ __forceinline__ void out(int c, float (&v)[8], float by) const {
+    // w: the weights of these columns, 0 behind the row
+    template <class W>
+    __device__ __forceinline__ void out(int c, float (&v)[8], double by, const W (&w)[8]) const {
         const int n = A.k - c;
+        double t[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= by;
-        if (A.w) {
-            float w[8];
-            load8<2, WIDE>(A.w, n > 0 ? c : 0, max(n, 1), w);
+        for (int j = 0; j < 8; ++j) t[j] = (WIDE ? 0 : j) < n ? (double)v[j] * by * (double)w[j] : 0.0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= w[j];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = (WIDE ? 0 : j) < n ? v[j] : 0.0f;       // (an infinite weight's 0 times it)
-        }
+        for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
         if (A.y && n > 0) store8<DT, WIDE>(A.y, (size_t)m * A.k + c, n, v);
         if (A.form == kFormFp8) {
             const int kb = fp8_blocks(A.k), b = c / kFp8Block;
             float s;
-            const uint2 q = quant_block(v, s);
+            const uint2 q = quant_block64(t, s);
             if (b >= kb) return;
             *(uint2*)(A.q + ((size_t)m * kb) * kFp8Block + c) = q;
             if (lane_id() % 16 == 0) ((float*)A.s)[(size_t)m * kb + b] = s;
@@ -101,41 +138,61 @@ struct Row {
     }
 };
 
+template <bool WIDE, class W>
+__device__ __forceinline__ void weights(const RmsNormArgs& A, int c, W (&w)[8]) {
+    const int n = A.k - c;
+    float f[8] = {1, 1, 1, 1, 1, 1, 1, 1};
+    if (A.w) load8<2, WIDE>(A.w, n > 0 ? c : 0, max(n, 1), f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = f[j];
+}
+
 template <int DT, int RDT, bool WIDE, int T, int C>
 __global__ void __launch_bounds__(T < kThreads ? kThreads : T) rms_norm_kernel(RmsNormArgs A) {
     constexpr int kRows = T < kThreads ? kThreads / T : 1;
-    const int64_t m = (int64_t)blockIdx.x * kRows + threadIdx.x / T;
-    if (m >= A.M) return;                            // (whole rows of T threads)
-    const int i = threadIdx.x % T, ks = (A.k + kFp4Stage - 1) / kFp4Stage * kFp4Stage;
-    const Row<DT, RDT, WIDE> row(A, m);
-    float sum = 0;
+    // (4-bit rows have whole stages of scales)
+    const int i = threadIdx.x % T, ks = A.form == kFormFp4 ? fp4_stages(A.k) * kFp4Stage : fp4_cols(A.k);
     if constexpr (C > 0) {
-        float v[C][8];
+        // (weights of one or two chunks in the 64 bits that they are used in)
+        std::conditional_t<C <= 2, double, float> w[C][8];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
+        for (int c = 0; c < C; ++c) weights<WIDE>(A, (c * T + i) * 8, w[c]);
+        // (whole rows of T threads; the same number of turns for all threads of a row)
+        for (int64_t m = (int64_t)blockIdx.x * kRows + threadIdx.x / T; m < A.M; m += (int64_t)gridDim.x * kRows) {
+            const Row<DT, RDT, WIDE> row(A, m);
+            double sum = 0;
+            float v[C][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[c][j] = 0;
-            if (c == 0 || c * T * 8 < ks) row.load((c * T + i) * 8, v[c]);
+            for (int c = 0; c < C; ++c) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[c][j] = 0;
+                if (c == 0 || c * T * 8 < ks) row.load((c * T + i) * 8, v[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum = __builtin_fma((double)v[c][j], (double)v[c][j], sum);
+            const double by = root_inverse(row_sum<T>(sum) * A.inv_k + (double)A.eps);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (c == 0 || c * T * 8 < ks) row.out((c * T + i) * 8, v[c], by, w[c]);
+            if constexpr (T > 64) __syncthreads();   // (the sum's LDS is used again)
         }
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[c][j], v[c][j], sum);
-        const float by = 1.0f / __builtin_sqrtf(row_sum<T>(sum) / (float)A.k + A.eps);
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (c == 0 || c * T * 8 < ks) row.out((c * T + i) * 8, v[c], by);
     } else {
-        float v[8];
+        const int64_t m = blockIdx.x;
+        const Row<DT, RDT, WIDE> row(A, m);
+        double sum = 0;
+        float v[8], w[8];
         for (int c = 0; c < ks; c += T * 8) {
             row.load(c + i * 8, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[j], v[j], sum);
+            for (int j = 0; j < 8; ++j) sum = __builtin_fma((double)v[j], (double)v[j], sum);
         }
-        const float by = 1.0f / __builtin_sqrtf(row_sum<T>(sum) / (float)A.k + A.eps);
+        const double by = root_inverse(row_sum<T>(sum) * A.inv_k + (double)A.eps);
         for (int c = 0; c < ks; c += T * 8) {
             row.again(c + i * 8, v);
-            row.out(c + i * 8, v, by);
+            weights<WIDE>(A, c + i * 8, w);
+            row.out(c + i * 8, v, by, w);
         }
     }
 }
@@ -143,15 +200,21 @@ __global__ void __launch_bounds__(T < kThreads ? kThreads : T) rms_norm_kernel(R
 template <int DT, int RDT, bool WIDE, int T, int C>
 void launch_rows(const RmsNormArgs& a, hipStream_t st) {
     constexpr int kRows = T < kThreads ? kThreads / T : 1;
-    hipLaunchKernelGGL((rms_norm_kernel<DT, RDT, WIDE, T, C>), dim3((unsigned)((a.M - 1) / kRows + 1)),
-                       dim3(T < kThreads ? kThreads : T), 0, st, a);
+    // (8 workgroups per CU, each with every 2,048th row: as many as are there at a time, and the weights are loaded once; 8,192 x
+    // 2,048 bf16 to bf16 23.9 us, a workgroup for every row 26.1)
+    const int64_t all = (int64_t)(a.M - 1) / kRows + 1, most = C > 0 ? kCus * 8 : all;
+    hipLaunchKernelGGL((rms_norm_kernel<DT, RDT, WIDE, T, C>), dim3((unsigned)(all < most ? all : most)), dim3(T < kThreads ? kThreads : T), 0,
+                       st, a);
 }
 
 template <int DT, int RDT, bool WIDE>
 void launch_norm(const RmsNormArgs& a, hipStream_t st) {
-    const int t = rms_norm_threads(a.k);
-    if (t == 16) launch_rows<DT, RDT, WIDE, 16, 2>(a, st);
-    else if (t == 64) launch_rows<DT, RDT, WIDE, 64, 4>(a, st);
+    const int t = rms_norm_threads(a.M, a.k);
+    if (t == 16 && a.k <= 128 && a.form != kFormFp4) launch_rows<DT, RDT, WIDE, 16, 1>(a, st);
+    else if (t == 16) launch_rows<DT, RDT, WIDE, 16, 2>(a, st);
+    else if (t == 64) launch_rows<DT, RDT, WIDE, 64, 2>(a, st);
+    else if (t == 256 && a.k <= 2048) launch_rows<DT, RDT, WIDE, 256, 1>(a, st);
+    else if (t == 256 && a.k <= 4096) launch_rows<DT, RDT, WIDE, 256, 2>(a, st);
     else if (t == 256) launch_rows<DT, RDT, WIDE, 256, 4>(a, st);
     else if (a.k <= 32768) launch_rows<DT, RDT, WIDE, 1024, 4>(a, st);
     else launch_rows<DT, RDT, WIDE, 1024, 0>(a, st);

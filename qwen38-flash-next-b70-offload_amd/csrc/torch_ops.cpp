@@ -655,17 +655,34 @@ void no_gradients(const at::Tensor& x, const char* what) {
 
 int64_t fp4_stages(int64_t k) { return (k + 255) / 256; }
 
+// The strides of scales [..., stages, 8] whose stages are outermost in memory: those of `lead` rows of 8, the stages, 1
+std::vector<int64_t> fp4_scale_strides(at::IntArrayRef lead, int64_t& rows) {
+    std::vector<int64_t> v(lead.size() + 2);
+    int64_t at = 8;
+    for (size_t i = lead.size(); i-- > 0;) {
+        v[i] = at;
+        at *= lead[i];
+    }
+    v[lead.size()] = at;
+    v[lead.size() + 1] = 1;
+    rows = at / 8;
+    return v;
+}
+
 // quantised rows of x's leading sizes and k columns: codes [..., kp / 2] and scales [..., stages, 8], the stages outermost in memory
 std::tuple<at::Tensor, at::Tensor> fp4_rows_empty(const at::Tensor& x, int64_t k) {
-    auto sizes = with_last(x.sizes(), 8);
-    sizes.insert(sizes.begin(), fp4_stages(k));
+    auto q = with_last(x.sizes(), fp8_up(k) / 2);
+    auto sizes = x.sizes().vec();
+    sizes.back() = fp4_stages(k);
+    sizes.push_back(8);
+    int64_t rows;
     const auto o = x.options().dtype(at::kByte);
-    return {at::empty(with_last(x.sizes(), fp8_up(k) / 2), o), at::empty(sizes, o).movedim(0, -2)};
+    return {at::empty(q, o), at::empty_strided(sizes, fp4_scale_strides(x.sizes().slice(0, x.dim() - 1), rows), o)};
 }
 
 // Quantised rows as the C-ABI takes them (copies only where the strides or addresses do not fit)
 struct Fp4Rows {
-    at::Tensor q, s;                                 // s with the stages first
+    at::Tensor q, s;
     int M = 0, kp = 0;
     int64_t s_stage = 0;
     Fp4Rows(const at::Tensor& q_, const at::Tensor& s_, const char* what) {
@@ -674,18 +691,24 @@ struct Fp4Rows {
                     what, ": q uint8 [..., a multiple of 64], got ", q_.scalar_type(), " ", q_.sizes());
         on_device_of(q_, s_, what);
         kp = (int)(2 * q_.size(-1));
-        M = (int)(q_.numel() / q_.size(-1));
-        auto want = with_last(q_.sizes(), fp4_stages(kp));
-        want.push_back(8);
-        TORCH_CHECK(s_.scalar_type() == at::kByte && s_.sizes().vec() == want, what, ": s uint8 ", want, ", got ",
-                    s_.scalar_type(), " ", s_.sizes());
-        q = q_.contiguous();
+        const int64_t d = q_.dim() - 1;
+        TORCH_CHECK(s_.scalar_type() == at::kByte && s_.dim() == d + 2 && s_.size(d) == fp4_stages(kp) && s_.size(d + 1) == 8 &&
+                        s_.sizes().slice(0, d) == q_.sizes().slice(0, d),
+                    what, ": s uint8 [..., ", fp4_stages(kp), ", 8] with q's leading sizes, got ", s_.scalar_type(), " ", s_.sizes());
+        q = q_.is_contiguous() ? q_ : q_.contiguous();
         if ((uintptr_t)q.const_data_ptr() % 16) q = q.clone();
-        s = s_.movedim(-2, 0);
-        const auto rows = s.select(0, 0);
-        if (!rows.is_contiguous() || (s.size(0) > 1 && (s.stride(0) < 8 * (int64_t)M || s.stride(0) % 8))) s = s.contiguous();
-        if ((uintptr_t)s.const_data_ptr() % 8) s = s.clone(at::MemoryFormat::Contiguous);
-        s_stage = s.size(0) > 1 ? s.stride(0) : 8 * (int64_t)M;
+        int64_t rows;
+        const auto want = fp4_scale_strides(q_.sizes().slice(0, d), rows);
+        M = (int)rows;
+        const bool one = s_.size(d) == 1;
+        bool fits = s_.stride(d + 1) == 1 && (one || (s_.stride(d) >= want[d] && s_.stride(d) % 8 == 0)) && (uintptr_t)s_.const_data_ptr() % 8 == 0;
+        for (int64_t i = 0; i < d; ++i) fits = fits && (s_.size(i) == 1 || s_.stride(i) == want[i]);
+        s = s_;
+        if (!fits && M > 0) {
+            s = at::empty_strided(s_.sizes(), want, s_.options());
+            s.copy_(s_);
+        }
+        s_stage = one || M == 0 ? 8 * rows : s.stride(d);
     }
 };
 
@@ -741,7 +764,8 @@ void fp4_weight_checks(const at::Tensor& x, const at::Tensor& w, const at::Tenso
                     w.size(0) <= INT32_MAX,
                 what, ": weight uint8 [n, ", fp8_up(k) / 2, "] contiguous, got ", w.scalar_type(), " ", w.sizes());
     TORCH_CHECK(sw.scalar_type() == at::kByte && sw.dim() == 3 && sw.size(0) == w.size(0) && sw.size(1) == fp4_stages(k) &&
-                    sw.size(2) == 8 && sw.movedim(1, 0).is_contiguous(),
+                    sw.size(2) == 8 && sw.stride(2) == 1 && sw.stride(0) == 8 &&
+                    (sw.size(1) == 1 || sw.stride(1) == 8 * sw.size(0)),
                 what, ": weight_scale uint8 [", w.size(0), ", ", fp4_stages(k), ", 8] with the stages outermost in memory, got ",
                 sw.scalar_type(), " ", sw.sizes());
 }

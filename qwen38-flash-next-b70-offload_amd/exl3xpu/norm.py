@@ -7,11 +7,11 @@
   q, s, h = norm.quant(x, residual, "fp4")      as 4-bit rows, as Fp4Linear.quantised and Fp4Mlp.quantised take them
   q, s, y, h = norm.quant(x, residual, "fp8", rows=True)     y as well: the router and the EXL3 experts take it
 
-One launch, each input read once. Everything is computed in fp32: h is rounded once, to the residual's dtype (x's or fp32), and the norm is
-that of the rounded h, so that it is the same as a norm of h by itself. q, s are those of the norm in fp32, not of y. The forms are
-exl3xpu.fp8's and exl3xpu.fp4's. Rows may lie inside wider ones at a uniform stride, and x [tokens, heads, k] inside the rows of a fused
-projection. Squares are summed in fp32: a row whose sum passes 3.4e38 gives 0, one with an infinite element NaN there and 0
-elsewhere, one with a NaN element NaN. Calls run on the device's current stream, keep no state and can be captured into a graph. They
+One launch, each input read once. h is added in fp32 and rounded once, to the residual's dtype (x's or fp32), and the norm is that of the
+rounded h, so that it is the same as a norm of h by itself; it is computed in 64 bits and rounded once. q, s are those of the norm before
+it is rounded to x's dtype, in the forms of exl3xpu.fp8 and exl3xpu.fp4. Rows may lie inside wider ones at a uniform stride, and x
+[tokens, heads, k] inside the rows of a fused projection. A row with an infinite element is NaN there and 0 elsewhere, one with a NaN
+element NaN. Calls run on the device's current stream, keep no state and can be captured into a graph. They
 are for inference: inputs that require gradients are refused.
 """
 from __future__ import annotations
