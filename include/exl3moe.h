@@ -436,8 +436,8 @@ int exl3_fp4_dequant(const void* q, const void* s, int64_t s_stage, int M, int k
  * <= 2^27. No state between calls, no workspace. */
 int exl3_fp4_matmul(const void* q, const void* s, int64_t s_stage, int M, int k, int n, const void* w, const void* sw,
                     const float* bias, void* out, int out_dtype, int64_t out_stride, void* stream);
-/* the same of x [M, k], quantised within the call; its workspace (whose size never falls as M grows) starts on 16 bytes and is
- * not shared by calls that run at the same time */
+/* the same of x [M, k], quantised within the call; its workspace (whose size never falls as M grows, 0 for few rows) starts on 16
+ * bytes and is not shared by calls that run at the same time */
 size_t exl3_fp4_linear_workspace(int M, int k, int n);
 int exl3_fp4_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, int n, const void* w, const void* sw,
                     const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,

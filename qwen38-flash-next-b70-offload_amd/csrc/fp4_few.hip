@@ -98,6 +98,12 @@ __global__ void __launch_bounds__(64 * NW) fp4_few_kernel(Fp4ProductArgs A, int 
     if (t >= ct * rt) return;
     const int n0 = t / rt * TN * 16, mb = t % rt * R, M = min(R, A.M - mb);
     const int pitch = A.kp / 2;
+    // (this thread's outputs' biases: on their way before anything else)
+    constexpr int kOuts = (TM * TN + NW - 1) / NW;
+    v4f bias[kOuts];
+    const Rsrc biases = buffer_of(A.bias, A.bias ? (uint32_t)A.n * 4 : 0);
+#pragma unroll
+    for (int o = 0; o < kOuts; ++o) bias[o] = floats_of(biases, n0 + (wave + o * NW) % TN * 16 + g * 4);
     v4f acc[TM][TN] = {};
     for (int b0 = wave; b0 < A.kb; b0 += NW * S) {
         v4i wf[S][TN][2], qf[S][TM][2];
@@ -196,16 +202,16 @@ __global__ void __launch_bounds__(64 * NW) fp4_few_kernel(Fp4ProductArgs A, int 
         for (int i = 0; i < TN; ++i) sums[wave][j * TN + i][l] = acc[j][i];
     __syncthreads();
     // a thread's four columns n0 + 16 i + 4 g of row 16 j + r
-    for (int f = wave; f < TM * TN; f += NW) {
+#pragma unroll
+    for (int o = 0; o < kOuts; ++o) {
+        const int f = wave + o * NW;
+        if (f >= TM * TN) break;
         const int m = f / TN * 16 + r, n = n0 + f % TN * 16 + g * 4;
         if (m >= M || n >= A.n) continue;
         v4f v = {};
 #pragma unroll
         for (int i = 0; i < NW; ++i) v += sums[i][f][l];
-        if (A.bias)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (n + c < A.n) v[c] += A.bias[n + c];
+        v += bias[o];
         const bool whole = n + 4 <= A.n && A.out_stride % 4 == 0;
         const size_t at = (size_t)(mb + m) * A.out_stride + n;
         if (out_dt == 2) {

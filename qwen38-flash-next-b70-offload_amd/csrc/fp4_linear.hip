@@ -15,7 +15,7 @@ struct Pick {
     bool few;                                        // at most one workgroup per CU
     int64_t cost;
 };
-Pick pick_tile(int M, int n) {
+Pick pick_tile(int M, int n, int kb) {
     constexpr int kSizes[][2] = {{32, 32}, {64, 64}, {128, 64}, {128, 128}, {256, 256}};
     Pick best{kFp4Tile256, false, 0};
     for (int i = kFp4Tile32; i <= kFp4Tile256; ++i) {
@@ -24,6 +24,7 @@ Pick pick_tile(int M, int n) {
         int64_t cost = rounds * rows;
         if (i == kFp4Tile128x64 && rounds > 1) continue;
         if (i == kFp4Tile128 && rounds > 1) cost = tiles * rows / kCus;
+        if (i == kFp4Tile256 && kb < 4 && best.cost) continue;
         if (i == kFp4Tile256) cost = rounds * (rows + rows / 5);
         else if ((tiles + 7) * 512 >= kMaxThreads) continue;
         if (!best.cost || cost <= best.cost) best = {i, rounds == 1, cost};
@@ -76,7 +77,7 @@ bool fp4_product_quantises(int M, int, int) { return M <= kOwnRows; }
 
 hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t st) {
     const FewTile f = pick_few(a.M, a.n, !a.q);
-    const Pick p = pick_tile(a.M, a.n);
+    const Pick p = pick_tile(a.M, a.n, a.kb);
     if (!a.q || a.M <= kOwnRows || (f.tn && f.cost * 4 <= p.cost * 3)) launch_fp4_few(a, f.tn, f.R, out_dt, st);
     else launch_tile<false>(p, a, out_dt, st);
     return hipGetLastError();
@@ -85,7 +86,7 @@ hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t s
 bool fp4_gate_up_in_tiles(int M) { return M > kOwnRows; }
 
 hipError_t launch_fp4_gate_up(const Fp4ProductArgs& a, hipStream_t st) {
-    launch_tile<true>(pick_tile(a.M, a.n), a, 2, st);
+    launch_tile<true>(pick_tile(a.M, a.n, a.kb), a, 2, st);
     return hipGetLastError();
 }
 

@@ -10,7 +10,7 @@
 
 namespace exl3 {
 
-template <bool SILU>
+template <bool SILU, bool BIAS>
 __global__ void __launch_bounds__(256, 1) fp4_tile256_kernel(Fp4ProductArgs A, int mt, int nt, int per, int out_dt) {
     constexpr int B = 256, NW = 4, T = 4, kCode = B / 8 / NW, kScale = 2 * B / 32 / NW, kLoads = 2 * kCode + kScale;
     // (one variable: where there are two the compiler tells their accesses apart, and waits for all loads to LDS before it
@@ -146,21 +146,28 @@ __global__ void __launch_bounds__(256, 1) fp4_tile256_kernel(Fp4ProductArgs A, i
         int e = l;                                   // (kept from being computed with before the loop: registers)
         asm volatile("" : "+v"(e));
         const int eh = e >> 5, er = e & 31;
-        auto four = [&](int j, int i, int b) {
-            v4f v = {acc[j][i][b * 4], acc[j][i][b * 4 + 1], acc[j][i][b * 4 + 2], acc[j][i][b * 4 + 3]};
-            if (A.bias) {
-                const int n = tile.n0 + wn + i * 32 + b * 8 + eh * 4;
+        v4f bias[T][4];
+        if constexpr (BIAS) {
+            const Rsrc biases = buffer_of(A.bias, (uint32_t)A.n * 4);
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (n + c < A.n) v[c] += A.bias[n + c];
-            }
-            return v;
+            for (int i = 0; i < T; ++i)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) bias[i][b] = floats_of(biases, tile.n0 + wn + i * 32 + b * 8 + eh * 4);
+        }
+        auto four = [&](int j, int i, int b) {
+            const v4f v = {acc[j][i][b * 4], acc[j][i][b * 4 + 1], acc[j][i][b * 4 + 2], acc[j][i][b * 4 + 3]};
+            if constexpr (BIAS) return v + bias[i][b];
+            else return v;
         };
+        // (a fragment stays in accumulation registers until its turn: moved out at once, they would not fit the others)
+        auto hold = [&](int j, int i) { asm volatile("" : "+a"(acc[j][i])); };
         if constexpr (SILU) {
 #pragma unroll
             for (int j = 0; j < T; ++j)
 #pragma unroll
                 for (int i = 0; i < T; i += 2) {
+                    hold(j, i);
+                    hold(j, i + 1);
                     float v[16];
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
@@ -211,6 +218,7 @@ __global__ void __launch_bounds__(256, 1) fp4_tile256_kernel(Fp4ProductArgs A, i
                     if constexpr (DT == 2) {
 #pragma unroll
                         for (int i = 0; i < T; ++i) {
+                            hold(j, i);
 #pragma unroll
                             for (int b = 0; b < 4; ++b) *(v4f*)(o + er * 128 + ((b * 2 + eh) ^ (er & 7)) * 16) = four(j, i, b);
                             store(j, tile.n0 + wn + i * 32, full);
@@ -218,6 +226,8 @@ __global__ void __launch_bounds__(256, 1) fp4_tile256_kernel(Fp4ProductArgs A, i
                     } else {
 #pragma unroll
                         for (int i = 0; i < T; i += 2) {
+                            hold(j, i);
+                            hold(j, i + 1);
 #pragma unroll
                             for (int b = 0; b < 8; ++b) *(v4u*)(o + er * 128 + (b ^ (er & 7)) * 16 + eh * 8) = narrow4<DT>(four(j, i + b / 4, b & 3));
                             store(j, tile.n0 + wn + i * 32, full);
@@ -242,8 +252,10 @@ __global__ void __launch_bounds__(256, 1) fp4_tile256_kernel(Fp4ProductArgs A, i
 void launch_fp4_tiles256(const Fp4ProductArgs& a, bool silu, int out_dt, hipStream_t st) {
     const int mt = (a.M - 1) / 256 + 1, nt = (a.n - 1) / 256 + 1, per = (int)(((int64_t)mt * nt + 7) / 8);
     const dim3 grid((unsigned)(per < kCus / 8 ? per : kCus / 8) * 8);
-    if (silu) hipLaunchKernelGGL((fp4_tile256_kernel<true>), grid, dim3(256), 0, st, a, mt, nt, per, out_dt);
-    else hipLaunchKernelGGL((fp4_tile256_kernel<false>), grid, dim3(256), 0, st, a, mt, nt, per, out_dt);
+    // (biases are a kernel of their own: the additions alone take 1.5 us a tile)
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a, mt, nt, per, out_dt); };
+    if (silu) a.bias ? launch(fp4_tile256_kernel<true, true>) : launch(fp4_tile256_kernel<true, false>);
+    else a.bias ? launch(fp4_tile256_kernel<false, true>) : launch(fp4_tile256_kernel<false, false>);
 }
 
 }  // namespace exl3

@@ -195,15 +195,15 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
                 for (int k = 0; k < KG - 1; ++k) acc[j][i] += lds.last.sums[k][wv][j * TN + i][l];
     }
     // a lane's columns of fragment i: fours at n0 + wn + 32 i + 8 b + 4 h, of row m0 + wm + 32 j + r
-    auto four = [&](int j, int i, int b) {
-        v4f v = {acc[j][i][b * 4], acc[j][i][b * 4 + 1], acc[j][i][b * 4 + 2], acc[j][i][b * 4 + 3]};
-        if (A.bias) {
-            const int n = n0 + wn + i * 32 + b * 8 + h * 4;
+    v4f bias[TN][4] = {};
+    const Rsrc biases = buffer_of(A.bias, (uint32_t)A.n * 4);
+    if (A.bias)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (n + c < A.n) v[c] += A.bias[n + c];
-        }
-        return v;
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) bias[i][b] = floats_of(biases, n0 + wn + i * 32 + b * 8 + h * 4);
+    auto four = [&](int j, int i, int b) {
+        return v4f{acc[j][i][b * 4], acc[j][i][b * 4 + 1], acc[j][i][b * 4 + 2], acc[j][i][b * 4 + 3]} + bias[i][b];
     };
     if constexpr (SILU) {
 #pragma unroll

@@ -1696,8 +1696,9 @@ int exl3_fp4_matmul(const void* q, const void* s, int64_t s_stage, int M, int k,
     return fp4_product("fp4_matmul", fp4_args(q, s, s_stage, M, k, n, w, sw, bias), out, out_dtype, out_stride, stream);
 }
 
+// The quantised rows; none for few rows, which the product quantises itself
 size_t exl3_fp4_linear_workspace(int M, int k, int n) {
-    if (M <= 0 || k <= 0 || n <= 0) return 0;
+    if (M <= 0 || k <= 0 || n <= 0 || fp4_product_quantises(M, k, n)) return 0;
     return fp4_rows_bytes(M, k);
 }
 
@@ -1710,7 +1711,7 @@ int exl3_fp4_linear(const void* x, int x_dtype, int64_t x_stride, int M, int k, 
     if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "%s: x dtype %d", what, x_dtype);
     if (M == 0) return EXL3_OK;
     const size_t need = exl3_fp4_linear_workspace(M, k, n);
-    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return fail(EXL3_EWORKSPACE, "%s: workspace of %zu bytes on 16, got %zu", what, need, workspace_bytes);
     Fp4ProductArgs a = fp4_args(nullptr, nullptr, 0, M, k, n, w, sw, bias);
     if (int r = fp4_quantised(what, a, x, x_dtype, x_stride, k, (uint8_t*)workspace, stream)) return r;
@@ -1735,7 +1736,7 @@ int exl3_fp4_mlp_matmul(const void* q, const void* s, int64_t s_stage, int M, in
 
 size_t exl3_fp4_mlp_workspace(int M, int k, int I) {
     if (M <= 0 || k <= 0 || I <= 0 || I > 1 << 22) return 0;
-    return fp4_rows_bytes(M, k) + exl3_fp4_mlp_matmul_workspace(M, I);
+    return exl3_fp4_linear_workspace(M, k, I) + exl3_fp4_mlp_matmul_workspace(M, I);
 }
 
 int exl3_fp4_mlp(const void* x, int x_dtype, int64_t x_stride, int M, int k, int I, int n, const void* gu, const void* gu_scale,
@@ -1750,7 +1751,7 @@ int exl3_fp4_mlp(const void* x, int x_dtype, int64_t x_stride, int M, int k, int
     Fp4ProductArgs a = fp4_args(nullptr, nullptr, 0, M, k, 2 * fp4_cols(I), gu, gu_scale, gu_bias);
     if (int r = fp4_quantised(what, a, x, x_dtype, x_stride, k, (uint8_t*)workspace, stream)) return r;
     return fp4_mlp_products(what, a, I, n, dn, dn_scale, dn_bias, out, out_dtype, out_stride,
-                            (uint8_t*)workspace + fp4_rows_bytes(M, k), stream);
+                            (uint8_t*)workspace + exl3_fp4_linear_workspace(M, k, I), stream);
 }
 
 }  // extern "C"

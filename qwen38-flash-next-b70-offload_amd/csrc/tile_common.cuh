@@ -35,6 +35,11 @@ __device__ __forceinline__ void to_lds(void* lds, Rsrc from, uint32_t lane_off, 
     else __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_any*)lds, 4, lane_off, off, 0, 0);
 }
 
+// four floats from element n on, 0 behind the buffer's end
+__device__ __forceinline__ v4f floats_of(Rsrc from, int n) {
+    return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, n * 4, 0, 0));
+}
+
 // place of 16-byte piece c of a row in LDS: rows are 128 bytes apart (or an odd multiple), and with this the fragment reads
 // of 16 rows meet every bank once
 __device__ __forceinline__ int piece_at(int row, int c) { return c ^ ((row >> 1) & 7); }

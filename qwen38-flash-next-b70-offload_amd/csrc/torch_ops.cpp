@@ -786,9 +786,10 @@ at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor
     auto out = fp4_linear_meta(x, w, sw, bias);
     if (M == 0) return out;
     const size_t ws = exl3_fp4_linear_workspace(M, k, (int)n);
-    auto buf = at::empty({(int64_t)ws}, x.options().dtype(at::kByte));
+    at::Tensor buf;
+    if (ws) buf = at::empty({(int64_t)ws}, x.options().dtype(at::kByte));
     check(exl3_fp4_linear(x2.data_ptr(), dt, row_stride(x2), M, k, (int)n, w.const_data_ptr(), sw.const_data_ptr(), b,
-                          out.data_ptr(), dt, n, buf.data_ptr(), ws, cur_stream(x)),
+                          out.data_ptr(), dt, n, ws ? buf.data_ptr() : nullptr, ws, cur_stream(x)),
           "fp4_linear");
     return out;
 }

@@ -101,7 +101,7 @@ def test_products_refuse_their_own():
     assert [f(**k) for f in (_matmul, _mlp_matmul) for k in (dict(q=None), dict(s=None), dict(q=P + 8), dict(s=P + 4), dict(stage=24),
                                                              dict(stage=33))] == [BAD] * 12
     assert [f(**k) for f in (_linear, _mlp) for k in (dict(x=None), dict(dtype=3), dict(xs=255), dict(x=P + 1))] == [BAD] * 8
-    assert [_linear(ws=None), _linear(size=16), _linear(ws=P + 4)] == [WORKSPACE] * 3
+    assert [_linear(M=40, stride=256, ws=None), _linear(M=40, size=16), _linear(M=40, ws=P + 4)] == [WORKSPACE] * 3
     assert _matmul(M=0, q=None, s=None, w=None, sw=None, out=None) == _linear(M=0, x=None, ws=None) == 0
     assert _mlp(M=0, x=None, ws=None) == _mlp_matmul(M=0, q=None, s=None, ws=None) == 0
 
@@ -112,7 +112,8 @@ def test_workspaces_never_fall_as_the_rows_grow(k, n):
     for f, least in ((lambda M: L.exl3_fp4_linear_workspace(M, k, n), lambda M: M * k // 2), (lambda M: L.exl3_fp4_mlp_matmul_workspace(M, n), lambda M: M * n // 2),
                      (lambda M: L.exl3_fp4_mlp_workspace(M, k, n), lambda M: M * (k + n) // 2)):
         b = [f(M) for M in [*range(1, 600), 1024, 4096, 8192, 60000]]
-        assert all(x <= y for x, y in zip(b, b[1:])) and b[0] >= least(1) and b[-1] >= least(60000)
+        # (few rows are quantised within the product)
+        assert all(x <= y for x, y in zip(b, b[1:])) and b[63] >= least(64) and b[-1] >= least(60000)
         assert [f(0), f(-5)] == [0] * 2
     assert [L.exl3_fp4_linear_workspace(4, 0, 8), L.exl3_fp4_linear_workspace(4, 8, -1), L.exl3_fp4_mlp_workspace(4, 0, 8),
             L.exl3_fp4_mlp_workspace(4, 8, 0), L.exl3_fp4_mlp_matmul_workspace(4, 0), L.exl3_fp4_mlp_matmul_workspace(4, 1 << 23)] == [0] * 6
