@@ -1,4 +1,30 @@
 // Which kernel computes a 4-bit float product: fp4_few.hip's, a tile of fp4_tiles.cuh or fp4_tile256.hip's.
+//
+// What takes the time is what a CU has to bring in (fp8_linear.hip has the rates): BM + BN rows of k for each tile. The tile is
+// the one for which that is least, max(1, tiles / 256 CUs) (BM + BN), the larger one where two are equal, but for these: 128 x 64
+// only where each CU has one at most; 128 x 128 with more than one counts by the tile, since two share a CU; 256 x 256, whose
+// rounds are whole, costs a fifth more, and is for four stages of k at least, since its first loads and last stores have nothing
+// beside them (512 -> 2048, 8,192 rows: 128 x 128 13.7, 256 x 256 14.8).
+//
+// Quantised rows, bf16 outputs, weights from HBM, us per call out of a graph; * is what the rule takes.
+//   4096 -> 2048, rows  100   200   400   777  1,024  1,500  2,048  4,096  8,192
+//   32 x 32             6.3*  7.0  11.9  20.8   22.6   32.1   42.6   83.2  163.7
+//   64 x 64             7.0   7.0*  7.4* 11.1   11.7   18.5   21.0   39.2   76.1
+//   128 x 64            8.8   8.9   9.2   9.5*   9.9*  17.0   18.7   33.4   65.6
+//   128 x 128          11.2  11.3  11.6  11.9   12.1   12.7*  14.1*  23.5*  43.1
+//   256 x 256          26.2  26.6  26.6  25.4   25.5   29.2   25.9   28.1   38.1*
+//   2048 -> 12,288
+//   32 x 32            15.1  25.4  40.7  71.2   98.4  130.9  181.3  346.6  677.1
+//   64 x 64             9.4  14.5  21.6  32.7   42.6   55.1   82.3  146.4  273.3
+//   128 x 64            7.8* 12.8  18.0  32.8   35.3   46.4   70.0  143.3  249.2
+//   128 x 128           9.4  10.1* 15.7* 26.6   27.6   35.2*  46.3   89.8  159.3
+//   256 x 256          21.1  21.8  21.8  20.8*  22.1*  40.2   40.8*  65.8* 120.7*
+//
+// Few rows (fp4_few.hip) cost by what a workgroup brings in too, 14 for each 16 columns and 1 for each row (5 where it quantises them),
+// and 10 for each further fragment of columns, which leaves fewer waves to load. They take that kernel up to a cost of 50, and up to
+// 48 rows where that is three quarters of the tile's at most (4096 -> 2048: 64 rows, cost 46, 5.9 us, in tiles 6.3; 100 rows, cost 63, 6.7 and
+// 6.3; 2048 -> 12,288: 32 rows, cost 94 and 128, 6.8 and 7.3; 64 rows, 126 and 128, 8.4 and 7.2). 12 rows and fewer are quantised inside
+// (2048 -> 12,288: 12 rows 8.1 us, by a launch before it 8.6; 16 rows 9.9 and 9.1).
 #include "fp4_tiles.cuh"
 
 namespace exl3 {
@@ -43,7 +69,7 @@ FewTile pick_few(int M, int n, bool own) {
         for (int groups = 1; groups <= 4 && groups <= M; groups *= 2) {
             const int R = (M + groups - 1) / groups;
             const int64_t workgroups = (int64_t)((n - 1) / (16 * tn) + 1) * ((M - 1) / R + 1), rounds = (workgroups + kCus - 1) / kCus;
-            if (R > (own ? 16 : 64) || (workgroups + 7) * 1024 >= kMaxThreads) continue;
+            if (R > (own ? 16 : 48) || (workgroups + 7) * 1024 >= kMaxThreads) continue;
             const int64_t cost = rounds * (14 * tn + (own ? 5 * R : R)) + (own ? 0 : 10 * (tn - 1));
             if (!best.tn || cost < best.cost) best = {tn, R, cost};
         }
@@ -78,7 +104,8 @@ bool fp4_product_quantises(int M, int, int) { return M <= kOwnRows; }
 hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t st) {
     const FewTile f = pick_few(a.M, a.n, !a.q);
     const Pick p = pick_tile(a.M, a.n, a.kb);
-    if (!a.q || a.M <= kOwnRows || (f.tn && f.cost * 4 <= p.cost * 3)) launch_fp4_few(a, f.tn, f.R, out_dt, st);
+    const bool few = f.tn && (f.cost <= 50 || (a.M <= 48 && f.cost * 4 <= p.cost * 3));
+    if (!a.q || a.M <= kOwnRows || few) launch_fp4_few(a, f.tn, f.R, out_dt, st);
     else launch_tile<false>(p, a, out_dt, st);
     return hipGetLastError();
 }

@@ -1,7 +1,9 @@
 // Rows to 4-bit floats (fp4_rows.cuh), of x or of silu(gate) * up of fused gate|up rows, and back.
 //
 // 32 lanes hold a stage of 256 columns of a row, 8 elements each: a block of 32 is four lanes, its amax two DPP steps, and each
-// element is read once. A workgroup's 8 rows are neighbours, so that their scales are one 64-byte piece. Bound by memory.
+// element is read once. A workgroup's 8 rows are neighbours, so that their scales are one 64-byte piece. Bound by memory. us per
+// call out of a graph: 8,192 x 2,048 bf16 10.4 (42 MB, 4.1 TB/s; a large copy 5.2; two or four groups of rows to a workgroup 10.4
+// and 9.8, but 2,000 rows 4.1 and 4.5 for 3.9), back to bf16 11.3, 301 x 1,000 fp16 2.2, any launch's.
 #include "exl3_kernels.h"
 #include "fp4_rows.cuh"
 
