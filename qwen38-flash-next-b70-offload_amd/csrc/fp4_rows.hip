@@ -3,7 +3,8 @@
 // 32 lanes hold a stage of 256 columns of a row, 8 elements each: a block of 32 is four lanes, its amax two DPP steps, and each
 // element is read once. A workgroup's 8 rows are neighbours, so that their scales are one 64-byte piece. Bound by memory. us per
 // call out of a graph: 8,192 x 2,048 bf16 10.4 (42 MB, 4.1 TB/s; a large copy 5.2; two or four groups of rows to a workgroup 10.4
-// and 9.8, but 2,000 rows 4.1 and 4.5 for 3.9), back to bf16 11.3, 301 x 1,000 fp16 2.2, any launch's.
+// and 9.8, but 2,000 rows 4.1 and 4.5 for 3.9; 16-bit pairs never unpacked 10.3), back to bf16 8.4 (11.4 with codes decoded by
+// shifts), 301 x 1,000 fp16 2.2, any launch's.
 #include "exl3_kernels.h"
 #include "fp4_rows.cuh"
 
@@ -47,14 +48,9 @@ __global__ void __launch_bounds__(kRowsThreads) fp4_dequant_kernel(Fp4DequantArg
     const uint32_t byte = A.s[(size_t)b * A.s_stage + (size_t)row * 8 + i / 4];
     // (2^-127, byte 0, is below fp32's normal values)
     const float s = __builtin_bit_cast(float, byte == 255u ? 0x7FC00000u : byte ? byte << 23 : 1u << 22);
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t code = u >> 4 * j & 15u, e = code >> 1 & 3u, m = code & 1u;
-        // (1 + m / 2) 2^(e - 1), or m / 2 for e = 0
-        const float a = __builtin_bit_cast(float, (e + 126u) << 23 | m << 22);
-        v[j] = (code & 8u ? -1.0f : 1.0f) * (e ? a : 0.5f * (float)m) * s;
-    }
+    const auto v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 1);
+    const auto v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 3);
+    const float v[8] = {v0[0] * s, v0[1] * s, v1[0] * s, v1[1] * s, v2[0] * s, v2[1] * s, v3[0] * s, v3[1] * s};
     store8<DT, WIDE>(A.out, (size_t)row * A.k + c, n, v);
 }
 

@@ -157,6 +157,23 @@ def test_quant_every_half_step():
     assert torch.equal(_fp4().dequant(q, s, torch.float32, 32)[0], x[0]) and (s[0, 0, 0] == 127).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quant_every_16_bit_value(dtype):
+    """Every finite value of the type, next to block maxima from its own size to 64 times it, and by itself; the same in fp32."""
+    v = torch.arange(1 << 16, device="cuda").to(torch.uint16).view(dtype)
+    v = v[v.isfinite()]
+    for up in (1, 2, 3, 6, 7, 24, 64):
+        x = v.view(-1, 16).repeat_interleave(2, 1)
+        x[:, 1::2] = (x[:, ::2].float() * up).to(dtype)      # a maximum beside each: some other value's blocks, some its own
+        x = torch.cat([x, torch.stack([v, (v.float() * up).to(dtype)], 1).repeat(1, 16)])
+        x = x[x.isfinite().all(1)]
+        q, s = _fp4().quant(x)
+        rq, rs = _quant_ref(x.double())
+        assert torch.equal(s, rs) and torch.equal(q, rq)
+        q2, s2 = _fp4().quant(x.float())
+        assert torch.equal(q2, q) and torch.equal(s2, s)
+
+
 def test_quant_infinities_nan_and_extremes():
     x = torch.randn(10, 400, generator=_gen(3), device="cuda")
     x[0, 5] = math.inf
@@ -176,6 +193,11 @@ def test_quant_infinities_nan_and_extremes():
     fine = [3, 4, 5, 6, 8, 9]
     rq, rs = _quant_ref(x[fine].double())
     assert torch.equal(q[fine], rq) and torch.equal(s[fine], rs)
+    for dtype in (torch.bfloat16, torch.float16):            # (the 16-bit types have a path of their own)
+        h = torch.randn(4, 96, generator=_gen(4), device="cuda").to(dtype)
+        h[0, 5], h[1, 40], h[2, 95] = math.inf, -math.inf, math.nan
+        hs = _fp4().quant(h)[1].reshape(4, -1)
+        assert hs.eq(255).nonzero().tolist() == [[0, 0], [1, 1], [2, 2]]
     assert (flat[9, :13] == 1).all() and not flat[:, 13:].any() and not q[9].any()
     back = _fp4().dequant(q, s, torch.float32, 400)
     assert back[0, :32].isnan().all() and back[0, 32:].isfinite().all() and back[7, 384:].isnan().all() and back[7, :384].isfinite().all()
