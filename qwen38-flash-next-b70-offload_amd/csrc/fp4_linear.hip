@@ -4,7 +4,7 @@
 // the one for which that is least, max(1, tiles / 256 CUs) (BM + BN), the larger one where two are equal, but for these: 128 x 64
 // only where each CU has one at most; 128 x 128 with more than one counts by the tile, since two share a CU; 256 x 256, whose
 // rounds are whole, costs a fifth more, and is for four stages of k at least, since its first loads and last stores have nothing
-// beside them (512 -> 2048, 8,192 rows: 128 x 128 13.7, 256 x 256 14.8).
+// beside them (512 -> 2048, 8,192 rows behind a gate|up product, by a kernel trace: 128 x 128 13.9 us, 256 x 256 18.3).
 //
 // Quantised rows, bf16 outputs, weights from HBM, us per call out of a graph; * is what the rule takes.
 //   4096 -> 2048, rows  100   200   400   777  1,024  1,500  2,048  4,096  8,192
@@ -20,11 +20,11 @@
 //   128 x 128           9.4  10.1* 15.7* 26.6   27.6   35.2*  46.3   89.8  159.3
 //   256 x 256          21.1  21.8  21.8  20.8*  22.1*  40.2   40.8*  65.8* 120.7*
 //
-// Few rows (fp4_few.hip) cost by what a workgroup brings in too, 14 for each 16 columns and 1 for each row (5 where it quantises them),
-// and 10 for each further fragment of columns, which leaves fewer waves to load. They take that kernel up to a cost of 50, and up to
-// 48 rows where that is three quarters of the tile's at most (4096 -> 2048: 64 rows, cost 46, 5.9 us, in tiles 6.3; 100 rows, cost 63, 6.7 and
-// 6.3; 2048 -> 12,288: 32 rows, cost 94 and 128, 6.8 and 7.3; 64 rows, 126 and 128, 8.4 and 7.2). 12 rows and fewer are quantised inside
-// (2048 -> 12,288: 12 rows 8.1 us, by a launch before it 8.6; 16 rows 9.9 and 9.1).
+// Few rows (fp4_few.hip) cost by what a workgroup brings in too, 14 for each 16 columns and 1 for each row (5 where it quantises
+// them), and 10 for each further fragment of columns, which leaves fewer waves to load. They take that kernel up to a cost of
+// 50, and up to 48 rows where that is three quarters of the tile's at most (4096 -> 2048: 64 rows, cost 46, 5.9 us, in tiles 6.3;
+// 100 rows, cost 63, 6.7 and 6.3; 2048 -> 12,288: 32 rows, cost 94 and 128, 6.8 and 7.3; 64 rows, 126 and 128, 8.4 and 7.2). 12
+// rows and fewer are quantised inside (2048 -> 12,288: 12 rows 8.1 us, by a launch before it 8.6; 16 rows 9.9 and 9.1).
 #include "fp4_tiles.cuh"
 
 namespace exl3 {
@@ -45,7 +45,8 @@ Pick pick_tile(int M, int n, int kb) {
     constexpr int kSizes[][2] = {{32, 32}, {64, 64}, {128, 64}, {128, 128}, {256, 256}};
     Pick best{kFp4Tile256, false, 0};
     for (int i = kFp4Tile32; i <= kFp4Tile256; ++i) {
-        const int64_t tiles = (int64_t)((M - 1) / kSizes[i][0] + 1) * ((n - 1) / kSizes[i][1] + 1), rounds = (tiles + kCus - 1) / kCus;
+        const int64_t tiles = (int64_t)((M - 1) / kSizes[i][0] + 1) * ((n - 1) / kSizes[i][1] + 1);
+        const int64_t rounds = (tiles + kCus - 1) / kCus;
         const int rows = kSizes[i][0] + kSizes[i][1];
         int64_t cost = rounds * rows;
         if (i == kFp4Tile128x64 && rounds > 1) continue;
@@ -68,7 +69,8 @@ FewTile pick_few(int M, int n, bool own) {
     for (int tn = 1; tn <= 3; ++tn)
         for (int groups = 1; groups <= 4 && groups <= M; groups *= 2) {
             const int R = (M + groups - 1) / groups;
-            const int64_t workgroups = (int64_t)((n - 1) / (16 * tn) + 1) * ((M - 1) / R + 1), rounds = (workgroups + kCus - 1) / kCus;
+            const int64_t workgroups = (int64_t)((n - 1) / (16 * tn) + 1) * ((M - 1) / R + 1);
+            const int64_t rounds = (workgroups + kCus - 1) / kCus;
             if (R > (own ? 16 : 48) || (workgroups + 7) * 1024 >= kMaxThreads) continue;
             const int64_t cost = rounds * (14 * tn + (own ? 5 * R : R)) + (own ? 0 : 10 * (tn - 1));
             if (!best.tn || cost < best.cost) best = {tn, R, cost};

@@ -11,8 +11,8 @@
 // random codes draw: MFMAs alone reach 6.4 of 9.5 PFLOP/s with them). About 42 us of it are the 201 MB of outputs, which all CUs
 // store at the same time; a stage of 256 columns takes 1.6 us, 0.85 of them MFMAs at the full clock. 8,192 columns: 357 us, 4.6
 // PFLOP/s. Measured and not kept: half of a tile's outputs held in registers and stored under the next tile's products (129 us for
-// 123: the wait for a stage's loads waits for the stores before them too; with waits that leave the stores out 143, as the registers that
-// they wait in cost others), starts at different times (130 for 134).
+// 123: the wait for a stage's loads waits for the stores before them too; with waits that leave the stores out 143, as the
+// registers that they wait in cost others), starts at different times (130 for 134).
 #include "fp4_tiles.cuh"
 
 namespace exl3 {
@@ -57,8 +57,10 @@ __global__ void __launch_bounds__(256, 1) fp4_tile256_kernel(Fp4ProductArgs A, i
         else {
             // (the first two of a wave's four are the weights')
             const int j = i - 2 * kCode, si = (j & 1) * NW + wv;
-            if (j < 2) to_lds<4>(st.sw + si * 256, buffer_of(A.sw + ((size_t)b * A.n + of.n0) * 8, (uint32_t)of.cols * 8), si * 256 + l * 4, 0);
-            else to_lds<4>(st.sq + si * 256, buffer_of(A.s + (size_t)b * A.s_stage + (size_t)of.m0 * 8, (uint32_t)of.rows * 8), si * 256 + l * 4, 0);
+            const uint8_t* sw = A.sw + ((size_t)b * A.n + of.n0) * 8;
+            const uint8_t* sq = A.s + (size_t)b * A.s_stage + (size_t)of.m0 * 8;
+            if (j < 2) to_lds<4>(st.sw + si * 256, buffer_of(sw, (uint32_t)of.cols * 8), si * 256 + l * 4, 0);
+            else to_lds<4>(st.sq + si * 256, buffer_of(sq, (uint32_t)of.rows * 8), si * 256 + l * 4, 0);
         }
     };
 
@@ -68,8 +70,12 @@ __global__ void __launch_bounds__(256, 1) fp4_tile256_kernel(Fp4ProductArgs A, i
     for (int j = 0; j < 4; ++j) at[j] = r * 128 + piece_at(r, j * 2 + h) * 16;
     v4i wf[2][T], qf[2][T];
     int sw[2][T], sq[2][T];
-    auto read_w = [&](const Fp4Stage<B, B>& st, int j, int i, int to) { wf[to][i] = *(const v4i*)(st.w + (wn + i * 32) * 128 + at[j]); };
-    auto read_q = [&](const Fp4Stage<B, B>& st, int j, int i, int to) { qf[to][i] = *(const v4i*)(st.q + (wm + i * 32) * 128 + at[j]); };
+    auto read_w = [&](const Fp4Stage<B, B>& st, int j, int i, int to) {
+        wf[to][i] = *(const v4i*)(st.w + (wn + i * 32) * 128 + at[j]);
+    };
+    auto read_q = [&](const Fp4Stage<B, B>& st, int j, int i, int to) {
+        qf[to][i] = *(const v4i*)(st.q + (wm + i * 32) * 128 + at[j]);
+    };
     auto read_scales = [&](const Fp4Stage<B, B>& st, int keep, int to) {
 #pragma unroll
         for (int i = 0; i < T; ++i) {
@@ -236,7 +242,8 @@ __global__ void __launch_bounds__(256, 1) fp4_tile256_kernel(Fp4ProductArgs A, i
                             hold(j, i);
                             hold(j, i + 1);
 #pragma unroll
-                            for (int b = 0; b < 8; ++b) *(v4u*)(o + er * 128 + (b ^ (er & 7)) * 16 + eh * 8) = narrow4<DT>(four(j, i + b / 4, b & 3));
+                            for (int b = 0; b < 8; ++b)
+                                *(v4u*)(o + er * 128 + (b ^ (er & 7)) * 16 + eh * 8) = narrow4<DT>(four(j, i + b / 4, b & 3));
                             store(j, tile.n0 + wn + i * 32, full);
                         }
                     }

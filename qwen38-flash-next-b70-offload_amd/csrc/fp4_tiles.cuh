@@ -3,8 +3,8 @@
 //
 // One MFMA (32 x 32 x 64, both operands e2m1 with a scale byte per lane) takes two blocks of 32 with their scales. Its products are
 // exact and its sums keep the bits that fp32 additions in a row would: against 64 bits, random scales 2^-7 to 2^7 and 4,096
-// columns, 1.312e-7 of the outputs' norm, a chain of fp32 additions of exact block sums 1.311e-7; scales 2^-3 to 2^3, 0. So outputs of
-// every type come from it. It runs at 7.5 PFLOP/s on random codes (8.9 on zeros); 16 x 16 x 128 at 4.3, as with e4m3.
+// columns, 1.312e-7 of the outputs' norm, a chain of fp32 additions of exact block sums 1.311e-7; scales 2^-3 to 2^3, 0. So
+// outputs of every type come from it. It runs at 7.5 PFLOP/s on random codes (8.9 on zeros); 16 x 16 x 128 at 4.3, as with e4m3.
 //
 // The weights are the MFMA's A operand and the rows its B operand, so a lane's accumulators are fours of neighbouring
 // columns of one row.
@@ -60,7 +60,8 @@ __device__ __forceinline__ void silu_block(const Fp4ProductArgs& A, const float 
     for (int c = 0; c < 16; ++c) amax = max(amax, abs_bits(v[c]));
     amax = max(amax, __float_as_uint(lane_xor(__uint_as_float(amax), 32)));
     const uint32_t scale = fp4_scale_byte(amax);
-    const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}, hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
+    const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+    const float hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
     const uint32_t own[2] = {pack_e2m1(lo, scale), pack_e2m1(hi, scale)};       // 16 bits of each b
     // the lower lane takes the first 8 bytes of the block, the upper one the last
     const uint32_t other = __float_as_uint(lane_xor(__uint_as_float(h ? own[0] : own[1]), 32));
@@ -114,8 +115,10 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
         else if (i < kW + kQ) to_lds<16>(st.q + ((i - kW) * NW + wv) * 1024, qb, off[i], b * 128);
         else {
             const int si = ((i - kW - kQ) * NW + wv) % kScales, sr = si - BN / 32;
-            if (si < BN / 32) to_lds<4>(st.sw + si * 256, buffer_of(A.sw + ((size_t)b * A.n + n0) * 8, (uint32_t)cols * 8), si * 256 + l * 4, 0);
-            else to_lds<4>(st.sq + sr * 256, buffer_of(A.s + (size_t)b * A.s_stage + (size_t)m0 * 8, (uint32_t)rows * 8), sr * 256 + l * 4, 0);
+            const uint8_t* sw = A.sw + ((size_t)b * A.n + n0) * 8;
+            const uint8_t* sq = A.s + (size_t)b * A.s_stage + (size_t)m0 * 8;
+            if (si < BN / 32) to_lds<4>(st.sw + si * 256, buffer_of(sw, (uint32_t)cols * 8), si * 256 + l * 4, 0);
+            else to_lds<4>(st.sq + sr * 256, buffer_of(sq, (uint32_t)rows * 8), sr * 256 + l * 4, 0);
         }
     };
 
@@ -165,8 +168,9 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
 #pragma unroll
             for (int j = 0; j < TM; ++j)
 #pragma unroll
-                for (int i = 0; i < TN; ++i) acc[j][i] = fp4_mfma<J>(fp4_operand(wf[X][i]), fp4_operand(qf[X][j]), acc[j][i], sw[i], sq[j]);
-            // (the MFMAs of a step stay in it: nothing else holds them to their place; in the registers that the compiler would choose)
+                for (int i = 0; i < TN; ++i)
+                    acc[j][i] = fp4_mfma<J>(fp4_operand(wf[X][i]), fp4_operand(qf[X][j]), acc[j][i], sw[i], sq[j]);
+            // (the MFMAs of a step stay in it: nothing else holds them to their place; in the registers that the compiler chooses)
 #pragma unroll
             for (int j = 0; j < TM; ++j)
 #pragma unroll
@@ -280,8 +284,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
 template <bool SILU, int BM, int BN, int WM, int WN, int KG, int ST>
 void launch_fp4_tiles(const Fp4ProductArgs& a, int out_dt, hipStream_t st) {
     const int mt = (a.M - 1) / BM + 1, nt = (a.n - 1) / BN + 1, per = (int)(((int64_t)mt * nt + 7) / 8);
-    hipLaunchKernelGGL((fp4_tile_kernel<SILU, BM, BN, WM, WN, KG, ST>), dim3((unsigned)per * 8), dim3(64 * WM * WN * KG), 0, st, a, mt,
-                       nt, per, out_dt);
+    hipLaunchKernelGGL((fp4_tile_kernel<SILU, BM, BN, WM, WN, KG, ST>), dim3((unsigned)per * 8), dim3(64 * WM * WN * KG), 0,
+                       st, a, mt, nt, per, out_dt);
 }
 
 }  // namespace exl3

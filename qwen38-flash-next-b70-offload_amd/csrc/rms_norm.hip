@@ -24,7 +24,8 @@ constexpr int kThreads = 256;
 
 __device__ __forceinline__ double lane_xor64(double v, int m) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __float_as_uint(lane_xor(__uint_as_float((uint32_t)u), m)), hi = __float_as_uint(lane_xor(__uint_as_float((uint32_t)(u >> 32)), m));
+    const uint32_t lo = __float_as_uint(lane_xor(__uint_as_float((uint32_t)u), m));
+    const uint32_t hi = __float_as_uint(lane_xor(__uint_as_float((uint32_t)(u >> 32)), m));
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
@@ -207,8 +208,8 @@ void launch_rows(const RmsNormArgs& a, hipStream_t st) {
     // (8 workgroups per CU, each with every 2,048th row: as many as are there at a time, and the weights are loaded once; 8,192 x
     // 2,048 bf16 to bf16 23.9 us, a workgroup for every row 26.1)
     const int64_t all = (int64_t)(a.M - 1) / kRows + 1, most = C > 0 ? kCus * 8 : all;
-    hipLaunchKernelGGL((rms_norm_kernel<DT, RDT, WIDE, T, C>), dim3((unsigned)(all < most ? all : most)), dim3(T < kThreads ? kThreads : T), 0,
-                       st, a);
+    hipLaunchKernelGGL((rms_norm_kernel<DT, RDT, WIDE, T, C>), dim3((unsigned)(all < most ? all : most)),
+                       dim3(T < kThreads ? kThreads : T), 0, st, a);
 }
 
 template <int DT, int RDT, bool WIDE>

@@ -701,7 +701,8 @@ struct Fp4Rows {
         const auto want = fp4_scale_strides(q_.sizes().slice(0, d), rows);
         M = (int)rows;
         const bool one = s_.size(d) == 1;
-        bool fits = s_.stride(d + 1) == 1 && (one || (s_.stride(d) >= want[d] && s_.stride(d) % 8 == 0)) && (uintptr_t)s_.const_data_ptr() % 8 == 0;
+        bool fits = s_.stride(d + 1) == 1 && (one || (s_.stride(d) >= want[d] && s_.stride(d) % 8 == 0)) &&
+                    (uintptr_t)s_.const_data_ptr() % 8 == 0;
         for (int64_t i = 0; i < d; ++i) fits = fits && (s_.size(i) == 1 || s_.stride(i) == want[i]);
         s = s_;
         if (!fits && M > 0) {
