@@ -410,14 +410,14 @@ int exl3_fp8_mlp(const void* x, int dtype, int64_t x_stride, int M, int k, int I
 /* ---- the norm, and the 4-bit float linear (none of these has a counterpart in the reference's op libraries) ----------- */
 
 /* h = x + residual, added in fp32 and rounded to the residual's type (x itself without a residual); y = h / sqrt(mean(h^2) +
- * eps) * weight in 64 bits, rounded to 32 once. x: [M, k] of x_dtype, row m at (m / inner) * x_outer + (m %
- * inner) * x_stride elements (inner 1: at m * x_stride). residual: x_dtype or fp32, or NULL; held: h, [M, k] of the residual's type, which may be the residual itself (NULL
- * without one). weight: fp32 [k] or NULL. y: [M, k] of x_dtype, or NULL. form 1: q and s as exl3_fp8_quant's, form 2: as
+ * eps) * weight (1 + weight with unit_offset) in 64 bits, rounded to 32 once. x: [M, k] of x_dtype, row m at (m / inner) * x_outer
+ * + (m % inner) * x_stride elements (inner 1: at m * x_stride). residual: x_dtype or fp32, or NULL; held: h, [M, k] of the
+ * residual's type, which may be the residual itself (NULL without one). weight: fp32 [k] or NULL. y: [M, k] of x_dtype, or NULL. form 1: q and s as exl3_fp8_quant's, form 2: as
  * exl3_fp4_quant's (s_stage as there), both of the norm before it is rounded to x_dtype; 0: none. At least one of y and a form. eps
  * is positive. An infinite element gives NaN and 0 in the rest of its row, a NaN a row of NaN. k <= 2^22 and, by k, up to 2^22 rows. */
 int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64_t x_outer, const void* residual,
-                  int residual_dtype, int64_t residual_stride, void* held, const float* weight, float eps, int M, int k,
-                  void* y, int form, void* q, void* s, int64_t s_stage, void* stream);
+                  int residual_dtype, int64_t residual_stride, void* held, const float* weight, int unit_offset, float eps,
+                  int M, int k, void* y, int form, void* q, void* s, int64_t s_stage, void* stream);
 
 /* Rows of microscaled 4-bit floats (OCP MX: e2m1 with one power of two per 32 columns): scale 2^(floor(log2(amax)) - 2), 2^-126
  * at the least, quotients rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, halves to even, 6 at the most. x: [M, k] of

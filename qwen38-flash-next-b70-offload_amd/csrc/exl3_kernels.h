@@ -344,6 +344,7 @@ struct RmsNormArgs {
     const void* x; int64_t x_stride, x_outer; int inner;
     const void* res; int64_t res_stride; void* held;   // null: no residual; held [M, k] of its type
     const float* w;                                // [k] or null
+    int unit_offset;                               // times 1 + w
     float eps;
     double inv_k;                                  // 1 / k
     int M, k;

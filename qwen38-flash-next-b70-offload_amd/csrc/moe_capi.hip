@@ -1615,8 +1615,8 @@ int fp4_mlp_checks(const char* what, int M, int k, int I, int n, const void* gu,
 }  // namespace
 
 int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64_t x_outer, const void* residual,
-                  int residual_dtype, int64_t residual_stride, void* held, const float* weight, float eps, int M, int k,
-                  void* y, int form, void* q, void* s, int64_t s_stage, void* stream) {
+                  int residual_dtype, int64_t residual_stride, void* held, const float* weight, int unit_offset, float eps,
+                  int M, int k, void* y, int form, void* q, void* s, int64_t s_stage, void* stream) {
     const char* what = "rms_norm";
     if (int r = fp4_dims(what, M, k, 1)) return r;
     if (!dt_ok(x_dtype)) return fail(EXL3_EINVAL, "%s: dtype %d", what, x_dtype);
@@ -1631,6 +1631,7 @@ int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64
     if (!residual != !held) return fail(EXL3_EINVAL, "%s: residual and held come together", what);
     if (residual && (residual_stride < k || !aligned(residual, dt_size(residual_dtype)) || !aligned(held, dt_size(residual_dtype))))
         return fail(EXL3_EINVAL, "%s: alignment of residual or held, or row stride %lld", what, (long long)residual_stride);
+    if (unit_offset && !weight) return fail(EXL3_EINVAL, "%s: unit_offset without a weight", what);
     if (!aligned(weight, 4) || !aligned(y, dt_size(x_dtype))) return fail(EXL3_EINVAL, "%s: alignment", what);
     if (!y && form == kFormNone) return fail(EXL3_EINVAL, "%s: no output", what);
     if (form == kFormFp8 && (!q || !s || !aligned(q, 16) || !aligned(s, 4)))
@@ -1648,6 +1649,7 @@ int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64
     a.res_stride = residual_stride;
     a.held = held;
     a.w = weight;
+    a.unit_offset = unit_offset != 0;
     a.eps = eps;
     a.inv_k = 1.0 / k;
     a.M = M;

@@ -115,13 +115,16 @@ struct Row {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = (WIDE ? 0 : j) < n ? v[j] : 0.0f;
     }
-    // w: the weights of these columns, 0 behind the row
+    // (weights that are held in 32 bits get their 1 here: 1 + w has more bits than they)
+    __device__ __forceinline__ double gain(double w) const { return w; }
+    __device__ __forceinline__ double gain(float w) const { return (double)w + A.unit_offset; }
+    // w: the weights of these columns
     template <class W>
     __device__ __forceinline__ void out(int c, float (&v)[8], double by, const W (&w)[8]) const {
         const int n = A.k - c;
         double t[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = (WIDE ? 0 : j) < n ? (double)v[j] * by * (double)w[j] : 0.0;
+        for (int j = 0; j < 8; ++j) t[j] = (WIDE ? 0 : j) < n ? (double)v[j] * by * gain(w[j]) : 0.0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
         if (A.y && n > 0) store8<DT, WIDE>(A.y, (size_t)m * A.k + c, n, v);
@@ -149,7 +152,10 @@ __device__ __forceinline__ void weights(const RmsNormArgs& A, int c, W (&w)[8]) 
     float f[8] = {1, 1, 1, 1, 1, 1, 1, 1};
     if (A.w) load8<2, WIDE>(A.w, n > 0 ? c : 0, max(n, 1), f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = f[j];
+    for (int j = 0; j < 8; ++j) {
+        w[j] = f[j];
+        if constexpr (sizeof(W) == 8) w[j] += A.unit_offset;
+    }
 }
 
 template <int DT, int RDT, bool WIDE, int T, int C>

@@ -895,12 +895,13 @@ std::vector<at::Tensor> rms_norm_empty(const at::Tensor& x, const std::optional<
 }
 
 std::vector<at::Tensor> rms_norm_meta(const at::Tensor& x, const std::optional<at::Tensor>& residual,
-                                      const std::optional<at::Tensor>&, double, int64_t form, bool rows) {
+                                      const std::optional<at::Tensor>&, double, int64_t form, bool rows, bool) {
     return rms_norm_empty(x, residual, form, rows);
 }
 
 std::vector<at::Tensor> rms_norm(const at::Tensor& x, const std::optional<at::Tensor>& residual,
-                                 const std::optional<at::Tensor>& weight, double eps, int64_t form, bool rows) {
+                                 const std::optional<at::Tensor>& weight, double eps, int64_t form, bool rows,
+                                 bool unit_offset) {
     const c10::DeviceGuard guard(x.device());
     no_gradients(x, "rms_norm");
     const int dt = dtype_code(x);
@@ -934,7 +935,7 @@ std::vector<at::Tensor> rms_norm(const at::Tensor& x, const std::optional<at::Te
     auto ptr = [&](size_t i) { return out[i].data_ptr(); };
     const size_t y = form ? 2 : 0, held = y + rows;
     check(exl3_rms_norm(x2.const_data_ptr(), dt, stride, (int)inner, outer, residual ? r2.const_data_ptr() : nullptr, rdt,
-                        residual ? row_stride(r2) : 0, residual ? ptr(held) : nullptr, w, (float)eps, M, (int)k,
+                        residual ? row_stride(r2) : 0, residual ? ptr(held) : nullptr, w, unit_offset, (float)eps, M, (int)k,
                         rows ? ptr(y) : nullptr, (int)form, form ? ptr(0) : nullptr, form ? ptr(1) : nullptr, 8 * (int64_t)M,
                         cur_stream(x)),
           "rms_norm");
@@ -975,7 +976,8 @@ TORCH_LIBRARY(exl3xpu_C, m) {
     m.def("fp8_matmul(Tensor q, Tensor s, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType dtype) -> Tensor");
     m.impl("fp8_matmul", c10::DispatchKey::CUDA, &fp8_matmul);
     m.impl("fp8_matmul", c10::DispatchKey::Meta, &fp8_matmul_meta);
-    m.def("rms_norm(Tensor x, Tensor? residual, Tensor? weight, float eps, int form, bool rows) -> Tensor[]");
+    m.def("rms_norm(Tensor x, Tensor? residual, Tensor? weight, float eps, int form, bool rows, bool unit_offset=False) -> "
+          "Tensor[]");
     m.impl("rms_norm", c10::DispatchKey::CUDA, &rms_norm);
     m.impl("rms_norm", c10::DispatchKey::Meta, &rms_norm_meta);
     m.def("fp4_quant(Tensor x) -> (Tensor q, Tensor s)");

@@ -93,7 +93,7 @@ SIGNATURES = {
     "exl3_fp8_mlp_workspace": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32]),
     "exl3_fp8_mlp": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_p,
                              c_sz, c_p]),
-    "exl3_rms_norm": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i64, c_p, c_i32, c_i64, c_p, c_p, ctypes.c_float, c_i32, c_i32, c_p,
+    "exl3_rms_norm": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i64, c_p, c_i32, c_i64, c_p, c_p, c_i32, ctypes.c_float, c_i32, c_i32, c_p,
                               c_i32, c_p, c_p, c_i64, c_p]),
     "exl3_fp4_quant": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_p, c_p, c_i64, c_p]),
     "exl3_fp4_silu_mul_quant": (c_i32, [c_p, c_i32, c_i64, c_i32, c_i32, c_p, c_p, c_i64, c_p]),

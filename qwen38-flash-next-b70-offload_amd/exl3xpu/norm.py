@@ -27,8 +27,8 @@ _FORMS = {"fp8": 1, "fp4": 2}
 
 class RmsNorm:
     def __init__(self, weight: torch.Tensor | None = None, eps: float = 1e-6, unit_offset: bool = False, device=None):
-        """weight: [k] or None, kept as fp32 on `device` (its own by default); with unit_offset the norm is multiplied by 1 + weight.
-        Raises ValueError on arguments that no rows could go with."""
+        """weight: [k] or None, kept as fp32 on `device` (its own by default); with unit_offset the norm is multiplied by 1 + weight,
+        which is added in 64 bits. Raises ValueError on arguments that no rows could go with."""
         if weight is not None and (weight.dim() != 1 or not weight.numel()):
             raise ValueError(f"exl3xpu: weight [k], got {tuple(weight.shape)}")
         if not 2.0 ** -126 <= eps <= 3.0e38:
@@ -36,18 +36,17 @@ class RmsNorm:
         if unit_offset and weight is None:
             raise ValueError("exl3xpu: unit_offset without a weight")
         if weight is not None:
-            weight = weight.detach().to(weight.device if device is None else torch.device(device), torch.float32)
-            weight = (weight + 1 if unit_offset else weight).contiguous()
-        self.weight, self.eps = weight, float(eps)
+            weight = weight.detach().to(weight.device if device is None else torch.device(device), torch.float32).contiguous()
+        self.weight, self.eps, self.unit_offset = weight, float(eps), bool(unit_offset)
         self._op = _C().rms_norm.default
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         """x [..., k] fp16 / bf16 / fp32 -> y, or (y, h) with a residual [..., k]."""
-        out = self._op(x, residual, self.weight, self.eps, 0, True)
+        out = self._op(x, residual, self.weight, self.eps, 0, True, self.unit_offset)
         return out[0] if residual is None else tuple(out)
 
     def quant(self, x: torch.Tensor, residual: torch.Tensor | None = None, form: str = "fp8", rows: bool = False):
         """-> (q, s) in the form "fp8" or "fp4", then y with rows=True, then h with a residual."""
         if form not in _FORMS:
             raise ValueError(f"exl3xpu: form 'fp8' or 'fp4', got {form!r}")
-        return tuple(self._op(x, residual, self.weight, self.eps, _FORMS[form], rows))
+        return tuple(self._op(x, residual, self.weight, self.eps, _FORMS[form], rows, self.unit_offset))

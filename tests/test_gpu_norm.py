@@ -261,12 +261,34 @@ def test_c_abi_in_place_and_what_is_behind():
         s = torch.full((-(-k // 256), M + 3, 8), 99, dtype=torch.uint8, device="cuda")
         last = res[M].clone()
         print(f"case norm c-abi k={k}", flush=True)
-        capi.check(L.exl3_rms_norm(x.data_ptr(), 1, k + 8, 1, 0, res.data_ptr(), 2, k, res.data_ptr(), norm.weight.data_ptr(), EPS,
-                                   M, k, y.data_ptr(), 2, q.data_ptr(), s.data_ptr(), 8 * (M + 3), st))
+        capi.check(L.exl3_rms_norm(x.data_ptr(), 1, k + 8, 1, 0, res.data_ptr(), 2, k, res.data_ptr(), norm.weight.data_ptr(), 0,
+                                   EPS, M, k, y.data_ptr(), 2, q.data_ptr(), s.data_ptr(), 8 * (M + 3), st))
         torch.cuda.synchronize()
         assert torch.equal(q[:M], want[0]) and torch.equal(s[:, :M].movedim(0, 1), want[1]) and torch.equal(y[:M], want[2])
         assert torch.equal(res[:M], want[3]) and torch.equal(res[M], last)
         assert (y[M:] == 7).all() and (q[M:] == 99).all() and (s[:, M:] == 99).all()
+
+
+@pytest.mark.parametrize("k", [100, 128, 1000, 2048, 2049, 5000, 9000, 40000])
+def test_unit_offset(k):
+    """1 + weight is not rounded: fp32 rows are off by their own rounding, 2^-24, and 2^-44; and no e4m3 value is on the wrong side
+    of a border that the norm rounded to 32 bits and its quotient do not come within 2^-40 of."""
+    g = _gen(31 * k)
+    for M in (1, 600):
+        x = torch.randn(M, k, generator=g, device="cuda")
+        weight = 0.2 * torch.randn(k, generator=g, device="cuda")
+        norm = _norm()(weight, EPS, unit_offset=True)
+        print(f"case norm unit_offset k={k} M={M}", flush=True)
+        y = norm(x)
+        q, s, h = norm.quant(x.bfloat16(), x)
+        torch.cuda.synchronize()
+        ref = _ref(x, 1 + weight.double())
+        assert ((y.double() - ref).abs() <= _units(k) * 2.0 ** -24 * ref.abs() + 2.0 ** -149).all()
+        ref = _ref(h, 1 + weight.double())
+        _check_fp8(q, s, ref, k)
+        quo = (torch.nn.functional.pad(ref, (0, -k % 128)).view(M, -1, 128) / s.double()[..., None]).view(M, -1)
+        lo, hi = (_e4m3((quo * f).float().double()) for f in (1 - 2.0 ** -40, 1 + 2.0 ** -40))
+        assert ((q.double() == lo) | (q.double() == hi)).all()
 
 
 def test_rows_past_32_bits():

@@ -10,8 +10,8 @@ P = 1 << 20                                     # an address that no refused cal
 
 
 def _norm(x=P, dtype=1, stride=256, inner=1, outer=0, res=P, rdt=1, rs=256, held=P, w=P, eps=1e-6, M=2, k=256, y=P, form=0,
-          q=None, s=None, stage=0):
-    return capi.lib().exl3_rms_norm(x, dtype, stride, inner, outer, res, rdt, rs, held, w, eps, M, k, y, form, q, s, stage, None)
+          q=None, s=None, stage=0, unit=0):
+    return capi.lib().exl3_rms_norm(x, dtype, stride, inner, outer, res, rdt, rs, held, w, unit, eps, M, k, y, form, q, s, stage, None)
 
 
 @pytest.mark.parametrize("k,code", [
@@ -212,4 +212,5 @@ def test_classes_refuse():
         with pytest.raises(ValueError):
             bad()
     n = norm.RmsNorm(torch.tensor([0.0, 0.5], dtype=torch.bfloat16), unit_offset=True)
-    assert n.weight.dtype == torch.float32 and n.weight.tolist() == [1.0, 1.5]
+    assert n.weight.dtype == torch.float32 and n.weight.tolist() == [0.0, 0.5] and n.unit_offset
+    assert _norm(w=None, unit=1) == BAD
