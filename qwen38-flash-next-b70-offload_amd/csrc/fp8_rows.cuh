@@ -69,18 +69,27 @@ __device__ __forceinline__ float silu_times_far(float g, float u) {
     return g * h * u * __builtin_fmaf(h, -x.e * kLn2, h);
 }
 
-// 8 consecutive elements of a row as fp32. WIDE: 16-byte aligned and all inside the row; else one by one, from the `n`-th on
-// (n > 0) the last one again
+// 16 bytes at a multiple of 16, 4 or 2 (one load or store takes any address)
+typedef uint32_t Bytes16 __attribute__((ext_vector_type(4)));
+typedef uint32_t Bytes16At4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t Bytes16At2 __attribute__((ext_vector_type(4), aligned(2)));
+template <int DT, bool WIDE>
+using RowBytes = std::conditional_t<WIDE, Bytes16, std::conditional_t<DT == 2, Bytes16At4, Bytes16At2>>;
+
+// 8 consecutive elements of a row as fp32. WIDE: 16-byte aligned and all inside the row; else at any element, from the `n`-th on
+// (n > 0) the last one again, and one by one where n < 8
 template <int DT, bool WIDE>
 __device__ __forceinline__ void load8(const void* x, size_t at, int n, float (&v)[8]) {
-    if constexpr (WIDE) {
+    using B = RowBytes<DT, WIDE>;
+    if (WIDE || n >= 8) {
         if constexpr (DT == 2) {
-            const float4* p = (const float4*)((const float*)x + at);
-            const float4 a = p[0], b = p[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            const B* p = (const B*)((const float*)x + at);
+            const B a = p[0], b = p[1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(a[j]), v[4 + j] = __uint_as_float(b[j]);
         } else {
-            const uint4 r = *(const uint4*)((const uint16_t*)x + at);
-            const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+            const B r = *(const B*)((const uint16_t*)x + at);
+            const uint32_t u[4] = {r[0], r[1], r[2], r[3]};          // (a bit cast of a vector's element takes its first one)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (DT == 0) {
@@ -104,14 +113,20 @@ __device__ __forceinline__ void load8(const void* x, size_t at, int n, float (&v
     }
 }
 
-// 8 consecutive elements of a row as DT. WIDE as above; else the first `n` of them one by one
+// 8 consecutive elements of a row as DT. WIDE as above; else at any element the first `n` of them
 template <int DT, bool WIDE>
 __device__ __forceinline__ void store8(void* y, size_t at, int n, const float (&v)[8]) {
+    using B = RowBytes<DT, WIDE>;
     if constexpr (DT == 2) {
         float* p = (float*)y + at;
-        if constexpr (WIDE) {
-            ((float4*)p)[0] = {v[0], v[1], v[2], v[3]};
-            ((float4*)p)[1] = {v[4], v[5], v[6], v[7]};
+        if (WIDE || n >= 8) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                B b;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] = __builtin_bit_cast(uint32_t, v[j * 4 + i]);
+                ((B*)p)[j] = b;
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -122,8 +137,11 @@ __device__ __forceinline__ void store8(void* y, size_t at, int n, const float (&
 #pragma unroll
         for (int j = 0; j < 8; ++j) u[j] = DT == 0 ? __builtin_bit_cast(uint16_t, (_Float16)v[j]) : __builtin_bit_cast(uint16_t, (__bf16)v[j]);
         uint16_t* p = (uint16_t*)y + at;
-        if constexpr (WIDE) {
-            *(uint4*)p = {u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16, u[6] | (uint32_t)u[7] << 16};
+        if (WIDE || n >= 8) {
+            B b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = u[2 * j] | (uint32_t)u[2 * j + 1] << 16;
+            *(B*)p = b;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
