@@ -11,7 +11,9 @@
 //
 // Bound by memory, few rows by a launch and one chain of loads. us per call out of a graph, bf16 with a bf16 residual: 1 x 2,048 to
 // e4m3 2.6, 8,192 x 2,048 to bf16 24.0 (134 MB, 5.6 TB/s), to e4m3 27.2 (117 MB, 4.3 TB/s), to e2m1 23.3; 8,192 x 4,096 to bf16
-// 44.5; 1,500 x 16 heads of 128 4.9.
+// 44.5; 1,500 x 16 heads of 128 4.9. Rows of any size, with nothing but their elements aligned: 3,962 x 2,883 fp16 with an fp32
+// residual to e4m3 35.4 (126 MB; 75 with elements one by one and their places held in registers), 2,000 x 8,192 28.5 (115 MB), x
+// 8,191 34.4, x 20,000 89, x 20,001 96 (239 and 461 where the registers did not hold the weights and places too).
 #include "exl3_kernels.h"
 #include "fp4_rows.cuh"
 
@@ -164,20 +166,25 @@ __global__ void __launch_bounds__(T < kThreads ? kThreads : T) rms_norm_kernel(R
     // (4-bit rows have whole stages of scales)
     const int i = threadIdx.x % T, ks = A.form == kFormFp4 ? fp4_stages(A.k) * kFp4Stage : fp4_cols(A.k);
     if constexpr (C > 0) {
-        // (weights of one or two chunks in the 64 bits that they are used in)
-        std::conditional_t<C <= 2, double, float> w[C][8];
+        // (weights of one or two chunks stay in the 64 bits that they are used in; those of four would not fit beside the row)
+        constexpr bool kKept = C <= 2;
+        std::conditional_t<kKept, double, float> w[kKept ? C : 1][8];
+        if constexpr (kKept)
 #pragma unroll
-        for (int c = 0; c < C; ++c) weights<WIDE>(A, (c * T + i) * 8, w[c]);
+            for (int c = 0; c < C; ++c) weights<WIDE>(A, (c * T + i) * 8, w[c]);
         // (whole rows of T threads; the same number of turns for all threads of a row)
         for (int64_t m = (int64_t)blockIdx.x * kRows + threadIdx.x / T; m < A.M; m += (int64_t)gridDim.x * kRows) {
             const Row<DT, RDT, WIDE> row(A, m);
+            // (kept from being taken out of the loop over the rows: the elements' places, which would fill the registers)
+            int at = i * 8;
+            if constexpr (!WIDE || !kKept) asm volatile("" : "+v"(at));
             double sum = 0;
             float v[C][8];
 #pragma unroll
             for (int c = 0; c < C; ++c) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[c][j] = 0;
-                if (c == 0 || c * T * 8 < ks) row.load((c * T + i) * 8, v[c]);
+                if (c == 0 || c * T * 8 < ks) row.load(c * T * 8 + at, v[c]);
             }
 #pragma unroll
             for (int c = 0; c < C; ++c)
@@ -186,7 +193,13 @@ __global__ void __launch_bounds__(T < kThreads ? kThreads : T) rms_norm_kernel(R
             const double by = root_inverse(row_sum<T>(sum) * A.inv_k + (double)A.eps);
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                if (c == 0 || c * T * 8 < ks) row.out((c * T + i) * 8, v[c], by, w[c]);
+                if (c == 0 || c * T * 8 < ks) {
+                    if constexpr (!kKept) {
+                        __builtin_amdgcn_sched_barrier(0);           // (a chunk at a time)
+                        weights<WIDE>(A, c * T * 8 + at, w[0]);
+                    }
+                    row.out(c * T * 8 + at, v[c], by, w[kKept ? c : 0]);
+                }
             if constexpr (T > 64) __syncthreads();   // (the sum's LDS is used again)
         }
     } else {
