@@ -217,11 +217,11 @@ __global__ void __launch_bounds__(64 * NW) fp4_few_kernel(Fp4ProductArgs A, int 
 #pragma unroll
         for (int i = 0; i < NW; ++i) v += sums[i][f][l];
         v += bias[o];
-        const bool whole = n + 4 <= A.n && A.out_stride % 4 == 0;
+        const bool whole = n + 4 <= A.n;             // (at any element: one store takes them)
         const size_t at = (size_t)(mb + m) * A.out_stride + n;
         if (out_dt == 2) {
             float* p = (float*)A.out + at;
-            if (whole && (uintptr_t)A.out % 16 == 0) *(v4f*)p = v;
+            if (whole) *(Bytes16At4*)p = __builtin_bit_cast(Bytes16, v);
             else
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(64 * NW) fp4_few_kernel(Fp4ProductArgs A, int 
         } else {
             const v4u u = out_dt == 0 ? narrow4<0>(v) : narrow4<1>(v);
             uint16_t* p = (uint16_t*)A.out + at;
-            if (whole && (uintptr_t)A.out % 8 == 0) *(v4u*)p = u;
+            if (whole) *(Bytes8At2*)p = __builtin_bit_cast(Bytes8, u);
             else
 #pragma unroll
                 for (int c = 0; c < 4; ++c)

@@ -226,8 +226,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
         return;
     }
     if (out_dt == 2) {
-        // a lane's four columns at once where they are there and every row's fours start on 16 bytes
-        const bool wide = A.n % 4 == 0 && A.out_stride % 4 == 0 && (uintptr_t)A.out % 16 == 0;
+        // a lane's four columns at once where they are there
 #pragma unroll
         for (int j = 0; j < TM; ++j)
 #pragma unroll
@@ -238,7 +237,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
                     const v4f v = four(j, i, b);
                     if (n >= A.n || m >= A.M) continue;
                     float* p = (float*)A.out + (size_t)m * A.out_stride + n;
-                    if (wide) *(v4f*)p = v;
+                    if (n + 4 <= A.n) *(Bytes16At4*)p = __builtin_bit_cast(Bytes16, v);
                     else
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
@@ -265,7 +264,6 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
     else to_out(std::integral_constant<int, 1>());
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const bool wide = A.out_stride % 8 == 0 && (uintptr_t)A.out % 16 == 0;
 #pragma unroll
     for (int k = 0; k < TM * 32 * kPieces / 64; ++k) {
         const int at = k * 64 + l, row = at / kPieces, piece = at % kPieces;
@@ -273,7 +271,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) fp4_tile_kernel(Fp4ProductA
         if (m >= A.M || n >= A.n) continue;
         const v8u v = *(const v8u*)(o + (row * kPieces + (piece ^ (row & (kPieces - 1)))) * 8);
         uint16_t* p = (uint16_t*)A.out + (size_t)m * A.out_stride + n;
-        if (wide && n + 8 <= A.n) *(v8u*)p = v;
+        if (n + 8 <= A.n) *(Bytes16At2*)p = __builtin_bit_cast(Bytes16, v);
         else
 #pragma unroll
             for (int c = 0; c < 8; ++c)

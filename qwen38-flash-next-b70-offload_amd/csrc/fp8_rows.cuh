@@ -73,6 +73,8 @@ __device__ __forceinline__ float silu_times_far(float g, float u) {
 typedef uint32_t Bytes16 __attribute__((ext_vector_type(4)));
 typedef uint32_t Bytes16At4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t Bytes16At2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t Bytes8 __attribute__((ext_vector_type(2)));
+typedef uint32_t Bytes8At2 __attribute__((ext_vector_type(2), aligned(2)));
 template <int DT, bool WIDE>
 using RowBytes = std::conditional_t<WIDE, Bytes16, std::conditional_t<DT == 2, Bytes16At4, Bytes16At2>>;
 

@@ -289,6 +289,33 @@ def test_linear_larger(M, n, k):
         assert torch.equal(lin(x), y)                        # the same sums in the same order
 
 
+@pytest.mark.parametrize("M,n,k", [(2200, 4099, 1100), (4100, 4097, 1030), (8192, 2307, 1024), (600, 2051, 700), (300, 1003, 500),
+                                   (40, 2049, 900), (3, 1005, 600)])
+def test_outputs_at_any_element(M, n, k):
+    """Rows of outputs that start at odd elements, in the kernels of few rows, of tiles and of 256 x 256 ones; nothing outside them
+    is written."""
+    from exl3xpu import capi
+    L, st = capi.lib(), torch.cuda.current_stream().cuda_stream
+    g = _gen(M + 3 * n)
+    w, sw = _weight(g, n, k)
+    bias = torch.randn(n, generator=g, device="cuda")
+    for lin in (_linear(w, sw), _linear(w, sw, bias)):
+        for code, dtype in ((0, torch.float16), (1, torch.bfloat16), (2, torch.float32)):
+            print(f"case fp4 odd outputs M={M} n={n} k={k} {dtype} bias={lin.bias is not None}", flush=True)
+            x = torch.randn(M, k, generator=g, device="cuda").to(dtype)
+            y = lin(x)
+            torch.cuda.synchronize()
+            _check_product(y, _values(*_quant_ref(x.double()), k), w, sw, lin.bias)
+            q, s = _fp4().quant(x)
+            store = torch.full((M * (n + 2) + 5,), 9.0, dtype=dtype, device="cuda")
+            out = store[1:1 + M * (n + 2)].view(M, n + 2)
+            capi.check(L.exl3_fp4_matmul(q.data_ptr(), s.data_ptr(), 8 * M, M, 2 * q.size(1), n, lin.weight.data_ptr(),
+                                         lin.weight_scale.data_ptr(), None if lin.bias is None else lin.bias.data_ptr(),
+                                         out.data_ptr(), code, n + 2, st))
+            torch.cuda.synchronize()
+            assert torch.equal(out[:, :n], y) and (out[:, n:] == 9).all() and store[0] == 9 and (store[-4:] == 9).all()
+
+
 @pytest.mark.parametrize("n,k,Ms", [(2000, 1300, (33, 40, 47, 64, 90, 100, 127, 300)), (2050, 4000, (17, 64, 97, 128)),
                                     (1990, 640, (770, 1000, 1090, 1500, 2200)), (5000, 2048, (1, 3, 4, 5, 8, 16, 17, 32, 33)),
                                     (1000, 4096, (1, 2, 3, 4, 5, 16, 17, 31)), (1100, 1152, (80, 2030)), (12200, 200, (100, 1100)),
