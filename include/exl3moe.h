@@ -412,9 +412,11 @@ int exl3_fp8_mlp(const void* x, int dtype, int64_t x_stride, int M, int k, int I
 /* h = x + residual, added in fp32 and rounded to the residual's type (x itself without a residual); y = h / sqrt(mean(h^2) +
  * eps) * weight (1 + weight with unit_offset) in 64 bits, rounded to 32 once. x: [M, k] of x_dtype, row m at (m / inner) * x_outer
  * + (m % inner) * x_stride elements (inner 1: at m * x_stride). residual: x_dtype or fp32, or NULL; held: h, [M, k] of the
- * residual's type, which may be the residual itself (NULL without one). weight: fp32 [k] or NULL. y: [M, k] of x_dtype, or NULL. form 1: q and s as exl3_fp8_quant's, form 2: as
- * exl3_fp4_quant's (s_stage as there), both of the norm before it is rounded to x_dtype; 0: none. At least one of y and a form. eps
- * is positive. An infinite element gives NaN and 0 in the rest of its row, a NaN a row of NaN. k <= 2^22 and, by k, up to 2^22 rows. */
+ * residual's type (NULL without one), which may be the residual itself where that has its rows next to each other
+ * (residual_stride k, or one row) and lies on it in no other way; other outputs lie on no input. weight: fp32 [k] or NULL. y:
+ * [M, k] of x_dtype, or NULL. form 1: q and s as exl3_fp8_quant's, form 2: as exl3_fp4_quant's (s_stage as there), both of the
+ * norm before it is rounded to x_dtype; 0: none. At least one of y and a form. eps is positive. An infinite element gives NaN and
+ * 0 in the rest of its row, a NaN a row of NaN. k <= 2^22 and, by k, up to 2^22 rows. */
 int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64_t x_outer, const void* residual,
                   int residual_dtype, int64_t residual_stride, void* held, const float* weight, int unit_offset, float eps,
                   int M, int k, void* y, int form, void* q, void* s, int64_t s_stage, void* stream);

@@ -1612,6 +1612,15 @@ int fp4_mlp_checks(const char* what, int M, int k, int I, int n, const void* gu,
     return EXL3_OK;
 }
 
+// whether rows that are written, [M, k] next to each other, lie on rows that are read, `stride` elements apart, other than element
+// for element on the same place
+bool rows_over_others(const void* to, const void* from, int64_t stride, int M, int k, size_t size) {
+    const __int128 each = (__int128)k * size, step = (__int128)stride * size, at = (__int128)(uintptr_t)to - (uintptr_t)from;
+    if (at == 0 && (M == 1 || stride == k)) return false;
+    const __int128 r = at < each ? 0 : (at - each) / step + 1;       // the first row that ends behind `to`
+    return r < M && r * step < at + M * each;
+}
+
 }  // namespace
 
 int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64_t x_outer, const void* residual,
@@ -1631,6 +1640,8 @@ int exl3_rms_norm(const void* x, int x_dtype, int64_t x_stride, int inner, int64
     if (!residual != !held) return fail(EXL3_EINVAL, "%s: residual and held come together", what);
     if (residual && (residual_stride < k || !aligned(residual, dt_size(residual_dtype)) || !aligned(held, dt_size(residual_dtype))))
         return fail(EXL3_EINVAL, "%s: alignment of residual or held, or row stride %lld", what, (long long)residual_stride);
+    if (residual && rows_over_others(held, residual, residual_stride, M, k, dt_size(residual_dtype)))
+        return fail(EXL3_EINVAL, "%s: held over other elements of the residual (row stride %lld)", what, (long long)residual_stride);
     if (unit_offset && !weight) return fail(EXL3_EINVAL, "%s: unit_offset without a weight", what);
     if (!aligned(weight, 4) || !aligned(y, dt_size(x_dtype))) return fail(EXL3_EINVAL, "%s: alignment", what);
     if (!y && form == kFormNone) return fail(EXL3_EINVAL, "%s: no output", what);

@@ -30,6 +30,25 @@ def test_norm_refuses(k, code):
     assert not code or capi.lib().exl3_last_error()
 
 
+@pytest.mark.parametrize("size", [2, 4])
+def test_norm_refuses_a_held_sum_over_other_elements_of_its_residual(size):
+    """Where an element of the held sum lies on another one's residual, it is written while that one is still read: refused, and
+    only there, against a search of all pairs of rows. (Every call has an output that is refused later: none is launched.)"""
+    k, a = 256, 1 << 30
+    seen = set()
+    for M in (1, 2, 3, 5):
+        for rs in (k, k + 8, k + 1, 2 * k, 3 * k, 8 * k):
+            for at in (0, 1, -1, k, -k, k // 2, rs, rs - k, (M - 1) * rs, (M - 1) * rs + k, (M - 1) * rs + k - 1, -M * k, -M * k + 1,
+                       1 - rs, rs * M, M * k):
+                meet = any(at + m * k < r * rs + k and r * rs < at + m * k + k for m in range(M) for r in range(M))
+                bad = meet and not (at == 0 and (M == 1 or rs == k))
+                dt = 1 if size == 2 else 2
+                assert _norm(dtype=dt, stride=k, res=a, rdt=dt, rs=rs, held=a + at * size, M=M, k=k, y=P + 1) == BAD
+                assert (b"held over" in capi.lib().exl3_last_error()) == bad, (M, rs, at)
+                seen.add((meet, bad))
+    assert seen == {(False, False), (True, False), (True, True)}
+
+
 def _rows(f, x=P, dtype=1, stride=256, M=2, k=256, q=P, s=P, stage=16):
     return getattr(capi.lib(), f)(x, dtype, stride, M, k, q, s, stage, None)
 
