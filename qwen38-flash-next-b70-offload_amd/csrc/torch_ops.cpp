@@ -648,9 +648,20 @@ at::Tensor fp8_matmul_meta(const at::Tensor& q, const at::Tensor&, const at::Ten
 
 // ---- the norm and the 4-bit float linear of exl3xpu_C (no counterpart in the reference) ---------------------------------
 
-void no_gradients(const at::Tensor& x, const char* what) {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), what,
-                ": no gradients; detach the input or call it under torch.no_grad()");
+// The operators' autograd kernel: they are for inference. It stands above the device's kernels, where torch.func's transforms show
+// their tensors too (below, those are plain ones); tangents count whether gradients are on or not, as torch.no_grad leaves them.
+void no_gradients(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+    const bool grad = at::GradMode::is_enabled(), tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const c10::IValue& v : torch::jit::last(stack, op.schema().arguments().size())) {
+        if (!v.isTensor() || !v.toTensor().defined()) continue;
+        const at::Tensor& t = v.toTensor();
+        if ((grad && t.requires_grad()) || (tangents && t._fw_grad(0).defined())) {
+            const std::string& name = op.schema().name();
+            TORCH_CHECK(false, name.substr(name.rfind(':') + 1),
+                        ": no gradients; detach the inputs, or call it under torch.no_grad() where they have no tangents");
+        }
+    }
+    op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
 }
 
 int64_t fp4_stages(int64_t k) { return (k + 255) / 256; }
@@ -718,7 +729,6 @@ std::tuple<at::Tensor, at::Tensor> fp4_silu_mul_quant_meta(const at::Tensor& x) 
 
 std::tuple<at::Tensor, at::Tensor> fp4_quant(const at::Tensor& x) {
     const c10::DeviceGuard guard(x.device());
-    no_gradients(x, "fp4_quant");
     const int dt = dtype_code(x);
     auto x2 = rows_of(x, "fp4_quant");
     auto out = fp4_rows_empty(x, x.size(-1));
@@ -730,7 +740,6 @@ std::tuple<at::Tensor, at::Tensor> fp4_quant(const at::Tensor& x) {
 
 std::tuple<at::Tensor, at::Tensor> fp4_silu_mul_quant(const at::Tensor& x) {
     const c10::DeviceGuard guard(x.device());
-    no_gradients(x, "fp4_silu_mul_quant");
     const int dt = dtype_code(x);
     auto x2 = rows_of(x, "fp4_silu_mul_quant");
     TORCH_CHECK(x2.size(1) % 2 == 0, "fp4_silu_mul_quant: gate|up rows of an even size, got ", x.sizes());
@@ -777,7 +786,6 @@ at::Tensor fp4_linear_meta(const at::Tensor& x, const at::Tensor& w, const at::T
 
 at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sw, const std::optional<at::Tensor>& bias) {
     const c10::DeviceGuard guard(x.device());
-    no_gradients(x, "fp4_linear");
     const int dt = dtype_code(x);
     auto x2 = rows_of(x, "fp4_linear");
     const int M = (int)x2.size(0), k = (int)x2.size(1);
@@ -834,7 +842,6 @@ at::Tensor fp4_mlp(const at::Tensor& x, int64_t I, const at::Tensor& gu, const a
                    const std::optional<at::Tensor>& gu_bias, const at::Tensor& dn, const at::Tensor& dn_scale,
                    const std::optional<at::Tensor>& dn_bias) {
     const c10::DeviceGuard guard(x.device());
-    no_gradients(x, "fp4_mlp");
     const int dt = dtype_code(x);
     auto x2 = rows_of(x, "fp4_mlp");
     const int M = (int)x2.size(0), k = (int)x2.size(1);
@@ -903,7 +910,6 @@ std::vector<at::Tensor> rms_norm(const at::Tensor& x, const std::optional<at::Te
                                  const std::optional<at::Tensor>& weight, double eps, int64_t form, bool rows,
                                  bool unit_offset) {
     const c10::DeviceGuard guard(x.device());
-    no_gradients(x, "rms_norm");
     const int dt = dtype_code(x);
     auto out = rms_norm_empty(x, residual, form, rows);
     const int64_t k = x.size(-1);
@@ -911,7 +917,6 @@ std::vector<at::Tensor> rms_norm(const at::Tensor& x, const std::optional<at::Te
     int rdt = dt;
     at::Tensor r2;
     if (residual) {
-        no_gradients(*residual, "rms_norm");
         on_device_of(x, *residual, "rms_norm");
         TORCH_CHECK(residual->sizes() == x.sizes(), "rms_norm: residual ", x.sizes(), ", got ", residual->sizes());
         rdt = dtype_code(*residual);
@@ -1003,6 +1008,9 @@ TORCH_LIBRARY(exl3xpu_C, m) {
           "Tensor down_scale, Tensor? down_bias, ScalarType dtype) -> Tensor");
     m.impl("fp4_mlp_matmul", c10::DispatchKey::CUDA, &fp4_mlp_matmul);
     m.impl("fp4_mlp_matmul", c10::DispatchKey::Meta, &fp4_mlp_matmul_meta);
+    for (const char* name : {"rms_norm", "fp4_quant", "fp4_silu_mul_quant", "fp4_dequant", "fp4_linear", "fp4_matmul", "fp4_mlp",
+                             "fp4_mlp_matmul"})
+        m.impl(name, c10::DispatchKey::Autograd, torch::CppFunction::makeFromBoxedFunction<&no_gradients>());
 }
 
 TORCH_LIBRARY(exl3xpu_moe, m) {

@@ -14,8 +14,9 @@ q is uint8 [..., kp / 2] with kp = k rounded up to 128: two codes to a byte, the
 + 127 of the scale of columns 256 b + 32 j to 256 b + 32 j + 31 (255: NaN; 0 behind k); in memory the stages b are outermost. The
 scale is 2^(floor(log2(amax)) - 2), 2^-126 at the least; x / scale is rounded to the nearest code, halves to even, 6 at the most. A
 block with an infinite or NaN element is NaN. Calls run on the device's current stream, keep no state and can be captured into a
-graph. They are for inference: inputs that require gradients are refused. How many rows a call has picks the order of a
-product's sums: a row alone and the same row in a batch may differ in the last bits.
+graph. They are for inference: inputs that require gradients (while gradients are on) or carry tangents are refused, and weights and
+biases are detached when a linear is made, so that parameters given to it get no gradients. How many rows a call has picks the order
+of a product's sums: a row alone and the same row in a batch may differ in the last bits.
 """
 from __future__ import annotations
 

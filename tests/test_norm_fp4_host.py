@@ -233,3 +233,50 @@ def test_classes_refuse():
     n = norm.RmsNorm(torch.tensor([0.0, 0.5], dtype=torch.bfloat16), unit_offset=True)
     assert n.weight.dtype == torch.float32 and n.weight.tolist() == [0.0, 0.5] and n.unit_offset
     assert _norm(w=None, unit=1) == BAD
+
+
+def _differentiable():
+    """(operator's name, its call, a floating-point input) for every operator and every such input of it."""
+    def t(*size, dtype=torch.float32):
+        return torch.empty(*size, device="meta", dtype=dtype)
+    x, r, w = t(2, 300), t(2, 300), t(300)
+    q, s, b = t(2, 192, dtype=torch.uint8), t(2, 2, 8, dtype=torch.uint8), t(130)
+    c, sc = t(130, 192, dtype=torch.uint8), t(2, 130, 8, dtype=torch.uint8).movedim(0, 1)
+    gu, gs, gb = t(768, 192, dtype=torch.uint8), t(2, 768, 8, dtype=torch.uint8).movedim(0, 1), t(768)
+    ops, f32 = C(), torch.float32
+    yield from (("rms_norm", lambda v, i=i: ops.rms_norm(*[v if j == i else a for j, a in enumerate((x, r, w))], 1e-6, 2, True), a)
+                for i, a in enumerate((x, r, w)))
+    yield "fp4_quant", lambda v: ops.fp4_quant(v), x
+    yield "fp4_silu_mul_quant", lambda v: ops.fp4_silu_mul_quant(v), x
+    yield "fp4_linear", lambda v: ops.fp4_linear(v, c, sc, b), x
+    yield "fp4_linear", lambda v: ops.fp4_linear(x, c, sc, v), b
+    yield "fp4_matmul", lambda v: ops.fp4_matmul(q, s, c, sc, v, f32), b
+    yield "fp4_mlp", lambda v: ops.fp4_mlp(v, 300, gu, gs, gb, c, sc, b), x
+    yield "fp4_mlp", lambda v: ops.fp4_mlp(x, 300, gu, gs, v, c, sc, b), gb
+    yield "fp4_mlp", lambda v: ops.fp4_mlp(x, 300, gu, gs, gb, c, sc, v), b
+    yield "fp4_mlp_matmul", lambda v: ops.fp4_mlp_matmul(q, s, 300, gu, gs, v, c, sc, b, f32), gb
+    yield "fp4_mlp_matmul", lambda v: ops.fp4_mlp_matmul(q, s, 300, gu, gs, gb, c, sc, v, f32), b
+
+
+def test_no_input_loses_its_gradient_or_tangent():
+    """Rows, residuals, weights and biases that need a gradient, or carry a tangent, are refused, in torch.func's transforms too; a
+    result without them would be taken for a constant."""
+    def first(out):
+        return out if torch.is_tensor(out) else out[0]
+    for name, f, a in _differentiable():
+        def refused(call, f=f, name=name):
+            with pytest.raises(RuntimeError, match=f"{name}: no gradients"):
+                call(f)
+        first(f(a))
+        refused(lambda f: f(a.clone().requires_grad_()))
+        with torch.no_grad():
+            first(f(a.clone().requires_grad_()))
+        with torch.inference_mode():
+            first(f(a))
+        with torch.autograd.forward_ad.dual_level():
+            refused(lambda f: f(torch.autograd.forward_ad.make_dual(a, torch.ones_like(a))))
+            with torch.no_grad():                            # (it stops no tangents)
+                refused(lambda f: f(torch.autograd.forward_ad.make_dual(a, torch.ones_like(a))))
+            first(f(a))
+        refused(lambda f: torch.func.jvp(lambda v: first(f(v)), (a,), (torch.ones_like(a),)))
+        refused(lambda f: torch.func.grad(lambda v: first(f(v)).float().sum())(a))
