@@ -765,3 +765,30 @@ def test_products_of_every_code_and_sums_that_cancel(M, n, k):
             fits = ref.abs() + tol < torch.finfo(dtype).max
             assert fits.all() if dtype != torch.float16 else fits.sum() > 50
             assert ((y.double() - ref).abs() <= tol)[fits].all()
+
+
+# (gate|up in 128 x 128 tiles, one to a CU at most and more; in 256 x 256 ones, one to a workgroup and several; each with an I whose
+# last 128 columns are half a stage, one that ends inside a block, ragged rows)
+@pytest.mark.parametrize("M,k,I,n", [(2000, 512, 1000, 260), (2000, 1100, 640, 130), (4100, 512, 1000, 260), (8190, 1024, 640, 130),
+                                     (8190, 1100, 1000, 260), (16001, 1024, 1000, 260)])
+def test_mlp_of_prompts(M, k, I, n):  # noqa: E741
+    fp4, g = _fp4(), _gen(61 + M)
+    gu, dn = _weight(g, 2 * I, k), _weight(g, n, I)
+    for bias in (False, True):
+        b = [torch.randn(c, generator=g, device="cuda") if bias else None for c in (2 * I, n)]
+        mlp = fp4.Fp4Mlp(fp4.Fp4Linear(*gu, b[0]), fp4.Fp4Linear(*dn, b[1]))
+        x = torch.randn(M, k, generator=g, device="cuda").bfloat16()
+        for dtype in DTYPES:
+            print(f"case fp4 mlp of prompts M={M} k={k} I={I} bias={bias} {dtype}", flush=True)
+            y = mlp.quantised(*fp4.quant(x), dtype)
+            torch.cuda.synchronize()
+            _check_mlp(y, x, gu, dn, b, k, I)
+            if dtype == x.dtype:
+                assert torch.equal(mlp(x), y)
+                want = y
+        bad = torch.tensor([0, 31, 32, 130, 255, 256, M // 2, M - 1], device="cuda")
+        x[bad[::2], k - 1] = math.nan
+        x[bad[1::2], 0] = math.inf
+        y = mlp(x)
+        rows = torch.ones(M, dtype=torch.bool, device="cuda").index_fill(0, bad, False)
+        assert y[bad].isnan().all() and torch.equal(y[rows], want[rows])
