@@ -336,3 +336,29 @@ def test_refusals():
         assert torch.equal(norm(x.clone().requires_grad_()), norm(x))
     with pytest.raises(NotImplementedError):
         _norm()(None, EPS)(x.cpu())
+
+
+# (as many columns as 16, 64, 256 and 1,024 threads hold in one, two and four chunks of a row, aligned and not)
+@pytest.mark.parametrize("k", [128, 250, 1000, 2048, 2047, 4096, 8191, 9000, 9001])
+def test_rows_in_a_loop(k):
+    """More rows than workgroups, so that one takes several in turn: of magnitudes 2^-30 to 2^30 that differ from row to row, none may
+    see anything of the ones before it."""
+    M, eps = 5003 if k > 1024 else 40_003, 2.0 ** -40                # (an eps that fp32 holds)
+    g = _gen(13 * k)
+    norm = _norm()(torch.randn(k, generator=g, device="cuda") + 1, eps)
+    for dtype in (torch.float32, torch.bfloat16):
+        scale = torch.exp2(torch.randint(-30, 31, (M, 1), generator=g, device="cuda").float())
+        x, res = ((torch.randn(M, k, generator=g, device="cuda") * t).to(dtype) for t in (scale, scale.flip(0)))
+        print(f"case norm rows in a loop k={k} {dtype}", flush=True)
+        outs = [norm.quant(x, res, form, rows=True) for form in ("fp8", "fp4")]
+        y = norm(x)
+        torch.cuda.synchronize()
+        h = _held(x, res)
+        for a in range(0, M, 1000):
+            at = slice(a, a + 1000)
+            _check_rows(y[at], _ref(x[at], norm.weight, eps), k)
+            ref = _ref(h[at], norm.weight, eps)
+            for (q, s, y2, h2), check in zip(outs, (_check_fp8, _check_fp4)):
+                assert torch.equal(h2[at], h[at])
+                check(q[at], s[at], ref, k)
+                _check_rows(y2[at], ref, k)
