@@ -3,8 +3,13 @@
 // What takes the time is what a CU has to bring in (fp8_linear.hip has the rates): BM + BN rows of k for each tile. The tile is
 // the one for which that is least, max(1, tiles / 256 CUs) (BM + BN), the larger one where two are equal, but for these: 128 x 64
 // only where each CU has one at most; 128 x 128 with more than one counts by the tile, since two share a CU; 256 x 256, whose
-// rounds are whole, costs a fifth more, and is for four stages of k at least, since its first loads and last stores have nothing
-// beside them (512 -> 2048, 8,192 rows behind a gate|up product, by a kernel trace: 128 x 128 13.9 us, 256 x 256 18.3).
+// rounds are whole, costs a fifth more, and for a gate|up product is for four stages of k at least: silu and the rows' conversion,
+// with no products beside them, are as much work as fewer stages' products. MLPs of 8,192 rows out of a graph, both forms on one
+// card, us with gate|up in tiles of 128 x 128 and of 256 x 256: 512 -> 2 x 1024 26.0 and 29.1, 768 -> 2 x 2048 50.0 and 54.5.
+// Plain products take them with fewer stages too:
+//   rows, k -> n   4,096, 128 -> 4096   8,192, 256 -> 2048   8,192, 512 -> 2048   2,048, 512 -> 12,288   8,192, 768 -> 12,288
+//   128 x 128                    12.9                 11.9                 13.6                   19.7                   88.7
+//   256 x 256                    10.9                 11.1                 12.8                   19.3                   64.3
 //
 // Quantised rows, bf16 outputs, weights from HBM, us per call out of a graph; * is what the rule takes.
 //   4096 -> 2048, rows  100   200   400   777  1,024  1,500  2,048  4,096  8,192
@@ -41,7 +46,7 @@ struct Pick {
     bool few;                                        // at most one workgroup per CU
     int64_t cost;
 };
-Pick pick_tile(int M, int n, int kb) {
+Pick pick_tile(int M, int n, int kb, bool silu) {
     constexpr int kSizes[][2] = {{32, 32}, {64, 64}, {128, 64}, {128, 128}, {256, 256}};
     Pick best{kFp4Tile256, false, 0};
     for (int i = kFp4Tile32; i <= kFp4Tile256; ++i) {
@@ -51,7 +56,7 @@ Pick pick_tile(int M, int n, int kb) {
         int64_t cost = rounds * rows;
         if (i == kFp4Tile128x64 && rounds > 1) continue;
         if (i == kFp4Tile128 && rounds > 1) cost = tiles * rows / kCus;
-        if (i == kFp4Tile256 && kb < 4 && best.cost) continue;
+        if (i == kFp4Tile256 && silu && kb < 4 && best.cost) continue;
         if (i == kFp4Tile256) cost = rounds * (rows + rows / 5);
         else if ((tiles + 7) * 512 >= kMaxThreads) continue;
         if (!best.cost || cost <= best.cost) best = {i, rounds == 1, cost};
@@ -105,7 +110,7 @@ bool fp4_product_quantises(int M, int, int) { return M <= kOwnRows; }
 
 hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t st) {
     const FewTile f = pick_few(a.M, a.n, !a.q);
-    const Pick p = pick_tile(a.M, a.n, a.kb);
+    const Pick p = pick_tile(a.M, a.n, a.kb, false);
     const bool few = f.tn && (f.cost <= 50 || (a.M <= 48 && f.cost * 4 <= p.cost * 3));
     if (!a.q || a.M <= kOwnRows || few) launch_fp4_few(a, f.tn, f.R, out_dt, st);
     else launch_tile<false>(p, a, out_dt, st);
@@ -115,7 +120,7 @@ hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t s
 bool fp4_gate_up_in_tiles(int M) { return M > kOwnRows; }
 
 hipError_t launch_fp4_gate_up(const Fp4ProductArgs& a, hipStream_t st) {
-    launch_tile<true>(pick_tile(a.M, a.n, a.kb), a, 2, st);
+    launch_tile<true>(pick_tile(a.M, a.n, a.kb, true), a, 2, st);
     return hipGetLastError();
 }
 

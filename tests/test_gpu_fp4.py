@@ -792,3 +792,22 @@ def test_mlp_of_prompts(M, k, I, n):  # noqa: E741
         y = mlp(x)
         rows = torch.ones(M, dtype=torch.bool, device="cuda").index_fill(0, bad, False)
         assert y[bad].isnan().all() and torch.equal(y[rows], want[rows])
+
+
+# (256 x 256 tiles of one to three stages of k, one to a workgroup and several, the last stage a half one and ending inside a block)
+@pytest.mark.parametrize("M,k,n", [(8192, 128, 2048), (8150, 100, 2047), (8150, 256, 2048), (4100, 250, 12287), (8192, 512, 2048),
+                                   (8150, 384, 4090), (16001, 300, 2048), (8150, 768, 2047), (2040, 640, 12288)])
+def test_products_of_few_stages(M, k, n):
+    g = _gen(71 + M + k)
+    w = _weight(g, n, k)
+    x = torch.randn(M, k, generator=g, device="cuda")
+    x[M // 3] = 0
+    q, s = _fp4().quant(x)
+    xv = _values(q, s, k)
+    for bias in (None, torch.randn(n, generator=g, device="cuda")):
+        lin = _linear(*w, bias)
+        for dtype in DTYPES:
+            print(f"case fp4 products of few stages M={M} k={k} n={n} bias={bias is not None} {dtype}", flush=True)
+            y = lin.quantised(q, s, dtype)
+            torch.cuda.synchronize()
+            _check_product(y, xv, *w, bias)
