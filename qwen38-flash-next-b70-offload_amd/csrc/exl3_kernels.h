@@ -328,7 +328,7 @@ struct Fp4ProductArgs {
 };
 hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t st);
 // whether the product quantises its rows itself (no launch_fp4_rows before it)
-bool fp4_product_quantises(int M, int k, int n);
+bool fp4_product_quantises(int M);
 static inline bool fp4_rows_wide(const void* x, int64_t x_stride, int k, int x_dt) {
     const int size = x_dt == 2 ? 4 : 2;
     return (uintptr_t)x % (4 * size) == 0 && x_stride % 4 == 0 && k % 4 == 0;

@@ -106,7 +106,7 @@ void launch_tile(const Pick& p, const Fp4ProductArgs& a, int out_dt, hipStream_t
 
 }  // namespace
 
-bool fp4_product_quantises(int M, int, int) { return M <= kOwnRows; }
+bool fp4_product_quantises(int M) { return M <= kOwnRows; }
 
 hipError_t launch_fp4_product(const Fp4ProductArgs& a, int out_dt, hipStream_t st) {
     const FewTile f = pick_few(a.M, a.n, !a.q);

@@ -1548,7 +1548,7 @@ Fp4ProductArgs fp4_args(const void* q, const void* s, int64_t s_stage, int M, in
 int fp4_quantised(const char* what, Fp4ProductArgs& a, const void* x, int x_dtype, int64_t x_stride, int k, uint8_t* q, void* stream) {
     if (!x || x_stride < k || !aligned(x, dt_size(x_dtype)))
         return fail(EXL3_EINVAL, "%s: x null, its alignment or row stride %lld", what, (long long)x_stride);
-    if (fp4_product_quantises(a.M, k, a.n)) {
+    if (fp4_product_quantises(a.M)) {
         a.x = x;
         a.x_stride = x_stride;
         a.k = k;
@@ -1711,7 +1711,7 @@ int exl3_fp4_matmul(const void* q, const void* s, int64_t s_stage, int M, int k,
 
 // The quantised rows; none for few rows, which the product quantises itself
 size_t exl3_fp4_linear_workspace(int M, int k, int n) {
-    if (M <= 0 || k <= 0 || n <= 0 || fp4_product_quantises(M, k, n)) return 0;
+    if (M <= 0 || k <= 0 || n <= 0 || fp4_product_quantises(M)) return 0;
     return fp4_rows_bytes(M, k);
 }
 
