@@ -1,6 +1,6 @@
-// The 4-bit float product of few rows (fp4_tiles.cuh has the definition): 16 columns to a workgroup, whose waves share the stages
-// of 256 columns of k among them, so that no two waves need the same operands: they go from memory straight to registers, and a
-// wave's loads are all under way at once. The waves' sums join in LDS, in the waves' order.
+// The 4-bit float product of few rows (fp4_tiles.cuh has the definition): 16 to 48 columns to a workgroup, whose waves share the
+// stages of 256 columns of k among them, so that no two waves need the same operands: they go from memory straight to registers,
+// and a wave's loads are all under way at once. The waves' sums join in LDS, in the waves' order.
 //
 // A lane's 16 bytes of an MFMA (16 x 16 x 128) are one block of 32 of one row, and its scale is one byte. Rows that are not
 // quantised yet (x, or the gates and ups of a gated MLP) are quantised by each wave for its own stages, in LDS: about 0.3 us a

@@ -28,8 +28,12 @@
 // Few rows (fp4_few.hip) cost by what a workgroup brings in too, 14 for each 16 columns and 1 for each row (5 where it quantises
 // them), and 10 for each further fragment of columns, which leaves fewer waves to load. They take that kernel up to a cost of
 // 50, and up to 48 rows where that is three quarters of the tile's at most (4096 -> 2048: 64 rows, cost 46, 5.9 us, in tiles 6.3;
-// 100 rows, cost 63, 6.7 and 6.3; 2048 -> 12,288: 32 rows, cost 94 and 128, 6.8 and 7.3; 64 rows, 126 and 128, 8.4 and 7.2). 12
-// rows and fewer are quantised inside (2048 -> 12,288: 12 rows 8.1 us, by a launch before it 8.6; 16 rows 9.9 and 9.1).
+// 100 rows, cost 63, 6.7 and 6.3; 2048 -> 12,288: 32 rows, cost 94 and 128, 6.8 and 7.3). 12 rows and fewer are quantised inside
+// (2048 -> 12,288: 12 rows 8.1 us, by a launch before it 8.6; 16 rows 9.9 and 9.1).
+//
+// A gate|up product of more rows than those 12 takes a tile by the same rule, with 32 x 64 ones where it says 32 x 32 (a wave has a
+// gate and its up). They are counted as 32 x 32, which takes 64 x 64 for some calls of one round of 32 x 64: MLP of 300 rows 2048
+// -> 2 x 512 -> 2048 14.4 us, with gate|up in 32 x 64 13.3; of 300 rows 512 -> 2 x 512 -> 512 11.3 and 11.8.
 #include "fp4_tiles.cuh"
 
 namespace exl3 {

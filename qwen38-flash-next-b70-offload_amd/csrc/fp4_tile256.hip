@@ -8,12 +8,12 @@
 // two before it has been read. The next tile's first stages are on their way while this tile's outputs are stored.
 //
 // 8,192 rows, 2048 -> 12,288: 118 to 123 us (3.4-3.5 PFLOP/s; with rows and weights of zeros 97, so 20 % of it is the power that
-// random codes draw: MFMAs alone reach 6.4 of 9.5 PFLOP/s with them). About 42 us of it are the 201 MB of outputs, which all CUs
-// store at the same time; a stage of 256 columns takes 1.6 us, 0.85 of them MFMAs at the full clock. 8,192 columns: 357 us, 4.6
-// PFLOP/s. Measured and not kept: half of a tile's outputs held in registers and stored under the next tile's products (129 us for
-// 123: the wait for a stage's loads waits for the stores before them too; with waits that leave the stores out 143, as the
-// registers that they wait in cost others), starts at different times (130 for 134).
-// Rows of outputs that start at any element (12,287 columns) 142 us, 260 with their elements stored one by one.
+// random codes draw: MFMAs alone reach 6.4 to 6.6 PFLOP/s with them, 8.8 to 9.6 with zeros). About 42 us of it are the 201 MB of
+// outputs, which all CUs store at the same time; a stage of 256 columns takes 1.6 us, 0.85 of them MFMAs at the full clock. 8,192
+// columns: 357 us, 4.6 PFLOP/s. Measured and not kept: half of a tile's outputs held in registers and stored under the next
+// tile's products (129 us for 123: the wait for a stage's loads waits for the stores before them too; with waits that leave the
+// stores out 143, as the registers that they wait in cost others), starts at different times (130 for 134). Rows of outputs that
+// start at any element (12,287 columns) 142 us, 260 with their elements stored one by one.
 #include "fp4_tiles.cuh"
 
 namespace exl3 {

@@ -1,10 +1,11 @@
 // The product of the 4-bit float linear (fp4_linear.hip has the rule that picks a tile): out[m][n] = sum_k q[m][k] w[n][k], each
 // times its block's scale, + bias[n].
 //
-// One MFMA (32 x 32 x 64, both operands e2m1 with a scale byte per lane) takes two blocks of 32 with their scales. Its products are
-// exact and its sums keep the bits that fp32 additions in a row would: against 64 bits, random scales 2^-7 to 2^7 and 4,096
+// One MFMA (32 x 32 x 64, both operands e2m1 with a scale byte per lane) takes two blocks of 32 with their scales. Its products
+// are exact and its sums keep the bits that fp32 additions in a row would: against 64 bits, random scales 2^-7 to 2^7 and 4,096
 // columns, 1.312e-7 of the outputs' norm, a chain of fp32 additions of exact block sums 1.311e-7; scales 2^-3 to 2^3, 0. So
-// outputs of every type come from it. It runs at 7.5 PFLOP/s on random codes (8.9 on zeros); 16 x 16 x 128 at 4.3, as with e4m3.
+// outputs of every type come from it. From registers, 4 x 4 accumulators to a wave, it runs at 6.4 to 6.6 PFLOP/s on random codes
+// (8.8 to 9.6 on zeros); 16 x 16 x 128 at 7.5 (9.2), but takes twice the fragments' reads per product.
 //
 // The weights are the MFMA's A operand and the rows its B operand, so a lane's accumulators are fours of neighbouring
 // columns of one row.

@@ -2,12 +2,15 @@
 // y = h / sqrt(mean(h^2) + eps) * w of what is held (x itself without a residual). y leaves as rows of x's type, as e4m3 rows with
 // fp32 scales (fp8_rows.cuh's form) or as 4-bit rows (fp4_rows.cuh).
 //
-// The sum and everything behind it are computed in 64 bits and rounded to 32 once (for e4m3 only its scale and its quotient are):
-// an error of 2^-24 takes one of 10^6 values over a border between two of e4m3's. It costs 2 us of 27 at 8,192 x 2,048 to e4m3.
+// The sum and everything behind it are computed in 64 bits and rounded to 32 once, rows of 16 bits from there (for e4m3 only its
+// scale and its quotient are): an error of 2^-24 takes one of 10^6 values over a border between two of e4m3's. It costs 2 us of
+// 27 at 8,192 x 2,048 to e4m3.
 //
-// A row is held in registers between its sum and its outputs: T lanes, up to C times 8 elements each, so every input is
-// read once and every output written once. 16 lanes hold 128 neighbouring columns, which is a block of e4m3 and four of the
-// 4-bit ones. Rows of more than 32,768 columns are read again for their outputs (they were just read: from the caches).
+// A row is held in registers between its sum and its outputs: T lanes, up to C times 8 elements each, so every input is read once
+// and every output written once. 16 lanes hold 128 neighbouring columns, which is a block of e4m3 and four of the 4-bit ones.
+// Rows of more than 32,768 columns are read again for their outputs (they were just read: from the caches). Those of 8,193 to
+// 32,768 fill the 128 registers that 1,024 threads have and spill 1 to 8 more (8 to 36 bytes a lane), and a CU has one workgroup,
+// with nothing under way beside its sum's barrier: 2,000 x 20,000 at 62 % of a large copy's rate.
 //
 // Bound by memory, few rows by a launch and one chain of loads. us per call out of a graph, bf16 with a bf16 residual: 1 x 2,048 to
 // e4m3 2.6, 8,192 x 2,048 to bf16 24.0 (134 MB, 5.6 TB/s), to e4m3 27.2 (117 MB, 4.3 TB/s), to e2m1 23.3; 8,192 x 4,096 to bf16

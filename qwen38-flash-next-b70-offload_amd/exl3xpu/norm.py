@@ -7,13 +7,14 @@
   q, s, h = norm.quant(x, residual, "fp4")      as 4-bit rows, as Fp4Linear.quantised and Fp4Mlp.quantised take them
   q, s, y, h = norm.quant(x, residual, "fp8", rows=True)     y as well: the router and the EXL3 experts take it
 
-One launch, each input read once. h is added in fp32 and rounded once, to the residual's dtype (x's or fp32), and the norm is that of the
-rounded h, so that it is the same as a norm of h by itself; it is computed in 64 bits and rounded once. q, s are those of the norm before
-it is rounded to x's dtype, in the forms of exl3xpu.fp8 and exl3xpu.fp4. Rows may lie inside wider ones at a uniform stride, and x
-[tokens, heads, k] inside the rows of a fused projection. A row with an infinite element is NaN there and 0 elsewhere, one with a NaN
-element NaN. Calls run on the device's current stream, keep no state and can be captured into a graph. They are for
-inference: inputs that require gradients (while gradients are on) or carry tangents are refused, and the weight is detached when
-the norm is made, so that a parameter given to it gets no gradient.
+One launch, each input read once (rows of more than 32,768 columns again for their outputs). h is added in fp32 and rounded once,
+to the residual's dtype (x's or fp32), and the norm is that of the rounded h, so that it is the same as a norm of h by itself; it
+is computed in 64 bits, rounded to 32, and from there to x's dtype. q, s are those of the norm before it is rounded to x's dtype,
+in the forms of exl3xpu.fp8 and exl3xpu.fp4. Rows may lie inside wider ones at a uniform stride, and x [tokens, heads, k] inside
+the rows of a fused projection. A row with an infinite element is NaN there and 0 elsewhere, one with a NaN element NaN. Calls run
+on the device's current stream, keep no state and can be captured into a graph. They are for inference: inputs that require
+gradients (while gradients are on) or carry tangents are refused, and the weight is detached when the norm is made, so that a
+parameter given to it gets no gradient.
 """
 from __future__ import annotations
 
